@@ -34,8 +34,12 @@ from .api import (  # noqa: F401
     matvec_q4_0,
     matvec_q8_0,
     argmax,
+    attn_paged,
+    attn_prompt,
     lm_head_argmax_sharded,
     matvec_sharded,
+    page_plan,
+    page_store,
     quantize_model,
     quantize_row,
     quantize_rows,

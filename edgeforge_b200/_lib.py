@@ -86,6 +86,12 @@ SIGNATURES = {
     "efg_matvec_sharded": (_i, [_i, _vp, _vp, _vp, _sz, _sz, _vp, _vp]),
     "efg_argmax": (_i, [_vp, _sz, _vp, _vp]),
     "efg_lm_head_argmax_sharded": (_i, [C.c_int, _vp, _vp, _vp, _vp, _vp, C.c_float, _sz, _sz, _vp, _vp]),
+    "efg_page_plan": (_i, [_vp, _sz, _vp, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _sz, _sz, _vp]),
+    "efg_page_store": (_i, [_i, _i, _vp, _vp, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _sz, _sz,
+                            _sz, _sz, _vp]),
+    "efg_attn_prompt": (_i, [_i, _vp, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _sz, _sz, _sz, _sz, C.c_float, _vp]),
+    "efg_attn_paged": (_i, [_i, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz,
+                            C.c_float, _vp]),
     "efg_efq_check": (_i, [_vp, _u64]),
     "efg_quantize_model": (_i, [C.c_char_p, C.c_char_p, C.c_char_p, C.c_char_p, C.POINTER(QuantizeReport)]),
     "efg_decoder_open": (_i, [C.c_char_p, _sz, C.POINTER(_vp)]),

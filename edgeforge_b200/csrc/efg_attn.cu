@@ -1,0 +1,146 @@
+// efg_attn.cu - softmax attention entry points: packed prompts (efg_attn_prompt) and new tokens
+// over a paged cache (efg_attn_paged).
+//
+//   out[r][h] = sum_j w_j v[j][h / group],  w = softmax_j(scale q[r][h] . k[j][h / group])
+//
+// over the positions j that row r sees: those of its own sequence up to its own position.
+#include <type_traits>
+
+#include <cuda_runtime.h>
+
+#include "../../include/efg.h"
+#include "efg_attn.cuh"
+#include "efg_host.h"
+
+namespace efg {
+namespace {
+
+constexpr int kRowWarps = 4;
+
+// Any head size, stride and alignment: one warp per row and query head.
+template <typename T>
+__global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(const AttnParams p) {
+  __shared__ float q_s[kRowWarps][256];
+  const int warp = threadIdx.x >> 5;
+  if (blockIdx.x == 0)  // one CTA looks at every offset: a row finds its sequence by bisection and may miss a bad one
+    for (int64_t s = threadIdx.x; s < p.n_seqs; s += blockDim.x)
+      if (p.cu[s] < 0 || p.cu[s + 1] < p.cu[s] || p.cu[s + 1] > p.n_rows) record_error(p.err, EFG_EINVAL);
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * kRowWarps + warp;
+  const int64_t row = item / p.heads;
+  if (row >= p.n_rows) return;
+  const int64_t s = find_sequence(p.cu, p.n_seqs, row);
+  if (s < 0 || s >= p.n_seqs) return;  // behind the last sequence
+  Chunk c;
+  if (!chunk_of_seq(p, s, c)) return;
+  attend_row<T>(p, c, row, static_cast<int>(item % p.heads), q_s[warp]);
+}
+
+template <typename T>
+int launch_rows(const AttnParams& p, cudaStream_t s) {
+  const int64_t items = p.n_rows * p.heads, ctas = (items + kRowWarps - 1) / kRowWarps;
+  if (ctas > 0x7FFFFFFFll) return fail(EFG_EINVAL, "attention: too many rows");
+  attn_rows_kernel<T><<<static_cast<unsigned>(ctas), kRowWarps * 32, 0, s>>>(p);
+  EFG_TRY_CUDA(cudaGetLastError(), "attention launch");
+  return EFG_OK;
+}
+
+int launch_attn(int type, const AttnParams& p, cudaStream_t s) {
+  if (type == EFG_F32) return launch_rows<float>(p, s);
+  if (type == EFG_F16) return launch_rows<__half>(p, s);
+  return launch_rows<__nv_bfloat16>(p, s);
+}
+
+// The checks that both calls make; `who` names the call.
+int check_attn(const char* who, int type, size_t n_seqs, size_t n_rows, size_t heads, size_t kv_heads,
+               size_t head_dim, size_t q_stride, float scale) {
+  if (type < EFG_F32 || type > EFG_BF16) return fail(EFG_EINVAL, "%s: unknown type %d", who, type);
+  if (head_dim == 0 || head_dim > 256) return fail(EFG_EINVAL, "%s: head_dim %zu is not in 1..256", who, head_dim);
+  if (kv_heads == 0 || heads == 0 || heads > 4096 || heads % kv_heads)
+    return fail(EFG_EINVAL, "%s: %zu query heads do not divide into %zu key heads", who, heads, kv_heads);
+  if (n_rows > 0x7FFFFFFFull || n_seqs > (1ull << 24)) return fail(EFG_EINVAL, "%s: a size is out of range", who);
+  if (q_stride < heads * head_dim) return fail(EFG_EINVAL, "%s: a row stride is shorter than a row", who);
+  if (!(scale == scale) || scale - scale != 0.f) return fail(EFG_EINVAL, "%s: scale is not finite", who);
+  return EFG_OK;
+}
+
+}  // namespace
+}  // namespace efg
+
+using efg::fail;
+
+extern "C" {
+
+int efg_attn_prompt(int type, void* d_out, const void* d_q, size_t q_stride, const void* d_k, size_t k_stride,
+                    const void* d_v, size_t v_stride, const int32_t* d_cu, size_t n_seqs, size_t n_rows, size_t heads,
+                    size_t kv_heads, size_t head_dim, float scale, void* stream) {
+  if (int st = efg::check_attn("attn_prompt", type, n_seqs, n_rows, heads, kv_heads, head_dim, q_stride, scale))
+    return st;
+  if (k_stride < kv_heads * head_dim || v_stride < kv_heads * head_dim)
+    return fail(EFG_EINVAL, "attn_prompt: a row stride is shorter than a row");
+  if (n_rows == 0 || n_seqs == 0) return EFG_OK;
+  if (!d_out || !d_q || !d_k || !d_v || !d_cu) return fail(EFG_EINVAL, "attn_prompt: null pointer");
+  efg::DeviceInfo* dev = efg::current_device();
+  if (!dev) return EFG_ECUDA;
+  efg::AttnParams p{};
+  p.out = d_out;
+  p.q = d_q;
+  p.k = d_k;
+  p.v = d_v;
+  p.cu = d_cu;
+  p.q_stride = static_cast<int64_t>(q_stride);
+  p.k_stride = static_cast<int64_t>(k_stride);
+  p.v_stride = static_cast<int64_t>(v_stride);
+  p.n_rows = static_cast<int64_t>(n_rows);
+  p.n_seqs = static_cast<int64_t>(n_seqs);
+  p.heads = static_cast<int>(heads);
+  p.kv_heads = static_cast<int>(kv_heads);
+  p.group = p.heads / p.kv_heads;
+  p.head_dim = static_cast<int>(head_dim);
+  p.scale = scale;
+  p.err = dev->d_err;
+  return efg::launch_attn(type, p, static_cast<cudaStream_t>(stream));
+}
+
+int efg_attn_paged(int type, void* d_out, const void* d_q, size_t q_stride, const void* d_k_cache,
+                   const void* d_v_cache, size_t n_pages, size_t page_size, const int32_t* d_block_table,
+                   size_t max_pages, const int32_t* d_cu, const int32_t* d_kv_len, size_t n_seqs, size_t n_rows,
+                   size_t max_new, size_t heads, size_t kv_heads, size_t head_dim, float scale, void* stream) {
+  if (int st = efg::check_attn("attn_paged", type, n_seqs, n_rows, heads, kv_heads, head_dim, q_stride, scale))
+    return st;
+  if (page_size == 0 || page_size > (1u << 30)) return fail(EFG_EINVAL, "attn_paged: page size %zu", page_size);
+  if (max_new > 0x7FFFFFFFull) return fail(EFG_EINVAL, "attn_paged: max_new is out of range");
+  if (n_pages > 0x7FFFFFFFull / page_size || max_pages > 0x7FFFFFFFull / page_size)
+    return fail(EFG_EINVAL, "attn_paged: %zu pages (%zu a sequence) of %zu slots pass the 2^31 slots of a cache",
+                n_pages, max_pages, page_size);
+  if (n_rows == 0 || n_seqs == 0 || max_new == 0) return EFG_OK;
+  if (!d_out || !d_q || !d_cu || !d_kv_len || (n_pages && (!d_k_cache || !d_v_cache)) ||
+      (max_pages && !d_block_table))
+    return fail(EFG_EINVAL, "attn_paged: null pointer");
+  efg::DeviceInfo* dev = efg::current_device();
+  if (!dev) return EFG_ECUDA;
+  efg::AttnParams p{};
+  p.out = d_out;
+  p.q = d_q;
+  p.k = d_k_cache;
+  p.v = d_v_cache;
+  p.cu = d_cu;
+  p.kv_len = d_kv_len;
+  p.table = d_block_table;
+  p.q_stride = static_cast<int64_t>(q_stride);
+  p.k_stride = p.v_stride = static_cast<int64_t>(kv_heads * head_dim);
+  p.n_rows = static_cast<int64_t>(n_rows);
+  p.n_seqs = static_cast<int64_t>(n_seqs);
+  p.n_pages = static_cast<int64_t>(n_pages);
+  p.max_pages = static_cast<int64_t>(max_pages);
+  p.page_size = static_cast<int64_t>(page_size);
+  p.max_new = static_cast<int64_t>(max_new);
+  p.heads = static_cast<int>(heads);
+  p.kv_heads = static_cast<int>(kv_heads);
+  p.group = p.heads / p.kv_heads;
+  p.head_dim = static_cast<int>(head_dim);
+  p.scale = scale;
+  p.err = dev->d_err;
+  return efg::launch_attn(type, p, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,135 @@
+// efg_attn.cuh - what the attention kernels share: the call's parameters, typed loads and the
+// row-by-row softmax that every other kernel falls back to.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "efg_device.cuh"
+#include "efg_paged.cuh"
+
+namespace efg {
+
+struct AttnParams {
+  void* out;                 // [n_rows][heads][head_dim]
+  const void* q;             // rows of q_stride elements
+  const void *k, *v;         // prompt: rows of k_stride / v_stride elements; paged: the pools
+  const int32_t* cu;         // [n_seqs + 1] first row of each sequence
+  const int32_t* kv_len;     // paged: positions of each sequence, the new ones included; null: prompt
+  const int32_t* table;      // paged: [n_seqs][max_pages]
+  int64_t q_stride, k_stride, v_stride;
+  int64_t n_rows, n_seqs, n_pages, max_pages, page_size, max_new;
+  int heads, kv_heads, group, head_dim;
+  float scale;
+  int* err;
+};
+
+__device__ __forceinline__ float attn_widen(float v) { return v; }
+__device__ __forceinline__ float attn_widen(__half v) { return __half2float(v); }
+__device__ __forceinline__ float attn_widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T attn_narrow(float v) {
+  if constexpr (sizeof(T) == 4)
+    return v;
+  else if constexpr (std::is_same_v<T, __half>)
+    return __float2half_rn(v);
+  else
+    return __float2bfloat16_rn(v);
+}
+
+// The chunk of the packed batch that a row belongs to.
+struct Chunk {
+  int64_t seq, begin, end;  // sequence and its rows [begin, end)
+  int64_t kv_len;           // its positions
+};
+
+// False for rows behind the last sequence and for offsets that make no sense (recorded).
+__device__ __forceinline__ bool chunk_of_seq(const AttnParams& p, int64_t s, Chunk& c) {
+  c.seq = s;
+  c.begin = p.cu[s];
+  c.end = p.cu[s + 1];
+  if (c.begin < 0 || c.end > p.n_rows || c.end < c.begin || (p.kv_len && c.end - c.begin > p.max_new)) {
+    record_error(p.err, EFG_EINVAL);
+    return false;
+  }
+  c.kv_len = c.end - c.begin;
+  if (p.kv_len) {
+    c.kv_len = p.kv_len[s];
+    if (c.kv_len < 0 || c.kv_len > p.max_pages * p.page_size) {
+      record_error(p.err, EFG_EINVAL);
+      return false;
+    }
+  }
+  return true;
+}
+
+// Offset of the key (stride k_stride) of position j of the chunk's sequence, in rows of kv_heads *
+// head_dim elements for pages; -1 where the block table has no valid page (recorded).
+__device__ __forceinline__ int64_t key_row(const AttnParams& p, const Chunk& c, int64_t j) {
+  if (!p.kv_len) return c.begin + j;
+  const int32_t page = p.table[c.seq * p.max_pages + j / p.page_size];
+  if (!page_ok(page, p.n_pages)) {
+    record_error(p.err, EFG_EINVAL);
+    return -1;
+  }
+  return page * p.page_size + j % p.page_size;
+}
+
+// One warp computes one row of one query head: 32 keys at a time, a lane per key for the scores
+// (running maximum and sum of the softmax in FP32), then a lane per dim for the values. A key
+// behind the row's last visible one is never read, so what lies there (stale, infinite or NaN)
+// cannot reach the row. head_dim <= 256; q_s holds the row's query as FP32, scaled to base 2.
+template <typename T>
+__device__ void attend_row(const AttnParams& p, const Chunk& c, int64_t row, int head, float* q_s) {
+  const int lane = threadIdx.x & 31, D = p.head_dim, kvh = head / p.group;
+  const int64_t count = visible_keys(row, c.begin, c.end, c.kv_len);
+  const T* q = static_cast<const T*>(p.q) + row * p.q_stride + static_cast<int64_t>(head) * D;
+  for (int d = lane; d < D; d += 32) q_s[d] = attn_widen(q[d]);
+  __syncwarp();
+  const float to_base2 = p.scale * 1.4426950408889634f;
+  float acc[8] = {}, top = -INFINITY, sum = 0.f;
+  for (int64_t j0 = 0; j0 < count; j0 += 32) {
+    int64_t kr = -1;
+    float sc = -INFINITY;
+    if (j0 + lane < count) kr = key_row(p, c, j0 + lane);
+    if (kr >= 0) {
+      const T* k = static_cast<const T*>(p.k) + kr * p.k_stride + static_cast<int64_t>(kvh) * D;
+      float dot = 0.f;
+      for (int d = 0; d < D; ++d) dot = fmaf(q_s[d], attn_widen(k[d]), dot);
+      sc = dot * to_base2;
+    }
+    float m = sc;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float t = __shfl_xor_sync(0xFFFFFFFFu, m, o);
+      m = (t != t || m != m) ? NAN : fmaxf(m, t);  // a NaN score makes the row NaN
+    }
+    const float high = (m != m || top != top) ? NAN : fmaxf(top, m);
+    // nothing visible so far (every score -inf): keep the sums at zero
+    const float ref = high == -INFINITY ? 0.f : high;
+    const float w = kr >= 0 ? exp2f(sc - ref) : 0.f;
+    const float back = exp2f(top - ref);
+    sum = sum * back + warp_sum(w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] *= back;
+    top = high;
+    const int n = static_cast<int>(min(static_cast<int64_t>(32), count - j0));
+    for (int t = 0; t < n; ++t) {
+      const int64_t vr = __shfl_sync(0xFFFFFFFFu, kr, t);
+      const float wt = __shfl_sync(0xFFFFFFFFu, w, t);
+      if (vr < 0) continue;
+      const T* v = static_cast<const T*>(p.v) + vr * p.v_stride + static_cast<int64_t>(kvh) * D;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (lane + 32 * i < D) acc[i] = fmaf(wt, attn_widen(v[lane + 32 * i]), acc[i]);
+    }
+  }
+  T* out = static_cast<T*>(p.out) + (row * p.heads + head) * D;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing is zeros
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (lane + 32 * i < D) out[lane + 32 * i] = attn_narrow<T>(acc[i] * inv);
+  __syncwarp();
+}
+
+}  // namespace efg

@@ -61,8 +61,9 @@ const char* efg_last_error(void);
 /* Name of a status code ("EFG_OK", "EFG_EINVAL", ...). */
 const char* efg_status_string(int status);
 
-/* Reads and clears the error word that device-side bounded waits write on the current
- * device (synchronises the device first). *code receives EFG_OK or EFG_ETIMEOUT. */
+/* Reads and clears the error word that device-side bounded waits (EFG_ETIMEOUT) and the
+ * device-side checks of the paged calls (EFG_EINVAL, EFG_ENOMEM) write on the current device
+ * (synchronises the device first). *code receives EFG_OK or the first such code. */
 int efg_device_error(int* code);
 
 /* Early weight streaming for the matvec calls made afterwards on this thread (default
@@ -276,6 +277,78 @@ int efg_argmax(const float* d_x, size_t n, int32_t* d_index, void* stream);
 int efg_lm_head_argmax_sharded(int qtype, float* d_logits_shard, int32_t* d_token, const uint8_t* d_W_shard,
                                const float* d_x, const float* d_norm_w, float eps, size_t rows, size_t cols,
                                efg_comm* comm, void* stream);
+
+/* ================================================================ paged serving
+ * Operators for decoding many sequences over one pool of cache pages: a step's block tables
+ * and slot map (efg_page_plan), its rotated keys and its values into their pages
+ * (efg_page_store), attention of its new tokens over the pages (efg_attn_paged), and attention
+ * over packed prompts without a cache (efg_attn_prompt). No reference counterpart: the
+ * reference decodes one sequence over one contiguous cache (src/model.cpp:153-276), whose
+ * arithmetic (RoPE src/kernels.cpp:133-147, causal softmax with grouped heads
+ * src/kernels.cpp:148-174) these follow.
+ *
+ * A step's rows are packed: sequence s owns rows d_cu[s] .. d_cu[s + 1] - 1 (d_cu[0] = 0,
+ * n_seqs + 1 offsets); rows from d_cu[n_seqs] to n_rows are padding, which a captured step of a
+ * fixed size may have, and their outputs stay as they were. A cache is n_pages pages of
+ * page_size token slots, [page][offset][kv_heads][head_dim], slot = page * page_size + offset;
+ * row s of the block table ([n_seqs][max_pages]) lists the pages of sequence s in order.
+ *
+ * Types are EFG_F32, EFG_F16 and EFG_BF16. Strides count elements between the rows of an input
+ * (heads lie back to back within a row), so q, k and v may be views of one projection's rows;
+ * outputs are contiguous. Lengths, offsets, pages and slots are read on the device: values that
+ * make no sense there read and write nothing out of range, record EFG_EINVAL for
+ * efg_device_error and leave the rows that they concern as they were or without a defined
+ * value. None of the calls allocates, keeps a workspace or synchronises, so they run on any
+ * streams at once and inside CUDA graphs (after one call outside a capture on each device).
+ */
+
+/* One step from lengths and a free list. Sequence s holds d_cached[s] tokens in the first
+ * ceil(d_cached[s] / page_size) entries of its block table row and gets d_new[s] tokens (0 is
+ * allowed); the fresh pages it needs are taken from d_free[0..n_free) in sequence order and
+ * entered in the table. Writes d_cu; d_slots and d_positions of every packed row (-1 for
+ * padding rows); d_kv_len[s] = cached + new; *d_taken = how many pages of d_free were taken.
+ * A sequence whose pages do not fit in the free list is not served, nor is any after it that
+ * needs a page (EFG_ENOMEM for efg_device_error); one with negative lengths or more positions
+ * than max_pages hold is not served either (EFG_EINVAL). The rows of a sequence that is not
+ * served get slot and position -1 and its kv_len is 0. More new tokens than n_rows: the rows
+ * behind n_rows are dropped and d_cu stops at n_rows (EFG_EINVAL). */
+int efg_page_plan(int32_t* d_block_table, size_t max_pages, int32_t* d_slots, int32_t* d_positions, size_t n_rows,
+                  int32_t* d_cu, int32_t* d_kv_len, int32_t* d_taken, const int32_t* d_cached, const int32_t* d_new,
+                  size_t n_seqs, const int32_t* d_free, size_t n_free, size_t n_pages, size_t page_size,
+                  void* stream);
+
+/* For every row r: q_out[r] = RoPE(q[r]) at d_positions[r], the cache's slot d_slots[r] gets
+ * RoPE(k[r]) and v[r]. d_cos and d_sin are [max_pos][head_dim / 2] tables (the rotation of
+ * src/kernels.cpp:133-147, halves of a head paired); both NULL: no rotation. d_q and d_q_out
+ * both NULL: keys and values only. q_out may be q itself (same type, rows back to back).
+ * cache_type (of q_out and of the caches) is `type`, or EFG_F16 / EFG_BF16 for EFG_F32 rows: the
+ * rotation is in FP32 and rounds once, to nearest even. A row with position -1 is left out, one
+ * with slot -1 has its query rotated and stores nothing. The slots of a call must be distinct.
+ * head_dim even, at most 256. */
+int efg_page_store(int type, int cache_type, void* d_q_out, void* d_k_cache, void* d_v_cache, size_t n_slots,
+                   const void* d_q, size_t q_stride, const void* d_k, size_t k_stride, const void* d_v,
+                   size_t v_stride, const int32_t* d_slots, const int32_t* d_positions, size_t n_rows,
+                   const float* d_cos, const float* d_sin, size_t max_pos, size_t heads, size_t kv_heads,
+                   size_t head_dim, void* stream);
+
+/* Causal attention over packed prompts: row r of sequence s attends to rows d_cu[s] .. r.
+ * out [n_rows][heads][head_dim] = softmax(scale q k^T) v, query head h reading key head
+ * h / (heads / kv_heads). Inputs and output of one type; scores, softmax and sums in FP32 (F32
+ * inputs keep FP32 accuracy). head_dim up to 256. out must not overlap an input. */
+int efg_attn_prompt(int type, void* d_out, const void* d_q, size_t q_stride, const void* d_k, size_t k_stride,
+                    const void* d_v, size_t v_stride, const int32_t* d_cu, size_t n_seqs, size_t n_rows, size_t heads,
+                    size_t kv_heads, size_t head_dim, float scale, void* stream);
+
+/* Attention of each sequence's new tokens over its pages: row i of the chunk of sequence s (of
+ * m = d_cu[s + 1] - d_cu[s] rows) attends to positions 0 .. d_kv_len[s] - m + i, so the chunk's
+ * own keys (stored before, efg_page_store) are the last m positions. m is 1 for a decode step
+ * and at most max_new, which sizes the launch; a longer chunk is an error (EFG_EINVAL for
+ * efg_device_error). A row that sees no position gets zeros. What lies in the pages behind the
+ * last position is never used. Types as efg_attn_prompt, the caches of `type` too. */
+int efg_attn_paged(int type, void* d_out, const void* d_q, size_t q_stride, const void* d_k_cache,
+                   const void* d_v_cache, size_t n_pages, size_t page_size, const int32_t* d_block_table,
+                   size_t max_pages, const int32_t* d_cu, const int32_t* d_kv_len, size_t n_seqs, size_t n_rows,
+                   size_t max_new, size_t heads, size_t kv_heads, size_t head_dim, float scale, void* stream);
 
 /* ================================================================ .efq and the decode step */
 

@@ -1,0 +1,169 @@
+"""Paged serving without a GPU: the index arithmetic that the kernels run (efg_paged.cuh, compiled for
+the host) on good and bad lengths and page ids, and the calls that are refused before any device work."""
+from __future__ import annotations
+
+import ctypes as C
+import random
+import subprocess
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+ROOT = Path(__file__).resolve().parent.parent
+
+HOST = r"""
+#include "efg_paged.cuh"
+using namespace efg;
+extern "C" {
+void need(int32_t c, int32_t f, int64_t ps, int64_t mp, int64_t* out) {
+  const SeqNeed n = seq_need(c, f, ps, mp);
+  out[0] = n.rows; out[1] = n.have; out[2] = n.need; out[3] = n.valid;
+}
+int served(int64_t need, int valid, int64_t first, int64_t n_free) {
+  return seq_served(SeqNeed{0, 0, need, valid != 0}, first, n_free);
+}
+int ok(int32_t page, int64_t n) { return page_ok(page, n); }
+int64_t visible(int64_t r, int64_t b, int64_t e, int64_t k) { return visible_keys(r, b, e, k); }
+int64_t find(const int32_t* cu, int64_t n, int64_t row) { return find_sequence(cu, n, row); }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def host(tmp_path_factory):
+    d = tmp_path_factory.mktemp("paged")
+    (d / "host.cpp").write_text(HOST)
+    subprocess.run(["g++", "-std=c++20", "-O1", "-Wall", "-Werror", "-fsanitize=undefined",
+                    "-fno-sanitize-recover", "-shared", "-fPIC", "-I", str(ROOT / "edgeforge_b200" / "csrc"),
+                    str(d / "host.cpp"), "-o", str(d / "host.so")], check=True)
+    lib = C.CDLL(str(d / "host.so"))
+    i64 = C.c_int64
+    lib.need.argtypes = [C.c_int32, C.c_int32, i64, i64, C.c_void_p]
+    lib.served.argtypes = [i64, C.c_int, i64, i64]
+    lib.ok.argtypes = [C.c_int32, i64]
+    lib.visible.argtypes, lib.visible.restype = [i64] * 4, i64
+    lib.find.argtypes, lib.find.restype = [C.c_void_p, i64, i64], i64
+    return lib
+
+
+def _need(lib, *a):
+    out = np.zeros(4, np.int64)
+    lib.need(*a, out.ctypes.data)
+    return tuple(int(v) for v in out)
+
+
+def test_needs(host):
+    assert _need(host, 0, 0, 16, 4) == (0, 0, 0, 1)
+    assert _need(host, 16, 1, 16, 4) == (1, 1, 1, 1)
+    assert _need(host, 15, 1, 16, 4) == (1, 1, 0, 1)
+    assert _need(host, 0, 64, 16, 4) == (64, 0, 4, 1)
+    assert _need(host, 0, 65, 16, 4) == (65, 0, 0, 0)  # more positions than the table holds
+    assert _need(host, -1, 5, 16, 4) == (5, 0, 0, 0)
+    assert _need(host, 5, -1, 16, 4) == (0, 0, 0, 0)
+    big = 2**31 - 1
+    assert _need(host, big, big, 16, big) == (big, 2**27, 2**27, 1)  # no 32-bit overflow
+    assert host.served(3, 1, 5, 8) and not host.served(4, 1, 5, 8)
+    assert host.served(0, 1, 100, 8) and not host.served(0, 0, 0, 8)
+
+
+def test_pages_and_visible_positions(host):
+    assert host.ok(0, 1) and not host.ok(1, 1) and not host.ok(-1, 5) and not host.ok(0, 0)
+    assert host.visible(0, 0, 1, 1) == 1
+    assert host.visible(12, 10, 14, 100) == 99
+    assert host.visible(10, 10, 14, 3) == 0  # a chunk longer than its cache: the first rows see nothing
+    assert host.visible(13, 10, 14, 3) == 3
+    assert host.visible(10, 10, 14, 0) == 0
+
+
+def test_find_sequence_stays_in_bounds(host):
+    r = random.Random(1)
+    for trial in range(300):
+        n = r.choice([1, 2, 5, 33])
+        good = trial % 2 == 0
+        cu = [0]
+        for _ in range(n):
+            cu.append(cu[-1] + r.choice([0, 0, 1, 7]) if good else r.randint(-2**31, 2**31 - 1))
+        a = np.array(cu, np.int32)
+        for row in range(-1, max(cu[-1], 3) + 2 if good else 20):
+            s = host.find(a.ctypes.data, n, row)
+            assert -1 <= s <= n
+            if good:
+                assert s == max((i for i in range(n + 1) if cu[i] <= row), default=-1)
+
+
+def test_c_refusals(efg_lib):
+    """Refused on the host, before a device is looked for (there is none here)."""
+    lib = efg_lib.load()
+    P = 4096  # never dereferenced
+
+    def said(code, text):
+        assert code == 1
+        assert text in lib.efg_last_error().decode(), lib.efg_last_error()
+
+    plan = lambda **k: lib.efg_page_plan(*{**dict(t=P, mp=4, s=P, p=P, r=8, cu=P, kv=P, tk=P, c=P, n=P, ns=2, f=P, nf=8,  # noqa: E731
+                                                  np=16, ps=16, st=None), **k}.values())
+    said(plan(cu=None), "null pointer")
+    said(plan(f=None), "null pointer")
+    said(plan(t=None), "null pointer")
+    said(plan(s=None), "null pointer")
+    said(plan(ps=0), "page size 0")
+    said(plan(np=2**30), "2^31 slots")
+    said(plan(r=2**31), "out of range")
+
+    store = lambda **k: lib.efg_page_store(*{**dict(ty=2, ct=2, qo=P, kc=P, vc=P, ns=64, q=P, qs=512, k=P, ks=128, v=P,  # noqa: E731
+                                                    vs=128, sl=P, po=P, r=3, co=P, si=P, mp=64, h=8, kv=2, d=64,
+                                                    st=None), **k}.values())
+    said(store(ty=3), "unknown type 3")
+    said(store(ct=1), "the cache has the rows' type")
+    said(store(ty=1, ct=0), "the cache has the rows' type")
+    said(store(d=63), "not an even number")
+    said(store(d=0), "not an even number")
+    said(store(kv=0), "key heads")
+    said(store(q=None), "come together")
+    said(store(si=None), "come together")
+    said(store(ks=127), "shorter than a row")
+    said(store(sl=None), "null pointer")
+    assert store(r=0) == 0  # nothing to do
+
+    prompt = lambda **k: lib.efg_attn_prompt(*{**dict(ty=2, o=P, q=P, qs=512, k=P, ks=128, v=P, vs=128, cu=P, n=1, r=5,  # noqa: E731
+                                                      h=8, kv=2, d=64, sc=0.125, st=None), **k}.values())
+    said(prompt(ty=4), "unknown type 4")
+    said(prompt(d=257), "not in 1..256")
+    said(prompt(h=7), "do not divide")
+    said(prompt(kv=0), "do not divide")
+    said(prompt(qs=511), "shorter than a row")
+    said(prompt(vs=100), "shorter than a row")
+    said(prompt(sc=float("nan")), "not finite")
+    said(prompt(sc=float("inf")), "not finite")
+    said(prompt(cu=None), "null pointer")
+    said(prompt(r=2**31), "out of range")
+    assert prompt(r=0) == 0 and prompt(n=0) == 0
+
+    paged = lambda **k: lib.efg_attn_paged(*{**dict(ty=2, o=P, q=P, qs=512, k=P, v=P, np=16, ps=16, t=P, mp=4, cu=P, kl=P,  # noqa: E731
+                                                    n=1, r=5, mn=5, h=8, kv=2, d=64, sc=0.125, st=None), **k}.values())
+    said(paged(ps=0), "page size 0")
+    said(paged(np=2**28), "2^31 slots")
+    said(paged(mp=2**28), "2^31 slots")
+    said(paged(mn=2**31), "max_new")
+    said(paged(t=None), "null pointer")
+    said(paged(v=None), "null pointer")
+    said(paged(h=9), "do not divide")
+    assert paged(r=0) == 0 and paged(mn=0) == 0
+
+
+def test_python_refusals(efg_lib):
+    torch = pytest.importorskip("torch")
+    E = efg_lib.EdgeForgeError
+    z = lambda *s, t=torch.float32: torch.zeros(*s, dtype=t)  # noqa: E731
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    with pytest.raises(E, match="current CUDA device"):
+        efg_lib.attn_prompt(z(4, 2, 8), z(4, 2, 8), z(4, 1, 8), z(4, 1, 8), i(2))
+    with pytest.raises(E, match="current CUDA device"):
+        efg_lib.attn_paged(z(4, 2, 8), z(4, 2, 8), z(3, 16, 1, 8), z(3, 16, 1, 8), i(1, 3), i(2), i(1), 4)
+    with pytest.raises(E, match="current CUDA device"):
+        efg_lib.page_plan(i(2, 4), i(8), i(8), i(3), i(2), i(1), i(2), i(2), i(4), 16, 16)
+    with pytest.raises(E, match="come together"):
+        efg_lib.page_store(None, z(3, 16, 1, 8), z(3, 16, 1, 8), z(4, 2, 8), z(4, 1, 8), z(4, 1, 8), i(4), i(4))
+    with pytest.raises(E, match="back to back"):
+        efg_lib.page_store(None, z(3, 16, 2, 8), z(3, 16, 2, 8), None, z(4, 8, 2).transpose(1, 2), z(4, 2, 8), i(4), i(4))
