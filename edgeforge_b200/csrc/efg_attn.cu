@@ -10,6 +10,7 @@
 
 #include "../../include/efg.h"
 #include "efg_attn.cuh"
+#include "efg_attn_launch.h"
 #include "efg_host.h"
 
 namespace efg {
@@ -22,9 +23,7 @@ template <typename T>
 __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(const AttnParams p) {
   __shared__ float q_s[kRowWarps][256];
   const int warp = threadIdx.x >> 5;
-  if (blockIdx.x == 0)  // one CTA looks at every offset: a row finds its sequence by bisection and may miss a bad one
-    for (int64_t s = threadIdx.x; s < p.n_seqs; s += blockDim.x)
-      if (p.cu[s] < 0 || p.cu[s + 1] < p.cu[s] || p.cu[s + 1] > p.n_rows) record_error(p.err, EFG_EINVAL);
+  if (blockIdx.x == 0) check_offsets(p);
   const int64_t item = static_cast<int64_t>(blockIdx.x) * kRowWarps + warp;
   const int64_t row = item / p.heads;
   if (row >= p.n_rows) return;
@@ -44,7 +43,8 @@ int launch_rows(const AttnParams& p, cudaStream_t s) {
   return EFG_OK;
 }
 
-int launch_attn(int type, const AttnParams& p, cudaStream_t s) {
+int launch_attn(int type, const AttnParams& p, int sms, cudaStream_t s) {
+  if (attn_mma_takes(type, p)) return launch_attn_mma(type, p, sms, s);
   if (type == EFG_F32) return launch_rows<float>(p, s);
   if (type == EFG_F16) return launch_rows<__half>(p, s);
   return launch_rows<__nv_bfloat16>(p, s);
@@ -98,7 +98,7 @@ int efg_attn_prompt(int type, void* d_out, const void* d_q, size_t q_stride, con
   p.head_dim = static_cast<int>(head_dim);
   p.scale = scale;
   p.err = dev->d_err;
-  return efg::launch_attn(type, p, static_cast<cudaStream_t>(stream));
+  return efg::launch_attn(type, p, dev->sm_count, static_cast<cudaStream_t>(stream));
 }
 
 int efg_attn_paged(int type, void* d_out, const void* d_q, size_t q_stride, const void* d_k_cache,
@@ -140,7 +140,7 @@ int efg_attn_paged(int type, void* d_out, const void* d_q, size_t q_stride, cons
   p.head_dim = static_cast<int>(head_dim);
   p.scale = scale;
   p.err = dev->d_err;
-  return efg::launch_attn(type, p, static_cast<cudaStream_t>(stream));
+  return efg::launch_attn(type, p, dev->sm_count, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -63,6 +63,13 @@ __device__ __forceinline__ bool chunk_of_seq(const AttnParams& p, int64_t s, Chu
   return true;
 }
 
+// Looks at every offset once (one CTA's threads): kernels that find a row's sequence by search may miss a
+// bad one.
+__device__ __forceinline__ void check_offsets(const AttnParams& p) {
+  for (int64_t s = threadIdx.x; s < p.n_seqs; s += blockDim.x)
+    if (p.cu[s] < 0 || p.cu[s + 1] < p.cu[s] || p.cu[s + 1] > p.n_rows) record_error(p.err, EFG_EINVAL);
+}
+
 // Offset of the key (stride k_stride) of position j of the chunk's sequence, in rows of kv_heads *
 // head_dim elements for pages; -1 where the block table has no valid page (recorded).
 __device__ __forceinline__ int64_t key_row(const AttnParams& p, const Chunk& c, int64_t j) {
@@ -130,6 +137,22 @@ __device__ void attend_row(const AttnParams& p, const Chunk& c, int64_t row, int
   for (int i = 0; i < 8; ++i)
     if (lane + 32 * i < D) out[lane + 32 * i] = attn_narrow<T>(acc[i] * inv);
   __syncwarp();
+}
+
+// Whether a non-finite value of the KV head lies at a position that the row does not see, but
+// that was in a tile with positions it sees (up to `end`): 0 times it is NaN in a matrix product.
+// One warp; every lane gets the answer.
+template <typename T>
+__device__ bool reached_from_behind(const AttnParams& p, const Chunk& c, int64_t row, int kvh, int64_t end) {
+  const int lane = threadIdx.x & 31;
+  bool bad = false;
+  for (int64_t j = visible_keys(row, c.begin, c.end, c.kv_len); j < end; ++j) {
+    const int64_t vr = key_row(p, c, j);
+    if (vr < 0) continue;
+    const T* v = static_cast<const T*>(p.v) + vr * p.v_stride + static_cast<int64_t>(kvh) * p.head_dim;
+    for (int d = lane; d < p.head_dim; d += 32) bad = bad || !(fabsf(attn_widen(v[d])) <= 3.402823466e38f);
+  }
+  return __any_sync(0xFFFFFFFFu, bad);
 }
 
 }  // namespace efg

@@ -44,6 +44,18 @@ int ensure_smem_attr(const void* fn, size_t bytes) {
   return EFG_OK;
 }
 
+int ensure_wide_cluster(const void* fn) {
+  static std::mutex mu;
+  static std::map<std::pair<int, const void*>, bool> done;
+  int dev = 0;
+  EFG_TRY_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
+  std::lock_guard<std::mutex> lk(mu);
+  bool& d = done[{dev, fn}];
+  if (!d) EFG_TRY_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "kernel cluster attribute");
+  d = true;
+  return EFG_OK;
+}
+
 int fail(int status, const char* fmt, ...) {
   char buf[1024];
   va_list ap;

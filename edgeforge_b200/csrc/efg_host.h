@@ -42,6 +42,9 @@ bool& small_gemm_flag();
 // later calls are free, so launches can be captured into CUDA graphs.
 int ensure_smem_attr(const void* fn, size_t bytes);
 
+// Allows clusters of more than 8 CTAs, once per (device, kernel).
+int ensure_wide_cluster(const void* fn);
+
 // A 2-D TMA tensor map over `rows` rows of `row_bytes` bytes (16-byte aligned base and row
 // stride) seen as 8-byte elements, with a box of box_elems x box_rows; the box may reach past
 // a row's end or past the last row (zero fill). cuTensorMapEncodeTiled from the driver, looked
