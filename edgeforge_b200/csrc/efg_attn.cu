@@ -44,6 +44,7 @@ int launch_rows(const AttnParams& p, cudaStream_t s) {
 }
 
 int launch_attn(int type, const AttnParams& p, int sms, cudaStream_t s) {
+  if (attn_tc_takes(type, p)) return launch_attn_tc(type, p, sms, s);
   if (attn_mma_takes(type, p)) return launch_attn_mma(type, p, sms, s);
   if (type == EFG_F32) return launch_rows<float>(p, s);
   if (type == EFG_F16) return launch_rows<__half>(p, s);

@@ -2,6 +2,8 @@
 // row-by-row softmax that every other kernel falls back to.
 #pragma once
 
+#include <type_traits>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -80,6 +82,71 @@ __device__ __forceinline__ int64_t key_row(const AttnParams& p, const Chunk& c, 
     return -1;
   }
   return page * p.page_size + j % p.page_size;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// The tile of rows a CTA owns: its sequence and its place among the sequence's tiles.
+struct RowTile {
+  int64_t seq, index;
+};
+
+// Tile `want` when every sequence has ceil(rows * mul / div) tiles, in order; the tiles of one
+// sequence come last to first (the last one of a prompt is the longest). The whole CTA (kThreads
+// threads) calls it; `scan` is shared, kThreads / 32 + 2 entries. False behind the last tile.
+template <int kThreads>
+__device__ bool find_tile(const AttnParams& p, int64_t want, int64_t mul, int64_t div, int64_t* scan, RowTile& t) {
+  constexpr int kWarps = kThreads / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int64_t base = 0;
+  for (int64_t s0 = 0; s0 < p.n_seqs; s0 += kThreads) {
+    int64_t n = 0;
+    if (s0 + tid < p.n_seqs) {
+      const int64_t m = static_cast<int64_t>(p.cu[s0 + tid + 1]) - p.cu[s0 + tid];
+      // lengths that make no sense get one tile, whose CTA records them
+      n = m < 0 || m > p.n_rows ? 1 : (m * mul + div - 1) / div;
+    }
+    int64_t inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    if (lane == 31) scan[warp] = inc;
+    __syncthreads();
+    int64_t before = base, total = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += scan[w];
+      total += scan[w];
+    }
+    if (want >= before + inc - n && want < before + inc) {
+      scan[kWarps] = s0 + tid;
+      scan[kWarps + 1] = before + inc - 1 - want;
+    }
+    __syncthreads();
+    if (want < base + total) {
+      t.seq = scan[kWarps];
+      t.index = scan[kWarps + 1];
+      return true;
+    }
+    base += total;
+  }
+  return false;
 }
 
 // One warp computes one row of one query head: 32 keys at a time, a lane per key for the scores

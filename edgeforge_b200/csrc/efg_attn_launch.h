@@ -12,4 +12,8 @@ struct AttnParams;
 bool attn_mma_takes(int type, const AttnParams& p);
 int launch_attn_mma(int type, const AttnParams& p, int sms, cudaStream_t s);
 
+// 5th-generation tensor cores (efg_attn_tc.cu): 16-bit types and more than 64 rows per key head.
+bool attn_tc_takes(int type, const AttnParams& p);
+int launch_attn_tc(int type, const AttnParams& p, int sms, cudaStream_t s);
+
 }  // namespace efg

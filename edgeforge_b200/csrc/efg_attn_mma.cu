@@ -42,12 +42,6 @@ constexpr int stages() {
   return stage_bytes<T, D>() <= 16384 ? 4 : 3;
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // 16 bytes to shared memory, or zeros.
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
@@ -103,17 +97,6 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
   lo = __float_as_uint(x - __uint_as_float(hi)) & 0xFFFFE000u;
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (std::is_same_v<T, __half>) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
-
 // Where 16-byte chunk c of key row r lies: the chunks of a row are exchanged so that the eight
 // addresses of every shared-memory phase fall into different banks. 16-bit: ldmatrix takes one
 // chunk of 8 rows. F32 keys: a quad of lanes takes 4 chunks of one row, two rows a phase. F32
@@ -127,50 +110,6 @@ __device__ __forceinline__ int value_chunk(int r, int c) {
   return sizeof(T) == 2 ? c ^ (r & 7) : c ^ (((r >> 1) & 3) << 1);
 }
 
-// The tile of rows a CTA owns: sequence and first row, found among the sequences in order.
-struct RowTile {
-  int64_t seq, index;
-};
-template <int kRows>
-__device__ bool find_tile(const AttnParams& p, int64_t want, int64_t* scan, RowTile& t) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int64_t base = 0;
-  for (int64_t s0 = 0; s0 < p.n_seqs; s0 += kThreads) {
-    int64_t n = 0;
-    if (s0 + tid < p.n_seqs) {
-      const int64_t m = static_cast<int64_t>(p.cu[s0 + tid + 1]) - p.cu[s0 + tid];
-      // lengths that make no sense get one tile, whose CTA records them
-      n = m < 0 || m > p.n_rows ? 1 : (m * p.group + kRows - 1) / kRows;
-    }
-    int64_t inc = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-      if (lane >= o) inc += up;
-    }
-    if (lane == 31) scan[warp] = inc;
-    __syncthreads();
-    int64_t before = base, total = 0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) before += scan[w];
-      total += scan[w];
-    }
-    if (want >= before + inc - n && want < before + inc) {
-      scan[4] = s0 + tid;
-      scan[5] = n - 1 - (want - (before + inc - n));  // the last tile of a prompt is the longest: first
-    }
-    __syncthreads();
-    if (want < base + total) {
-      t.seq = scan[4];
-      t.index = scan[5];
-      return true;
-    }
-    base += total;
-  }
-  return false;
-}
-
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2)
     attn_mma_kernel(const AttnParams p, const int tiles_per_seq) {
@@ -181,7 +120,7 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
   constexpr int KK = D / 16;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int32_t slot_s[2][kKeys];
-  __shared__ int64_t scan_s[6];
+  __shared__ int64_t scan_s[kThreads / 32 + 2];
   __shared__ float top_s[4][16], sum_s[4][16];  // per warp, then (row order) per CTA
   __shared__ float part_top[64], part_sum[64];
   __shared__ float q_s[4][256];
@@ -197,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
   if (tiles_per_seq > 0) {
     rt.seq = tile_id / tiles_per_seq;
     rt.index = tile_id - rt.seq * tiles_per_seq;
-  } else if (!find_tile<kRows>(p, tile_id, scan_s, rt)) {
+  } else if (!find_tile<kThreads>(p, tile_id, p.group, kRows, scan_s, rt)) {
     return;  // uniform over the cluster
   }
   Chunk c;

@@ -7,6 +7,9 @@ operands split for the tensor cores leave out at most 2^-21 of a product, counte
 weight by twice that plus 2^-21 (exponential, running maximum, normalisation), and a sum over n weights
 by (n / 8 + 40) 2^-24 of A: no kernel adds more than n / 8 products one after the other outside the
 tensor cores, whose sums over 16 or more products are at least as good as one FP32 chain over n / 8.
+The 16-bit kernels may take the exponential from a polynomial that is off by 2.6e-6 < 2^-18, which counts
+twice (weight and normalisation), and F16 holds a weight of at most 2^-14 of the largest within 2^-25 of it,
+which over n weights is at most n 2^-25 max |v|.
 """
 from __future__ import annotations
 
@@ -17,13 +20,13 @@ EPS = {"f32": 2.0**-23, "f16": 2.0**-10, "bf16": 2.0**-7}
 
 def attend(q, k, v, scale, last=None):
     """q [m][h][d], k and v [n][kv][d] in float64; row i sees keys 0 .. n - m + i. Returns (out, tolerance
-    without the type's own roundings as a multiple of A, A)."""
+    without the type's own roundings as a multiple of A, A, n max |v|)."""
     m, h, d = q.shape
     n, kv, _ = k.shape
     g = h // kv
     out = np.zeros((m, h, d))
     A = np.zeros((m, h, d))
-    rel = np.zeros((m, h, 1))
+    rel, tiny = np.zeros((m, h, 1)), np.zeros((m, h, 1))
     for i in range(m):
         c = n - m + i + 1
         if c <= 0:
@@ -37,12 +40,15 @@ def attend(q, k, v, scale, last=None):
             out[i, a * g : (a + 1) * g] = w @ v[:c, a]
             A[i, a * g : (a + 1) * g] = w @ np.abs(v[:c, a])
             rel[i, a * g : (a + 1) * g] = 2 * (d + 12) * 2.0**-24 * B + 2.0**-21 + (c / 8 + 40) * 2.0**-24
-    return out, rel, A
+            tiny[i, a * g : (a + 1) * g] = c * np.abs(v[:c, a]).max()
+    return out, rel, A, tiny
 
 
-def tolerance(kind, out, rel, A):
+def tolerance(kind, out, rel, A, tiny):
     u = EPS[kind] / 2
-    return u * np.abs(out) + A * (rel + (0 if kind == "f32" else u)) + (2.0**-25 if kind == "f16" else 0.0)
+    if kind == "f32":
+        return u * np.abs(out) + A * rel
+    return u * np.abs(out) + A * (rel + u + 2.0**-17) + (2.0**-25 * (1 + tiny) if kind == "f16" else 0.0)
 
 
 def plan(cached, new, table, free, page_size, n_rows):
