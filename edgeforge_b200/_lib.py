@@ -91,7 +91,8 @@ SIGNATURES = {
                             _sz, _sz, _vp]),
     "efg_attn_prompt": (_i, [_i, _vp, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _sz, _sz, _sz, _sz, C.c_float, _vp]),
     "efg_attn_paged": (_i, [_i, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz,
-                            C.c_float, _vp]),
+                            C.c_float, _vp, _sz, _vp]),
+    "efg_attn_paged_workspace": (_u64, [_i, _sz, _sz, _sz, _sz, _sz, _sz, _sz, _sz]),
     "efg_efq_check": (_i, [_vp, _u64]),
     "efg_quantize_model": (_i, [C.c_char_p, C.c_char_p, C.c_char_p, C.c_char_p, C.POINTER(QuantizeReport)]),
     "efg_decoder_open": (_i, [C.c_char_p, _sz, C.POINTER(_vp)]),

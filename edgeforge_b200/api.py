@@ -468,13 +468,16 @@ def attn_prompt(out, q, k, v, cu, scale: float | None = None) -> None:
 def attn_paged(out, q, k_cache, v_cache, block_table, cu, kv_len, max_new: int, scale: float | None = None) -> None:
     """Attention of each sequence's new tokens over its cache pages (efg_attn_paged): out and q
     [rows][heads][dim], caches [pages][page_size][kv_heads][dim], block_table [n][max_pages], cu
-    [n + 1] and kv_len [n] as page_plan writes them; max_new: no chunk is longer (1 for decode)."""
+    [n + 1] and kv_len [n] as page_plan writes them; max_new: no chunk is longer (1 for decode).
+    The workspace that long sequences need comes from torch's allocator, for this call."""
+    import torch
+
     _here("attn_paged", out, q, k_cache, v_cache, block_table, cu, kv_len)
     _ints("attn_paged", block_table, cu, kv_len)
     _whole("attn_paged", out, k_cache, v_cache)
     n_rows, dim = q.shape[0], q.shape[-1]
     heads, q_stride = _rows3("attn_paged: q", q, n_rows, dim)
-    n = kv_len.numel()
+    n, max_new = kv_len.numel(), int(max_new)
     if k_cache.dim() != 4 or k_cache.shape[3] != dim or v_cache.shape != k_cache.shape:
         raise EdgeForgeError(1, f"attn_paged: caches {list(k_cache.shape)} and {list(v_cache.shape)} for head size {dim}")
     if out.shape != q.shape or not (out.dtype == q.dtype == k_cache.dtype == v_cache.dtype):
@@ -482,10 +485,14 @@ def attn_paged(out, q, k_cache, v_cache, block_table, cu, kv_len, max_new: int, 
     if block_table.dim() != 2 or block_table.shape[0] != n or cu.numel() != n + 1:
         raise EdgeForgeError(1, f"attn_paged: block table {list(block_table.shape)} and {cu.numel()} offsets for {n} "
                                 "sequences")
-    check(load().efg_attn_paged(_plain_type(q, "attn_paged"), out.data_ptr(), q.data_ptr(), q_stride, k_cache.data_ptr(),
-                                v_cache.data_ptr(), k_cache.shape[0], k_cache.shape[1], block_table.data_ptr(),
-                                block_table.shape[1], cu.data_ptr(), kv_len.data_ptr(), n, n_rows, int(max_new), heads,
-                                k_cache.shape[2], dim, max(dim, 1)**-0.5 if scale is None else scale, _stream()))
+    pages, page_size, kv_heads, _ = k_cache.shape
+    kind, wide, lib = _plain_type(q, "attn_paged"), block_table.shape[1], load()
+    need = lib.efg_attn_paged_workspace(kind, page_size, wide, n, n_rows, max_new, heads, kv_heads, dim)
+    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    check(lib.efg_attn_paged(kind, out.data_ptr(), q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(), pages,
+                             page_size, block_table.data_ptr(), wide, cu.data_ptr(), kv_len.data_ptr(), n, n_rows, max_new,
+                             heads, kv_heads, dim, max(dim, 1)**-0.5 if scale is None else scale,
+                             work.data_ptr() if need else None, need, _stream()))
 
 
 # ---------------------------------------------------------------- .efq and the decode step

@@ -4,6 +4,7 @@
 //   out[r][h] = sum_j w_j v[j][h / group],  w = softmax_j(scale q[r][h] . k[j][h / group])
 //
 // over the positions j that row r sees: those of its own sequence up to its own position.
+#include <algorithm>
 #include <type_traits>
 
 #include <cuda_runtime.h>
@@ -43,7 +44,13 @@ int launch_rows(const AttnParams& p, cudaStream_t s) {
   return EFG_OK;
 }
 
-int launch_attn(int type, const AttnParams& p, int sms, cudaStream_t s) {
+int launch_attn(int type, const AttnParams& p, int sms, void* work, size_t work_bytes, cudaStream_t s) {
+  if (attn_decode_takes(type, p)) {
+    const size_t need = attn_decode_workspace(type, p, sms);
+    if (need > work_bytes || (need && !work))
+      return fail(EFG_EINVAL, "attention: a workspace of %zu bytes is needed, got %zu", need, work_bytes);
+    return launch_attn_decode(type, p, sms, work, s);
+  }
   if (attn_tc_takes(type, p)) return launch_attn_tc(type, p, sms, s);
   if (attn_mma_takes(type, p)) return launch_attn_mma(type, p, sms, s);
   if (type == EFG_F32) return launch_rows<float>(p, s);
@@ -99,13 +106,29 @@ int efg_attn_prompt(int type, void* d_out, const void* d_q, size_t q_stride, con
   p.head_dim = static_cast<int>(head_dim);
   p.scale = scale;
   p.err = dev->d_err;
-  return efg::launch_attn(type, p, dev->sm_count, static_cast<cudaStream_t>(stream));
+  return efg::launch_attn(type, p, dev->sm_count, nullptr, 0, static_cast<cudaStream_t>(stream));
+}
+
+uint64_t efg_attn_paged_workspace(int type, size_t page_size, size_t max_pages, size_t n_seqs, size_t n_rows,
+                                  size_t max_new, size_t heads, size_t kv_heads, size_t head_dim) {
+  efg::AttnParams p{};
+  p.kv_len = reinterpret_cast<const int32_t*>(1);  // a paged call; never read
+  p.n_seqs = static_cast<int64_t>(n_seqs);
+  p.max_pages = static_cast<int64_t>(max_pages);
+  p.page_size = static_cast<int64_t>(page_size);
+  p.kv_heads = static_cast<int>(kv_heads);
+  p.head_dim = static_cast<int>(head_dim);
+  if (kv_heads == 0 || n_seqs == 0 || std::min(max_new, n_rows) * (heads / kv_heads) > efg::kDecodeRows || head_dim > 128)
+    return 0;
+  efg::DeviceInfo* dev = efg::current_device();
+  return dev ? efg::attn_decode_workspace(type, p, dev->sm_count) : 0;
 }
 
 int efg_attn_paged(int type, void* d_out, const void* d_q, size_t q_stride, const void* d_k_cache,
                    const void* d_v_cache, size_t n_pages, size_t page_size, const int32_t* d_block_table,
                    size_t max_pages, const int32_t* d_cu, const int32_t* d_kv_len, size_t n_seqs, size_t n_rows,
-                   size_t max_new, size_t heads, size_t kv_heads, size_t head_dim, float scale, void* stream) {
+                   size_t max_new, size_t heads, size_t kv_heads, size_t head_dim, float scale, void* d_workspace,
+                   size_t workspace_bytes, void* stream) {
   if (int st = efg::check_attn("attn_paged", type, n_seqs, n_rows, heads, kv_heads, head_dim, q_stride, scale))
     return st;
   if (page_size == 0 || page_size > (1u << 30)) return fail(EFG_EINVAL, "attn_paged: page size %zu", page_size);
@@ -135,13 +158,14 @@ int efg_attn_paged(int type, void* d_out, const void* d_q, size_t q_stride, cons
   p.max_pages = static_cast<int64_t>(max_pages);
   p.page_size = static_cast<int64_t>(page_size);
   p.max_new = static_cast<int64_t>(max_new);
+  p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctzll(page_size) : -1;
   p.heads = static_cast<int>(heads);
   p.kv_heads = static_cast<int>(kv_heads);
   p.group = p.heads / p.kv_heads;
   p.head_dim = static_cast<int>(head_dim);
   p.scale = scale;
   p.err = dev->d_err;
-  return efg::launch_attn(type, p, dev->sm_count, static_cast<cudaStream_t>(stream));
+  return efg::launch_attn(type, p, dev->sm_count, d_workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

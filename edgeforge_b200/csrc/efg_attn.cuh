@@ -21,6 +21,7 @@ struct AttnParams {
   const int32_t* table;      // paged: [n_seqs][max_pages]
   int64_t q_stride, k_stride, v_stride;
   int64_t n_rows, n_seqs, n_pages, max_pages, page_size, max_new;
+  int page_shift;            // page_size = 1 << page_shift, or -1
   int heads, kv_heads, group, head_dim;
   float scale;
   int* err;
@@ -76,12 +77,15 @@ __device__ __forceinline__ void check_offsets(const AttnParams& p) {
 // head_dim elements for pages; -1 where the block table has no valid page (recorded).
 __device__ __forceinline__ int64_t key_row(const AttnParams& p, const Chunk& c, int64_t j) {
   if (!p.kv_len) return c.begin + j;
-  const int32_t page = p.table[c.seq * p.max_pages + j / p.page_size];
+  // a position fits 31 bits, so the division (where the page size is no power of two) is a 32-bit one
+  const uint32_t pos = static_cast<uint32_t>(j), size = static_cast<uint32_t>(p.page_size);
+  const uint32_t pi = p.page_shift >= 0 ? pos >> p.page_shift : pos / size;
+  const int32_t page = p.table[c.seq * p.max_pages + pi];
   if (!page_ok(page, p.n_pages)) {
     record_error(p.err, EFG_EINVAL);
     return -1;
   }
-  return page * p.page_size + j % p.page_size;
+  return page * p.page_size + (pos - pi * size);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -99,6 +103,30 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
+}
+
+// Waits of a CTA for its own copies, MMAs and threads: an error that another CTA recorded (a bad page,
+// say) does not end them, only their own time limit.
+__device__ __forceinline__ bool wait_own(uint64_t* bar, uint32_t parity, int* err) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+#pragma unroll 1
+  for (uint32_t i = 0;; ++i) {
+    if (mbar_try_wait_sleep(bar, parity, 2000u)) return true;
+    if ((i & 15u) == 15u && globaltimer_ns() - t0 > kWaitTimeoutNs) {
+      record_error(err, EFG_ETIMEOUT);
+      return false;
+    }
+  }
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+      : "memory");
 }
 
 // The tile of rows a CTA owns: its sequence and its place among the sequence's tiles.

@@ -1,6 +1,8 @@
 // efg_attn_launch.h - the attention kernels' launchers (efg_attn.cu chooses among them).
 #pragma once
 
+#include <cstddef>
+
 #include <cuda_runtime.h>
 
 namespace efg {
@@ -11,6 +13,12 @@ struct AttnParams;
 // and bases 16-byte aligned.
 bool attn_mma_takes(int type, const AttnParams& p);
 int launch_attn_mma(int type, const AttnParams& p, int sms, cudaStream_t s);
+
+// At most kDecodeRows rows per key head (efg_attn_decode.cu); the workspace joins the parts of long sequences.
+constexpr int kDecodeRows = 16;
+bool attn_decode_takes(int type, const AttnParams& p);
+size_t attn_decode_workspace(int type, const AttnParams& p, int sms);
+int launch_attn_decode(int type, const AttnParams& p, int sms, void* work, cudaStream_t s);
 
 // 5th-generation tensor cores (efg_attn_tc.cu): 16-bit types and more than 64 rows per key head.
 bool attn_tc_takes(int type, const AttnParams& p);

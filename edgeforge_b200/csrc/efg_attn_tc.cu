@@ -48,30 +48,6 @@ constexpr size_t smem_bytes() {
   return 1024 + static_cast<size_t>(2 + kv_stages<D>()) * (D / 64) * kPanel;
 }
 
-// Waits of a CTA for its own copies, MMAs and threads: an error that another CTA recorded (a bad page,
-// say) does not end them, only their own time limit.
-__device__ __forceinline__ bool wait_own(uint64_t* bar, uint32_t parity, int* err) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-#pragma unroll 1
-  for (uint32_t i = 0;; ++i) {
-    if (mbar_try_wait_sleep(bar, parity, 2000u)) return true;
-    if ((i & 15u) == 15u && globaltimer_ns() - t0 > kWaitTimeoutNs) {
-      record_error(err, EFG_ETIMEOUT);
-      return false;
-    }
-  }
-}
-
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z,
-                                            uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
-      : "memory");
-}
-
 // A value tile as the B operand of O += P V: keys run along K, so the tile (rows of keys, 64 dims of 128
 // bytes, 128-byte swizzle) is MN-major: 64-dim panels kPanel apart, groups of 8 keys 1024 bytes apart.
 __device__ __forceinline__ uint64_t desc_values(uint32_t saddr) {
@@ -590,13 +566,13 @@ int launch(const AttnParams& p, int64_t max_new, int64_t max_keys, int sms, cuda
   TcParams tp;
   tp.a = p;
   tp.tokens = kTileRows / p.group;
-  const bool bf16 = std::is_same_v<T, __nv_bfloat16>;
+  const int type = std::is_same_v<T, __nv_bfloat16> ? EFG_BF16 : EFG_F16;
   const int64_t kv_rows = p.kv_len ? p.n_pages * p.page_size : p.n_rows;
   tp.box_rows = p.kv_len ? static_cast<int>(std::min<int64_t>(p.page_size, kTileKeys)) : kTileKeys;
   CUtensorMap mq, mk, mv;
-  if (!encode_heads_map(&mq, bf16, p.q, p.head_dim, p.heads, p.n_rows, p.q_stride, p.group, tp.tokens) ||
-      !encode_heads_map(&mk, bf16, p.k, p.head_dim, p.kv_heads, kv_rows, p.k_stride, 1, tp.box_rows) ||
-      !encode_heads_map(&mv, bf16, p.v, p.head_dim, p.kv_heads, kv_rows, p.v_stride, 1, tp.box_rows))
+  if (!encode_heads_map(&mq, type, p.q, p.head_dim, p.heads, p.n_rows, p.q_stride, p.group, tp.tokens) ||
+      !encode_heads_map(&mk, type, p.k, p.head_dim, p.kv_heads, kv_rows, p.k_stride, 1, tp.box_rows) ||
+      !encode_heads_map(&mv, type, p.v, p.head_dim, p.kv_heads, kv_rows, p.v_stride, 1, tp.box_rows))
     return fail(EFG_ECUDA, "attention: the driver rejects a tensor map");
   const int64_t pair_tokens = 2 * tp.tokens, per_seq = (max_new + pair_tokens - 1) / pair_tokens;
   const int64_t fixed = p.n_seqs * per_seq, bound = p.n_rows / pair_tokens + p.n_seqs;

@@ -140,17 +140,21 @@ bool encode_u64_rows_map(CUtensorMap* m, const void* base, uint64_t rows, uint64
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool encode_heads_map(CUtensorMap* m, bool bf16, const void* base, uint64_t dim, uint64_t heads, uint64_t rows,
+bool encode_heads_map(CUtensorMap* m, int type, const void* base, uint64_t dim, uint64_t heads, uint64_t rows,
                       uint64_t row_stride, uint32_t box_heads, uint32_t box_rows) {
   const EncodeTiledFn fn = encode_tiled();
-  if (!fn || rows == 0 || dim % 8 != 0 || row_stride % 8 != 0 || row_stride == 0 ||
+  const cuuint64_t es = type == EFG_F32 ? 4 : 2;
+  if (!fn || rows == 0 || dim * es % 16 != 0 || row_stride * es % 16 != 0 || row_stride == 0 ||
       reinterpret_cast<uintptr_t>(base) % 16 != 0)
     return false;
   const cuuint64_t dims[3] = {dim, heads, rows};
-  const cuuint64_t strides[2] = {2 * dim, 2 * row_stride};
-  const cuuint32_t box[3] = {64, box_heads, box_rows};
+  const cuuint64_t strides[2] = {es * dim, es * row_stride};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / es), box_heads, box_rows};
   const cuuint32_t estr[3] = {1, 1, 1};
-  return fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base),
+  const CUtensorMapDataType dt = type == EFG_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : type == EFG_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return fn(m, dt, 3, const_cast<void*>(base),
             dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }

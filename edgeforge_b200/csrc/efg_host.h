@@ -52,10 +52,11 @@ int ensure_wide_cluster(const void* fn);
 bool encode_u64_rows_map(CUtensorMap* m, const void* base, uint64_t rows, uint64_t row_bytes, uint32_t box_elems,
                          uint32_t box_rows);
 
-// A 3-D TMA tensor map over `rows` rows of `heads` heads of `dim` 16-bit values (heads back to back,
-// rows row_stride values apart), box {64, box_heads, box_rows}, 128-byte swizzle, zero fill outside.
+// A 3-D TMA tensor map over `rows` rows of `heads` heads of `dim` values of a plain type (heads back to
+// back, rows row_stride values apart), box {128 bytes, box_heads, box_rows}, 128-byte swizzle, zero
+// fill outside.
 // False when the driver rejects it.
-bool encode_heads_map(CUtensorMap* m, bool bf16, const void* base, uint64_t dim, uint64_t heads, uint64_t rows,
+bool encode_heads_map(CUtensorMap* m, int type, const void* base, uint64_t dim, uint64_t heads, uint64_t rows,
                       uint64_t row_stride, uint32_t box_heads, uint32_t box_rows);
 
 // State of the current device, created on first use (allocates the error word).

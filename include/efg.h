@@ -298,8 +298,9 @@ int efg_lm_head_argmax_sharded(int qtype, float* d_logits_shard, int32_t* d_toke
  * outputs are contiguous. Lengths, offsets, pages and slots are read on the device: values that
  * make no sense there read and write nothing out of range, record EFG_EINVAL for
  * efg_device_error and leave the rows that they concern as they were or without a defined
- * value. None of the calls allocates, keeps a workspace or synchronises, so they run on any
- * streams at once and inside CUDA graphs (after one call outside a capture on each device).
+ * value. None of the calls allocates, keeps memory of its own or synchronises, so they run on any
+ * streams at once and inside CUDA graphs (after one call outside a capture on each device); calls
+ * that share a workspace (efg_attn_paged) must not overlap.
  */
 
 /* One step from lengths and a free list. Sequence s holds d_cached[s] tokens in the first
@@ -344,11 +345,18 @@ int efg_attn_prompt(int type, void* d_out, const void* d_q, size_t q_stride, con
  * own keys (stored before, efg_page_store) are the last m positions. m is 1 for a decode step
  * and at most max_new, which sizes the launch; a longer chunk is an error (EFG_EINVAL for
  * efg_device_error). A row that sees no position gets zeros. What lies in the pages behind the
- * last position is never used. Types as efg_attn_prompt, the caches of `type` too. */
+ * last position is never used. Types as efg_attn_prompt, the caches of `type` too.
+ * Long sequences with few new tokens are cut into parts that meet in d_workspace (16-byte aligned
+ * device memory of at least efg_attn_paged_workspace bytes for the same arguments, contents of no
+ * account before and after; NULL when that is 0). */
 int efg_attn_paged(int type, void* d_out, const void* d_q, size_t q_stride, const void* d_k_cache,
                    const void* d_v_cache, size_t n_pages, size_t page_size, const int32_t* d_block_table,
                    size_t max_pages, const int32_t* d_cu, const int32_t* d_kv_len, size_t n_seqs, size_t n_rows,
-                   size_t max_new, size_t heads, size_t kv_heads, size_t head_dim, float scale, void* stream);
+                   size_t max_new, size_t heads, size_t kv_heads, size_t head_dim, float scale, void* d_workspace,
+                   size_t workspace_bytes, void* stream);
+/* Bytes of d_workspace for such a call on the current device. */
+uint64_t efg_attn_paged_workspace(int type, size_t page_size, size_t max_pages, size_t n_seqs, size_t n_rows,
+                                  size_t max_new, size_t heads, size_t kv_heads, size_t head_dim);
 
 /* ================================================================ .efq and the decode step */
 

@@ -141,7 +141,8 @@ def test_c_refusals(efg_lib):
     assert prompt(r=0) == 0 and prompt(n=0) == 0
 
     paged = lambda **k: lib.efg_attn_paged(*{**dict(ty=2, o=P, q=P, qs=512, k=P, v=P, np=16, ps=16, t=P, mp=4, cu=P, kl=P,  # noqa: E731
-                                                    n=1, r=5, mn=5, h=8, kv=2, d=64, sc=0.125, st=None), **k}.values())
+                                                    n=1, r=5, mn=5, h=8, kv=2, d=64, sc=0.125, w=None, wb=0,
+                                                    st=None), **k}.values())
     said(paged(ps=0), "page size 0")
     said(paged(np=2**28), "2^31 slots")
     said(paged(mp=2**28), "2^31 slots")
