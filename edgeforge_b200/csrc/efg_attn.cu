@@ -65,7 +65,7 @@ int check_attn(const char* who, int type, size_t n_seqs, size_t n_rows, size_t h
   if (head_dim == 0 || head_dim > 256) return fail(EFG_EINVAL, "%s: head_dim %zu is not in 1..256", who, head_dim);
   if (kv_heads == 0 || heads == 0 || heads > 4096 || heads % kv_heads)
     return fail(EFG_EINVAL, "%s: %zu query heads do not divide into %zu key heads", who, heads, kv_heads);
-  if (n_rows > 0x7FFFFFFFull || n_seqs > (1ull << 24)) return fail(EFG_EINVAL, "%s: a size is out of range", who);
+  if (n_rows > 0x7FFFFF00ull || n_seqs > (1ull << 24)) return fail(EFG_EINVAL, "%s: a size is out of range", who);
   if (q_stride < heads * head_dim) return fail(EFG_EINVAL, "%s: a row stride is shorter than a row", who);
   if (!(scale == scale) || scale - scale != 0.f) return fail(EFG_EINVAL, "%s: scale is not finite", who);
   return EFG_OK;
@@ -133,7 +133,7 @@ int efg_attn_paged(int type, void* d_out, const void* d_q, size_t q_stride, cons
     return st;
   if (page_size == 0 || page_size > (1u << 30)) return fail(EFG_EINVAL, "attn_paged: page size %zu", page_size);
   if (max_new > 0x7FFFFFFFull) return fail(EFG_EINVAL, "attn_paged: max_new is out of range");
-  if (n_pages > 0x7FFFFFFFull / page_size || max_pages > 0x7FFFFFFFull / page_size)
+  if (n_pages > 0x7FFFFF00ull / page_size || max_pages > 0x7FFFFF00ull / page_size)
     return fail(EFG_EINVAL, "attn_paged: %zu pages (%zu a sequence) of %zu slots pass the 2^31 slots of a cache",
                 n_pages, max_pages, page_size);
   if (n_rows == 0 || n_seqs == 0 || max_new == 0) return EFG_OK;

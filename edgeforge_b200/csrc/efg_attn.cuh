@@ -42,13 +42,15 @@ __device__ __forceinline__ T attn_narrow(float v) {
 
 // The chunk of the packed batch that a row belongs to.
 struct Chunk {
-  int64_t seq, begin, end;  // sequence and its rows [begin, end)
-  int64_t kv_len;           // its positions
+  int32_t seq, begin, end;  // sequence and its rows [begin, end)
+  int32_t kv_len;           // its positions
 };
+
+__device__ __forceinline__ int32_t seen_by(const Chunk& c, int32_t row) { return visible_keys(row, c.end, c.kv_len); }
 
 // False for rows behind the last sequence and for offsets that make no sense (recorded).
 __device__ __forceinline__ bool chunk_of_seq(const AttnParams& p, int64_t s, Chunk& c) {
-  c.seq = s;
+  c.seq = static_cast<int32_t>(s);
   c.begin = p.cu[s];
   c.end = p.cu[s + 1];
   if (c.begin < 0 || c.end > p.n_rows || c.end < c.begin || (p.kv_len && c.end - c.begin > p.max_new)) {
@@ -75,12 +77,12 @@ __device__ __forceinline__ void check_offsets(const AttnParams& p) {
 
 // Offset of the key (stride k_stride) of position j of the chunk's sequence, in rows of kv_heads *
 // head_dim elements for pages; -1 where the block table has no valid page (recorded).
-__device__ __forceinline__ int64_t key_row(const AttnParams& p, const Chunk& c, int64_t j) {
-  if (!p.kv_len) return c.begin + j;
+__device__ __forceinline__ int64_t key_row(const AttnParams& p, const Chunk& c, int32_t j) {
+  if (!p.kv_len) return static_cast<int64_t>(c.begin) + j;
   // a position fits 31 bits, so the division (where the page size is no power of two) is a 32-bit one
   const uint32_t pos = static_cast<uint32_t>(j), size = static_cast<uint32_t>(p.page_size);
   const uint32_t pi = p.page_shift >= 0 ? pos >> p.page_shift : pos / size;
-  const int32_t page = p.table[c.seq * p.max_pages + pi];
+  const int32_t page = p.table[static_cast<int64_t>(c.seq) * p.max_pages + pi];
   if (!page_ok(page, p.n_pages)) {
     record_error(p.err, EFG_EINVAL);
     return -1;
@@ -182,15 +184,15 @@ __device__ bool find_tile(const AttnParams& p, int64_t want, int64_t mul, int64_
 // behind the row's last visible one is never read, so what lies there (stale, infinite or NaN)
 // cannot reach the row. head_dim <= 256; q_s holds the row's query as FP32, scaled to base 2.
 template <typename T>
-__device__ void attend_row(const AttnParams& p, const Chunk& c, int64_t row, int head, float* q_s) {
+__device__ __noinline__ void attend_row(const AttnParams& p, const Chunk& c, int64_t row, int head, float* q_s) {
   const int lane = threadIdx.x & 31, D = p.head_dim, kvh = head / p.group;
-  const int64_t count = visible_keys(row, c.begin, c.end, c.kv_len);
+  const int32_t count = seen_by(c, static_cast<int32_t>(row));
   const T* q = static_cast<const T*>(p.q) + row * p.q_stride + static_cast<int64_t>(head) * D;
   for (int d = lane; d < D; d += 32) q_s[d] = attn_widen(q[d]);
   __syncwarp();
   const float to_base2 = p.scale * 1.4426950408889634f;
   float acc[8] = {}, top = -INFINITY, sum = 0.f;
-  for (int64_t j0 = 0; j0 < count; j0 += 32) {
+  for (int32_t j0 = 0; j0 < count; j0 += 32) {
     int64_t kr = -1;
     float sc = -INFINITY;
     if (j0 + lane < count) kr = key_row(p, c, j0 + lane);
@@ -215,7 +217,7 @@ __device__ void attend_row(const AttnParams& p, const Chunk& c, int64_t row, int
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] *= back;
     top = high;
-    const int n = static_cast<int>(min(static_cast<int64_t>(32), count - j0));
+    const int n = min(32, count - j0);
     for (int t = 0; t < n; ++t) {
       const int64_t vr = __shfl_sync(0xFFFFFFFFu, kr, t);
       const float wt = __shfl_sync(0xFFFFFFFFu, w, t);
@@ -238,10 +240,10 @@ __device__ void attend_row(const AttnParams& p, const Chunk& c, int64_t row, int
 // that was in a tile with positions it sees (up to `end`): 0 times it is NaN in a matrix product.
 // One warp; every lane gets the answer.
 template <typename T>
-__device__ bool reached_from_behind(const AttnParams& p, const Chunk& c, int64_t row, int kvh, int64_t end) {
+__device__ __noinline__ bool reached_from_behind(const AttnParams& p, const Chunk& c, int64_t row, int kvh, int32_t end) {
   const int lane = threadIdx.x & 31;
   bool bad = false;
-  for (int64_t j = visible_keys(row, c.begin, c.end, c.kv_len); j < end; ++j) {
+  for (int32_t j = seen_by(c, static_cast<int32_t>(row)); j < end; ++j) {
     const int64_t vr = key_row(p, c, j);
     if (vr < 0) continue;
     const T* v = static_cast<const T*>(p.v) + vr * p.v_stride + static_cast<int64_t>(kvh) * p.head_dim;

@@ -1,14 +1,15 @@
 // efg_attn_decode.cu - attention of at most 16 rows per key head (a decode step's head group, a few
 // drafted tokens): bound by reading the keys and values once.
 //
-// The keys of a sequence are cut into parts of `chunk` positions; one CTA takes one part of one key
-// head for all of its rows. A producer thread streams 64-key tiles (K, V) through a ring by TMA,
-// page by page, and four consumer warps take 16 keys of every tile each, with their own running
-// maximum and sum, so nothing but the ring's barriers is shared until the end. Partial rows of the
-// warps meet in shared memory; with more than one part they go to the caller's workspace and a second
-// launch (already resident by then: programmatic dependent launch) joins them in part order. The parts
-// have the same size whatever the sequences' lengths are, so ragged batches stay balanced, and they
-// may be any number, so one long sequence still fills every SM.
+// The key tiles (64 positions) of all sequences and key heads form one line (each key head weighs its
+// tiles and what its begin and end cost), which is cut into as many equal runs as there are CTAs resident on the GPU: whatever the lengths are, every SM gets the same
+// bytes, and one long sequence fills the GPU as well as a large ragged batch. A producer warp streams
+// a run's tiles (K, V) through a ring by TMA, page by page, across the borders of sequences; four
+// consumer warps take 16 keys of every tile each, with their own running maximum and sum, so nothing
+// but the ring's barriers is shared until a key head's part of the run ends. Then the warps' rows meet
+// in shared memory. A key head that lies inside one run is written out; the pieces of one that is cut
+// go to the caller's workspace (at most two per CTA) and a second launch, which is resident by then
+// (programmatic dependent launch), joins them in order: no atomics, the same bits on every call.
 //
 // Arithmetic as in efg_attn_mma.cu: 16-bit types by mma m16n8k16; F32 by TF32 parts. Up to 8 rows of
 // F32 fill the 16 rows of the matrix instruction with both parts of the queries (rows 0-7 hi, 8-15 lo):
@@ -26,11 +27,15 @@
 #include "efg_attn_launch.h"
 #include "efg_attn_warp.cuh"
 #include "efg_host.h"
+#include "efg_tcgen05.cuh"
 
 namespace efg {
 namespace {
 
 constexpr int kConsumers = 4, kThreads = 32 * (kConsumers + 1);
+constexpr int kHeadCost = 2;   // what the begin and end of a key head cost, in key tiles
+constexpr int kMinRun = 3;     // weight of a run, at least
+constexpr int kMaxCtas = 1024;
 
 template <typename T, int D>
 struct Shape {
@@ -39,32 +44,41 @@ struct Shape {
   static constexpr int kPanels = D * static_cast<int>(sizeof(T)) / 128;
   static constexpr int kPanelBytes = kKeys * 128;
   static constexpr int kTileBytes = kPanels * kPanelBytes;  // K or V
-  static constexpr int kStages = kTileBytes <= 8192 ? 4 : 2;  // 64 KB a CTA: three CTAs on an SM
-  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * 2 * kTileBytes;
+  // about 64 KB of tiles in flight a CTA, three CTAs on an SM (two for wide heads)
+  static constexpr int kCtas = D == 128 ? 2 : 3;
+  static constexpr int kStages = kTileBytes <= 8192 ? 3 : 2;
+  static constexpr size_t smem(int rows) {  // tiles, then every warp's rows in FP32
+    return 1024 + static_cast<size_t>(kStages) * 2 * kTileBytes + static_cast<size_t>(kConsumers) * rows * D * 4;
+  }
+};
+
+// A cut key head's pieces are slot `first` of CTA i (1: the last part of its run, 0: all of it) and
+// slot 0 of the CTAs behind it.
+struct JoinDesc {
+  int32_t seq, kvh, first, parts;  // parts 0: nothing begins here that is cut
 };
 
 struct DecodeParams {
   AttnParams a;
-  float* work;   // [seq][kv_head][part]{top[16], sum[16], o[16][D]}; null: one part each
-  int chunk;     // positions of a part, a multiple of the tile
-  int parts;     // parts that the grid has for every sequence
-  int box_rows;  // rows of one TMA box
+  JoinDesc* desc;  // [ctas]
+  float* slots;    // [ctas][2]{top[16], sum[16], o[16][D]}; null: key heads are never cut
+  int box_rows;    // rows of one TMA box
 };
 
 // The rows of one sequence under one key head.
 struct Rows {
   Chunk c;
   int rows;                     // packed rows: token * group + head
-  int64_t see_first, see_all;   // keys that the first and the last token see
+  int see_first, see_all;       // keys that the first and the last token see
 };
 
 __device__ __forceinline__ bool rows_of(const AttnParams& p, int64_t seq, Rows& w) {
   if (!chunk_of_seq(p, seq, w.c)) return false;
-  const int64_t m = w.c.end - w.c.begin;
-  if (m == 0 || m * p.group > kDecodeRows) return false;
-  w.rows = static_cast<int>(m) * p.group;
-  w.see_first = visible_keys(w.c.begin, w.c.begin, w.c.end, w.c.kv_len);
-  w.see_all = visible_keys(w.c.end - 1, w.c.begin, w.c.end, w.c.kv_len);
+  const int m = w.c.end - w.c.begin;
+  if (m == 0 || m > kDecodeRows || m * p.group > kDecodeRows) return false;
+  w.rows = m * p.group;
+  w.see_first = seen_by(w.c, w.c.begin);
+  w.see_all = seen_by(w.c, w.c.end - 1);
   return true;
 }
 
@@ -73,26 +87,87 @@ template <typename T>
 __device__ __forceinline__ bool store_row(const AttnParams& p, const Rows& w, int kvh, int r, int d, float v, float l) {
   const int token = r / p.group;
   const float o = l == 0.f ? 0.f : v / l;
-  static_cast<T*>(p.out)[((w.c.begin + token) * p.heads + kvh * p.group + r - token * p.group) * p.head_dim + d] =
+  static_cast<T*>(p.out)[(static_cast<int64_t>(w.c.begin + token) * p.heads + kvh * p.group + r - token * p.group) * p.head_dim + d] =
       attn_narrow<T>(o);
   return !(fabsf(o) <= 3.402823466e38f);
 }
 
 // Rows marked in `redo` once more, alone, where something behind their last position reached them.
+// One warp; scratch holds one query.
 template <typename T>
-__device__ __forceinline__ void redo_rows(const AttnParams& p, const Rows& w, int kvh, const int* redo, float* scratch,
-                                          int warps) {
-  if (w.see_first == w.see_all) return;  // every row sees every key that was used
-  for (int r = threadIdx.x >> 5; r < w.rows; r += warps) {
-    if (!redo[r]) continue;
+__device__ __forceinline__ void redo_rows(const AttnParams& p, const Rows& w, int kvh, const int* redo, float* scratch) {
+  for (int r = 0; r < w.rows; ++r) {
     const int token = r / p.group;
-    if (reached_from_behind<T>(p, w.c, w.c.begin + token, kvh, w.see_all))
-      attend_row<T>(p, w.c, w.c.begin + token, kvh * p.group + r - token * p.group, scratch + (threadIdx.x >> 5) * 256);
+    if (redo[r] && seen_by(w.c, w.c.begin + token) < w.see_all &&
+        reached_from_behind<T>(p, w.c, w.c.begin + token, kvh, w.see_all))
+      attend_row<T>(p, w.c, w.c.begin + token, kvh * p.group + r - token * p.group, scratch);
   }
 }
 
+// The consumer warps alone.
+__device__ __forceinline__ void consumer_barrier() {
+  __syncwarp();
+  asm volatile("bar.sync 1, %0;" ::"n"(32 * kConsumers) : "memory");
+}
+
+// Key tiles of a key head; one that sees nothing has one (its rows are zeros).
+template <typename T, int D>
+__device__ __forceinline__ int tiles_of(const Rows& w) {
+  return max(1, (w.see_all + Shape<T, D>::kKeys - 1) / Shape<T, D>::kKeys);
+}
+
+// Weight of a sequence on the line: of each key head its begin and end, then its tiles; 1 per key head when
+// they are never cut. 0 without new tokens.
+template <typename T, int D>
+__device__ __forceinline__ int64_t weight_of(const DecodeParams& dp, int64_t seq) {
+  Rows w;
+  if (!rows_of(dp.a, seq, w)) return 0;
+  return static_cast<int64_t>(dp.slots ? kHeadCost + tiles_of<T, D>(w) : 1) * dp.a.kv_heads;
+}
+
+// Walks the parts of a run: for each, the sequence, the key head and the tiles [from, to) of it.
+template <typename T, int D>
+struct Walk {
+  int64_t left, at;  // what is left of the run, and the place inside the sequence's weight
+  int seq, kvh, from, to, all;
+  Rows w;
+  bool loaded;
+  __device__ __forceinline__ void start(int64_t s, int64_t place, int64_t count) {
+    seq = static_cast<int>(s);
+    at = place;
+    left = count;
+    loaded = false;
+  }
+  __device__ __forceinline__ bool next(const DecodeParams& dp) {
+    const bool cut = dp.slots != nullptr;
+    while (left > 0) {
+      if (!loaded) {
+        if (seq >= dp.a.n_seqs) return false;  // not reached: runs end with the line
+        loaded = rows_of(dp.a, seq, w);
+        if (loaded) all = tiles_of<T, D>(w);
+      }
+      const int weight = cut ? kHeadCost + all : 1;
+      if (!loaded || at >= static_cast<int64_t>(weight) * dp.a.kv_heads) {
+        ++seq;
+        at = 0;
+        loaded = false;
+        continue;
+      }
+      kvh = static_cast<int>(at / weight);
+      const int off = static_cast<int>(at - static_cast<int64_t>(kvh) * weight);
+      const int step = static_cast<int>(min(static_cast<int64_t>(weight - off), left));
+      left -= step;
+      at += step;
+      from = cut ? max(0, off - kHeadCost) : 0;
+      to = cut ? off + step - kHeadCost : all;
+      if (to > from) return true;  // else the run ends before the head's first tile
+    }
+    return false;
+  }
+};
+
 template <typename T, int D, bool kStack>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && (D == 128 || !kStack) ? 2 : 3)
+__global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : Shape<T, D>::kCtas)
     attn_decode_kernel(const __grid_constant__ DecodeParams dp, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v) {
   using S = Shape<T, D>;
@@ -102,21 +177,25 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && (D == 128 || !kSta
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[S::kStages], empty[S::kStages];
   __shared__ float top_s[kConsumers][16], sum_s[kConsumers][16];
+  __shared__ int64_t scan_s[kThreads / 32], place_s[3];
   __shared__ int redo_s[16];
   const AttnParams& p = dp.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int64_t seq = blockIdx.x / dp.parts;
-  const int part = static_cast<int>(blockIdx.x - seq * dp.parts), kvh = blockIdx.y;
+  const bool cut = dp.slots != nullptr;
   pdl_launch_dependents();
-  Rows w;
-  if (!rows_of(p, seq, w)) return;
-  const int64_t part_begin = static_cast<int64_t>(part) * dp.chunk;
-  if (part > 0 && part_begin >= w.see_all) return;
-  const int tile_begin = static_cast<int>(part_begin / kKeys);
-  const int tile_end = static_cast<int>((min(w.see_all, part_begin + dp.chunk) + kKeys - 1) / kKeys);
-  const uint32_t raw = smem_addr(smem_raw), base = (raw + 1023u) & ~1023u;
-  uint8_t* ring = smem_raw + (base - raw);
 
+  // ---- this CTA's run of the line: every thread adds up a block of sequences, then the one whose block
+  // holds the run's beginning finds the sequence
+  const int64_t per = (p.n_seqs + kThreads - 1) / kThreads, s_lo = min(p.n_seqs, tid * per), s_hi = min(p.n_seqs, s_lo + per);
+  int64_t mine = 0;
+  for (int64_t s = s_lo; s < s_hi; ++s) mine += weight_of<T, D>(dp, s);
+  int64_t inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t up = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+    if (lane >= o) inc += up;
+  }
+  if (lane == 31) scan_s[warp] = inc;
   if (tid == 0) {
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&full[i], 1);
@@ -124,64 +203,97 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && (D == 128 || !kSta
     }
     fence_barrier_init();
   }
-  if (tid < 16) redo_s[tid] = 0;
   __syncthreads();
+  int64_t line = 0, before = inc - mine;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += scan_s[w];
+    line += scan_s[w];
+  }
+  const int64_t runs = min(static_cast<int64_t>(gridDim.x), cut ? max(int64_t{1}, line / kMinRun) : line);
+  if (blockIdx.x >= runs || line == 0) {
+    if (cut && tid == 0) dp.desc[blockIdx.x].parts = 0;
+    return;
+  }
+  const int64_t begin = blockIdx.x * line / runs, end = (blockIdx.x + 1) * line / runs;
+  if (begin >= before && begin < before + mine) {
+    int64_t at = begin - before, s = s_lo;
+    for (int64_t n; (n = weight_of<T, D>(dp, s)) <= at; ++s) at -= n;
+    place_s[0] = s;
+    place_s[1] = at;
+  }
+  __syncthreads();
+  Walk<T, D> walk;
+  walk.start(place_s[0], place_s[1], end - begin);
 
-  float acc[D / 8][4];
-  float top[kHalves], sum[kHalves];
-#pragma unroll
-  for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
-#pragma unroll
-  for (int i = 0; i < kHalves; ++i) top[i] = -INFINITY, sum[i] = 0.f;
+  const uint32_t raw = smem_addr(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* ring = smem_raw + (base - raw);
+  constexpr int kSlabRows = 8 * kHalves;
+  float* o_s = reinterpret_cast<float*>(ring + S::kStages * 2 * S::kTileBytes);  // [warp][kSlabRows][D]
+  int it = 0;  // tiles of the run so far
 
   if (warp == kConsumers) {
     // ---- producer: a lane per box of a tile (page by page), K and V
     const int boxes = kKeys / dp.box_rows, b = lane % boxes, panel = lane / boxes;
-    auto row_of = [&](int tile) -> int32_t {
-      const int64_t pos = static_cast<int64_t>(tile) * kKeys + b * dp.box_rows;
-      if (tile >= tile_end) return 0;
-      if (!p.kv_len) return static_cast<int32_t>(w.c.begin + pos);
-      const int64_t row = pos < w.see_all ? key_row(p, w.c, pos) : -1;
-      return static_cast<int32_t>(row >= 0 ? row : p.n_pages * p.page_size);  // outside: zeros
-    };
-    int32_t row = row_of(tile_begin);
     bool ok = true;
-    int issued = 0;
-    for (int tile = tile_begin; tile < tile_end; ++tile) {
-      const int it = tile - tile_begin, st = it % S::kStages;
-      const int32_t next = row_of(tile + 1);
-      if (it >= S::kStages) ok = wait_own(&empty[st], ((it / S::kStages) - 1) & 1, p.err);
-      ok = __all_sync(0xFFFFFFFFu, ok);
-      if (!ok) break;
-      if (lane == 0) mbar_arrive_expect_tx(&full[st], 2 * S::kTileBytes);
-      __syncwarp();
-      uint8_t* dst = ring + st * 2 * S::kTileBytes + b * dp.box_rows * 128;
-      for (int h = panel; h < S::kPanels; h += 32 / boxes) {
-        constexpr int kPerPanel = 128 / static_cast<int>(sizeof(T));
-        tma_load_3d(dst + h * S::kPanelBytes, &map_k, kPerPanel * h, kvh, row, &full[st]);
-        tma_load_3d(dst + S::kTileBytes + h * S::kPanelBytes, &map_v, kPerPanel * h, kvh, row, &full[st]);
+    while (ok && walk.next(dp)) {
+      const Rows& w = walk.w;
+      auto row_of = [&](int tile) -> int32_t {
+        const int pos = tile * kKeys + b * dp.box_rows;
+        if (tile >= walk.to) return 0;
+        if (!p.kv_len) return static_cast<int32_t>(w.c.begin + pos);
+        const int64_t row = pos < w.see_all ? key_row(p, w.c, pos) : -1;
+        return static_cast<int32_t>(row >= 0 ? row : p.n_pages * p.page_size);  // outside: zeros
+      };
+      int32_t row = row_of(walk.from);
+      for (int tile = walk.from; tile < walk.to; ++tile) {
+        const int st = it % S::kStages;
+        const int32_t next = row_of(tile + 1);
+        if (it >= S::kStages) ok = wait_own(&empty[st], ((it / S::kStages) - 1) & 1, p.err);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], 2 * S::kTileBytes);
+        __syncwarp();
+        uint8_t* dst = ring + st * 2 * S::kTileBytes + b * dp.box_rows * 128;
+        for (int h = panel; h < S::kPanels; h += 32 / boxes) {
+          constexpr int kPerPanel = 128 / static_cast<int>(sizeof(T));
+          tma_load_3d(dst + h * S::kPanelBytes, &map_k, kPerPanel * h, walk.kvh, row, &full[st]);
+          tma_load_3d(dst + S::kTileBytes + h * S::kPanelBytes, &map_v, kPerPanel * h, walk.kvh, row, &full[st]);
+        }
+        ++it;
+        row = next;
       }
-      ++issued;
-      row = next;
     }
     if (!ok)  // the copies in flight land before the shared memory is given back
-      for (int it = max(0, issued - S::kStages); it < issued; ++it)
-        wait_own(&full[it % S::kStages], (it / S::kStages) & 1, p.err);
-  } else {
+      for (int i = max(0, it - S::kStages); i < it; ++i) wait_own(&full[i % S::kStages], (i / S::kStages) & 1, p.err);
+    return;
+  }
+
+  const float scale2 = p.scale * 1.4426950408889634f;
+  const int key0 = warp * kWarpKeys, perm = (g >> 1) + 4 * (g & 1);
+  bool ok = true, owner = false, first_part = true;
+  while (walk.next(dp)) {
+    const Rows& w = walk.w;
+    const int kvh = walk.kvh;
+    float acc[D / 8][4];
+    float top[kHalves], sum[kHalves];
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kHalves; ++i) top[i] = -INFINITY, sum[i] = 0.f;
     // ---- queries as A fragments
     const T* qrow[2];
-    int64_t sees[kHalves];
+    int sees[kHalves];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = kStack ? g : g + 8 * i;
       const int token = r / p.group;
       const bool live = r < w.rows;
-      qrow[i] = live ? static_cast<const T*>(p.q) + (w.c.begin + token) * p.q_stride +
+      qrow[i] = live ? static_cast<const T*>(p.q) + static_cast<int64_t>(w.c.begin + token) * p.q_stride +
                            static_cast<int64_t>(kvh * p.group + r - token * p.group) * p.head_dim
                      : nullptr;
-      if (i < kHalves) sees[i] = live ? visible_keys(w.c.begin + token, w.c.begin, w.c.end, w.c.kv_len) : 0;
+      if (i < kHalves) sees[i] = live ? seen_by(w.c, w.c.begin + token) : 0;
     }
     uint32_t qa[kF32 ? 1 : KK][4], qs[kStack ? KK : 1][2][4];
     float4 qf[kF32 && !kStack ? KK : 1][2];
@@ -210,24 +322,23 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && (D == 128 || !kSta
         }
       }
     }
-    const float scale2 = p.scale * 1.4426950408889634f;
-    const int key0 = warp * kWarpKeys, perm = (g >> 1) + 4 * (g & 1);
-    bool ok = true;
 
-    for (int tile = tile_begin; tile < tile_end; ++tile) {
-      const int it = tile - tile_begin, st = it % S::kStages;
-      ok = wait_own(&full[st], (it / S::kStages) & 1, p.err);
-      if (!__all_sync(0xFFFFFFFFu, ok)) break;
+    for (int tile = walk.from; tile < walk.to; ++tile, ++it) {
+      const int st = it % S::kStages;
+      if (ok) ok = wait_own(&full[st], (it / S::kStages) & 1, p.err);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) continue;  // a wait gave up (recorded): no more work, but every barrier below is met
       const uint32_t ks = base + static_cast<uint32_t>(st) * (2 * S::kTileBytes), vs = ks + S::kTileBytes;
-      const int64_t j0 = static_cast<int64_t>(tile) * kKeys + key0;
+      const int j0 = tile * kKeys + key0;
       if (j0 + kWarpKeys > w.see_all) {
         // values behind the last position become zeros: 0 times what may lie there need not be 0
-        const int keep = static_cast<int>(max(int64_t{0}, w.see_all - j0));
+        const int keep = max(0, w.see_all - j0);
         for (int e = lane; e < (kWarpKeys - keep) * S::kPanels * 8; e += 32) {
           const int r = key0 + keep + e / (S::kPanels * 8), h = (e / 8) % S::kPanels;
           *reinterpret_cast<uint4*>(ring + (vs - base) + h * S::kPanelBytes + r * 128 + (e % 8) * 16) =
               make_uint4(0, 0, 0, 0);
         }
+        fence_proxy_async();  // before the copy that fills this stage again
         __syncwarp();
       }
       float s[NT][4], s2[kStack ? NT : 1][4];
@@ -296,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && (D == 128 || !kSta
       const bool edge = j0 + kWarpKeys > w.see_first;
 #pragma unroll
       for (int i = 0; i < kHalves; ++i) {
-        const int limit = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(kWarpKeys), sees[i] - j0)));
+        const int limit = sees[i] - j0;
         float mx = top[i];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -386,11 +497,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && (D == 128 || !kSta
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[st]);
     }
-  }
-  __syncthreads();  // the ring becomes the exchange area: [warp][16][D]
-
-  float* o_s = reinterpret_cast<float*>(ring);
-  if (warp < kConsumers) {
+    // ---- the warps' rows meet
+    consumer_barrier();  // the rows of the part before have been read
 #pragma unroll
     for (int i = 0; i < kHalves; ++i) {
       float v = sum[i];
@@ -400,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && (D == 128 || !kSta
         top_s[warp][g + 8 * i] = top[i];
         sum_s[warp][g + 8 * i] = v;
       }
-      float* o = o_s + (warp * 16 + g + 8 * i) * D;
+      float* o = o_s + (warp * kSlabRows + g + 8 * i) * D;
 #pragma unroll
       for (int n = 0; n < D / 8; ++n)
 #pragma unroll
@@ -409,117 +517,124 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && (D == 128 || !kSta
           o[d] = kStack ? acc[n][e] + acc[n][e + 2] : acc[n][2 * i + e];
         }
     }
-  }
-  __syncthreads();
-  const bool joined = dp.work && w.see_all > dp.chunk;  // more than one part: the second launch joins them
-  float* slot = joined ? dp.work + ((seq * p.kv_heads + kvh) * dp.parts + part) * (16 * (D + 2)) : nullptr;
-  for (int e = tid; e < w.rows * D; e += kThreads) {
-    const int r = e / D, d = e % D;
-    float mx = top_s[0][r];
+    const bool whole = walk.from == 0 && walk.to == walk.all, uneven = whole && w.see_first < w.see_all;
+    if (uneven && tid < 16) redo_s[tid] = 0;
+    consumer_barrier();
+    float* slot = whole ? nullptr : dp.slots + (static_cast<int64_t>(blockIdx.x) * 2 + (first_part ? 0 : 1)) * (16 * (D + 2));
+    for (int e = tid; e < w.rows * D; e += 32 * kConsumers) {
+      const int r = e / D, d = e % D;
+      float mx = top_s[0][r];
 #pragma unroll
-    for (int x = 1; x < kConsumers; ++x) mx = fmaxf(mx, top_s[x][r]);
-    const float ref = mx == -INFINITY ? 0.f : mx;
-    float v = 0.f, l = 0.f;
+      for (int x = 1; x < kConsumers; ++x) mx = fmaxf(mx, top_s[x][r]);
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      float v = 0.f, l = 0.f;
 #pragma unroll
-    for (int x = 0; x < kConsumers; ++x) {
-      const float f = ex2(top_s[x][r] - ref);
-      v += f * o_s[(x * 16 + r) * D + d];
-      l += f * sum_s[x][r];
-    }
-    if (joined) {
-      slot[32 + e] = v;
-      if (d == 0) {
-        slot[r] = mx;
-        slot[16 + r] = l;
+      for (int x = 0; x < kConsumers; ++x) {
+        const float f = ex2(top_s[x][r] - ref);
+        v += f * o_s[x * kSlabRows * D + e];
+        l += f * sum_s[x][r];
       }
-    } else if (d < p.head_dim) {
-      if (store_row<T>(p, w, kvh, r, d, v, l)) redo_s[r] = 1;
+      if (!whole) {
+        slot[32 + e] = v;
+        if (d == 0) {
+          slot[r] = mx;
+          slot[16 + r] = l;
+        }
+      } else if (d < p.head_dim) {
+        if (store_row<T>(p, w, kvh, r, d, v, l) && uneven) redo_s[r] = 1;
+      }
     }
+    if (uneven) {
+      consumer_barrier();
+      if (warp == 0) redo_rows<T>(p, w, kvh, redo_s, o_s);
+    }
+    if (warp == 0) {
+      if (!whole && walk.from == 0) {  // a key head that is cut begins here: its last piece is in another run
+        const int64_t last = end - 1 + (walk.all - walk.to);
+        const int64_t cta = ((last + 1) * runs - 1) / line;
+        owner = true;
+        if (lane == 0)
+          dp.desc[blockIdx.x] = JoinDesc{static_cast<int32_t>(walk.seq), kvh, first_part ? 0 : 1,
+                                         static_cast<int32_t>(cta - blockIdx.x + 1)};
+      }
+    }
+    first_part = false;
   }
-  if (!joined) {
-    __syncthreads();
-    redo_rows<T>(p, w, kvh, redo_s, o_s, kThreads / 32);
-  }
+  if (cut && tid == 0 && !owner) dp.desc[blockIdx.x].parts = 0;
 }
 
-// Joins the parts of one sequence and key head: out = sum_x 2^(top_x - top) o_x / sum_x 2^(top_x - top) l_x.
+// Joins the pieces of the key head whose first piece is at the end of CTA blockIdx.x's run:
+// out = sum_x 2^(top_x - top) o_x / sum_x 2^(top_x - top) l_x. Rows blockIdx.y, blockIdx.y + gridDim.y, ..
 template <typename T, int D>
 __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ DecodeParams dp) {
-  __shared__ float scratch[4 * 256];
+  constexpr int kGroups = 128 / (D / 4);  // threads of one group read one piece's row, 16 bytes each
+  __shared__ float weight[kMaxCtas], part[kGroups][D], red[8];
   __shared__ int redo_s[16];
   const AttnParams& p = dp.a;
-  const int64_t seq = blockIdx.x;
-  const int kvh = blockIdx.y;
-  if (threadIdx.x < 16) redo_s[threadIdx.x] = 0;
-  __syncthreads();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = tid / (D / 4), d = tid % (D / 4) * 4;
+  if (tid < 16) redo_s[tid] = 0;
   pdl_wait();
+  const JoinDesc j = dp.desc[blockIdx.x];
+  if (j.parts <= 1) return;
   Rows w;
-  if (!rows_of(p, seq, w) || w.see_all <= dp.chunk) return;
-  const int parts = static_cast<int>((w.see_all + dp.chunk - 1) / dp.chunk);
-  const float* slots = dp.work + (seq * p.kv_heads + kvh) * dp.parts * static_cast<int64_t>(16 * (D + 2));
-  const int r0 = blockIdx.z * 4, r = r0 + (threadIdx.x >> 5), lane = threadIdx.x & 31;  // one warp per row
-  if (r < w.rows) {
-    float mx = -INFINITY;
-    for (int x = lane; x < parts; x += 32) mx = fmaxf(mx, slots[static_cast<int64_t>(x) * (16 * (D + 2)) + r]);
+  if (!rows_of(p, j.seq, w)) return;
+  constexpr int64_t kSlot = 16 * (D + 2);
+  auto slot = [&](int x) { return dp.slots + ((static_cast<int64_t>(blockIdx.x) + x) * 2 + (x == 0 ? j.first : 0)) * kSlot; };
+  for (int r = blockIdx.y; r < w.rows; r += gridDim.y) {
+    float mx = -INFINITY, l = 0.f;
+    for (int x = tid; x < j.parts; x += 128) mx = fmaxf(mx, slot(x)[r]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+    if (lane == 0) red[warp] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     const float ref = mx == -INFINITY ? 0.f : mx;
-    float l = 0.f, acc[D / 32] = {};
-    for (int x0 = 0; x0 < parts; x0 += 32) {  // weights of 32 parts at once, then their values in order
-      const float* mine = slots + static_cast<int64_t>(x0 + lane) * (16 * (D + 2));
-      const float f = x0 + lane < parts ? ex2(mine[r] - ref) : 0.f;
-      const float fl = x0 + lane < parts ? f * mine[16 + r] : 0.f;
-      const int n = min(32, parts - x0);
-#pragma unroll 4
-      for (int x = 0; x < n; ++x) {
-        const float* o = slots + static_cast<int64_t>(x0 + x) * (16 * (D + 2)) + 32 + r * D;
-        const float fx = __shfl_sync(0xFFFFFFFFu, f, x);
-        l += __shfl_sync(0xFFFFFFFFu, fl, x);
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) acc[i] += fx * o[lane + 32 * i];
-      }
+    for (int x = tid; x < j.parts; x += 128) {
+      const float f = ex2(slot(x)[r] - ref);
+      weight[x] = f;
+      l += f * slot(x)[16 + r];
     }
+    l = warp_sum(l);
+    if (lane == 0) red[4 + warp] = l;
+    __syncthreads();
+    l = (red[4] + red[5]) + (red[6] + red[7]);
+    float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int x = group; x < j.parts; x += kGroups) {
+      const float4 v = *reinterpret_cast<const float4*>(slot(x) + 32 + r * D + d);
+      const float f = weight[x];
+      acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+    }
+    *reinterpret_cast<float4*>(&part[group][d]) = acc;
+    __syncthreads();
+    if (tid < D && tid < p.head_dim) {
+      float v = 0.f;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-      if (lane + 32 * i < p.head_dim && store_row<T>(p, w, kvh, r, lane + 32 * i, acc[i], l)) redo_s[r] = 1;
+      for (int x = 0; x < kGroups; ++x) v += part[x][tid];
+      if (store_row<T>(p, w, j.kvh, r, tid, v, l)) redo_s[r] = 1;
+    }
+    __syncthreads();
+    if (warp == 0 && redo_s[r]) {
+      redo_rows<T>(p, w, j.kvh, redo_s, weight);
+      __syncwarp();
+      if (lane == 0) redo_s[r] = 0;
+    }
+    __syncthreads();
   }
-  __syncwarp();
-  if (r < w.rows && redo_s[r] && w.see_first < w.see_all) {
-    const int token = r / p.group;
-    if (reached_from_behind<T>(p, w.c, w.c.begin + token, kvh, w.see_all))
-      attend_row<T>(p, w.c, w.c.begin + token, kvh * p.group + r - token * p.group, scratch + (threadIdx.x >> 5) * 256);
-  }
-}
-
-// How a call is cut: positions of a part and parts per sequence.
-struct Cut {
-  int chunk, parts;
-};
-Cut cut_of(int type, const AttnParams& p, int sms) {
-  const int es = type == EFG_F32 ? 4 : 2, D = p.head_dim <= 64 ? 64 : 128;
-  const int64_t max_keys = std::max<int64_t>(1, p.kv_len ? p.max_pages * p.page_size : p.n_rows);
-  // Three CTAs on every SM when all sequences are as long as the table allows; but not below 128 positions
-  // (a CTA's start and end cost as much as that) and not above 512 KB, which keeps ragged batches balanced.
-  const int64_t even = (max_keys * p.n_seqs * p.kv_heads + 3 * sms - 1) / (3 * sms);
-  const int64_t chunk = (std::max<int64_t>(128, std::min<int64_t>(even, (512 << 10) / (2 * D * es))) + 63) / 64 * 64;
-  return Cut{static_cast<int>(chunk), static_cast<int>((max_keys + chunk - 1) / chunk)};
 }
 
 template <typename T, int D, bool kStack>
-int launch(const DecodeParams& dp, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t s) {
+int launch(const DecodeParams& dp, const CUtensorMap& mk, const CUtensorMap& mv, int ctas, cudaStream_t s) {
   using S = Shape<T, D>;
   const auto fn = attn_decode_kernel<T, D, kStack>;
-  if (int st = ensure_smem_attr(reinterpret_cast<const void*>(fn), S::kSmem)) return st;
+  if (int st = ensure_smem_attr(reinterpret_cast<const void*>(fn), S::smem(kStack ? 8 : 16))) return st;
   const AttnParams& p = dp.a;
-  if (p.n_seqs * dp.parts > 0x7FFFFFFFll) return fail(EFG_EINVAL, "attention: too many rows");
-  fn<<<dim3(static_cast<unsigned>(p.n_seqs * dp.parts), static_cast<unsigned>(p.kv_heads)), kThreads, S::kSmem, s>>>(
-      dp, mk, mv);
+  fn<<<static_cast<unsigned>(ctas), kThreads, S::smem(kStack ? 8 : 16), s>>>(dp, mk, mv);
   EFG_TRY_CUDA(cudaGetLastError(), "attention launch");
-  if (!dp.work) return EFG_OK;
+  if (!dp.slots) return EFG_OK;
   cudaLaunchConfig_t cf{};
   const int64_t rows = std::min<int64_t>(kDecodeRows, std::min(p.kv_len ? p.max_new : p.n_rows, p.n_rows) * p.group);
-  cf.gridDim = dim3(static_cast<unsigned>(p.n_seqs), static_cast<unsigned>(p.kv_heads),
-                    static_cast<unsigned>((rows + 3) / 4));
+  cf.gridDim = dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(std::min<int64_t>(rows, 4)));
   cf.blockDim = dim3(128);
   cf.stream = s;
   cudaLaunchAttribute attr[1];
@@ -531,14 +646,22 @@ int launch(const DecodeParams& dp, const CUtensorMap& mk, const CUtensorMap& mv,
   return EFG_OK;
 }
 
+int64_t max_keys_of(const AttnParams& p) { return p.kv_len ? p.max_pages * p.page_size : p.n_rows; }
+
+// Whether key heads may be cut: not when each is at most a few tiles.
+bool cuts(const AttnParams& p) { return max_keys_of(p) > kMinRun * 64; }
+
+int ctas_of(const AttnParams& p, int sms) { return std::min(kMaxCtas, (p.head_dim <= 64 ? 3 : 2) * sms); }
+
 template <typename T, int D>
-int dispatch(int type, const AttnParams& p, const Cut& cut, void* work, cudaStream_t s) {
+int dispatch(int type, const AttnParams& p, int sms, void* work, cudaStream_t s) {
   using S = Shape<T, D>;
+  static_assert(S::kCtas == (D == 64 ? 3 : 2));
+  const int ctas = ctas_of(p, sms);
   DecodeParams dp;
   dp.a = p;
-  dp.work = cut.parts > 1 ? static_cast<float*>(work) : nullptr;
-  dp.chunk = cut.chunk;
-  dp.parts = cut.parts;
+  dp.desc = static_cast<JoinDesc*>(work);
+  dp.slots = cuts(p) ? reinterpret_cast<float*>(dp.desc + ctas) : nullptr;
   dp.box_rows = p.kv_len ? static_cast<int>(std::min<int64_t>(p.page_size, S::kKeys)) : S::kKeys;
   const int64_t kv_rows = p.kv_len ? p.n_pages * p.page_size : p.n_rows;
   CUtensorMap mk, mv;
@@ -546,9 +669,9 @@ int dispatch(int type, const AttnParams& p, const Cut& cut, void* work, cudaStre
       !encode_heads_map(&mv, type, p.v, p.head_dim, p.kv_heads, kv_rows, p.v_stride, 1, dp.box_rows))
     return fail(EFG_ECUDA, "attention: the driver rejects a tensor map");
   if constexpr (S::kF32) {
-    if (std::min(p.kv_len ? p.max_new : p.n_rows, p.n_rows) * p.group <= 8) return launch<T, D, true>(dp, mk, mv, s);
+    if (std::min(p.kv_len ? p.max_new : p.n_rows, p.n_rows) * p.group <= 8) return launch<T, D, true>(dp, mk, mv, ctas, s);
   }
-  return launch<T, D, false>(dp, mk, mv, s);
+  return launch<T, D, false>(dp, mk, mv, ctas, s);
 }
 
 }  // namespace
@@ -560,20 +683,16 @@ bool attn_decode_takes(int type, const AttnParams& p) {
   return attn_mma_takes(type, p) && max_new * p.group <= kDecodeRows;
 }
 
-size_t attn_decode_workspace(int type, const AttnParams& p, int sms) {
-  const Cut cut = cut_of(type, p, sms);
-  if (cut.parts <= 1) return 0;
-  return static_cast<size_t>(p.n_seqs) * p.kv_heads * cut.parts * 16 * ((p.head_dim <= 64 ? 64 : 128) + 2) * sizeof(float);
+size_t attn_decode_workspace(int, const AttnParams& p, int sms) {
+  if (!cuts(p)) return 0;
+  return static_cast<size_t>(ctas_of(p, sms)) * (sizeof(JoinDesc) + 2 * 16 * ((p.head_dim <= 64 ? 64 : 128) + 2) * sizeof(float));
 }
 
 int launch_attn_decode(int type, const AttnParams& p, int sms, void* work, cudaStream_t s) {
-  const Cut cut = cut_of(type, p, sms);
   const bool small = p.head_dim <= 64;
-  if (type == EFG_F32)
-    return small ? dispatch<float, 64>(type, p, cut, work, s) : dispatch<float, 128>(type, p, cut, work, s);
-  if (type == EFG_F16)
-    return small ? dispatch<__half, 64>(type, p, cut, work, s) : dispatch<__half, 128>(type, p, cut, work, s);
-  return small ? dispatch<__nv_bfloat16, 64>(type, p, cut, work, s) : dispatch<__nv_bfloat16, 128>(type, p, cut, work, s);
+  if (type == EFG_F32) return small ? dispatch<float, 64>(type, p, sms, work, s) : dispatch<float, 128>(type, p, sms, work, s);
+  if (type == EFG_F16) return small ? dispatch<__half, 64>(type, p, sms, work, s) : dispatch<__half, 128>(type, p, sms, work, s);
+  return small ? dispatch<__nv_bfloat16, 64>(type, p, sms, work, s) : dispatch<__nv_bfloat16, 128>(type, p, sms, work, s);
 }
 
 }  // namespace efg

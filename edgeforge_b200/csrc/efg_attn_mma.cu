@@ -97,19 +97,19 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
   }
   Chunk c;
   if (!chunk_of_seq(p, rt.seq, c)) return;
-  const int64_t m = c.end - c.begin, row0 = rt.index * kRows;  // packed rows of this tile: row0 ..
+  const int64_t m = c.end - c.begin;
+  const int64_t row0 = rt.index * kRows;  // packed rows of this tile: row0 ..
   if (row0 >= m * p.group) return;
   const int64_t rows_here = min(static_cast<int64_t>(kRows), m * p.group - row0);
-  const int64_t first_token = row0 / p.group, last_token = (row0 + rows_here - 1) / p.group;
-  const int64_t see_first = visible_keys(c.begin + first_token, c.begin, c.end, c.kv_len);
-  const int64_t see_all = visible_keys(c.begin + last_token, c.begin, c.end, c.kv_len);
+  const int first_token = static_cast<int>(row0 / p.group), last_token = static_cast<int>((row0 + rows_here - 1) / p.group);
+  const int see_first = seen_by(c, c.begin + first_token), see_all = seen_by(c, c.begin + last_token);
   const int tiles = static_cast<int>((see_all + kKeys - 1) / kKeys);
   const int tile_begin = static_cast<int>(static_cast<int64_t>(tiles) * rank / splits);
   const int tile_end = static_cast<int>(static_cast<int64_t>(tiles) * (rank + 1) / splits);
 
   // ---- this warp's rows
   const int wrow = MT == 1 ? 0 : warp * 16;
-  int64_t sees[2];  // rows g and g + 8 of the warp
+  int sees[2];  // rows g and g + 8 of the warp
   const T* qrow[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
     if (r < rows_here) {
       const int64_t token = (row0 + r) / p.group;
       const int head = kvh * p.group + static_cast<int>(row0 + r - token * p.group);
-      sees[i] = visible_keys(c.begin + token, c.begin, c.end, c.kv_len);
+      sees[i] = seen_by(c, c.begin + static_cast<int>(token));
       qrow[i] = static_cast<const T*>(p.q) + (c.begin + token) * p.q_stride + static_cast<int64_t>(head) * p.head_dim;
     } else {
       sees[i] = 0;
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
 
   // ---- key slots of a tile, one thread per key: looked up a tile ahead of its copies
   auto slot_of = [&](int tile) -> int32_t {
-    const int64_t j = static_cast<int64_t>(tile) * kKeys + tid;
+    const int j = tile * kKeys + tid;
     if (tile >= tile_end || j >= see_all) return -1;
     return static_cast<int32_t>(key_row(p, c, j));
   };
@@ -241,11 +241,11 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
       }
     }
     // ---- softmax of this tile (base 2), rows g and g + 8
-    const int64_t j0 = static_cast<int64_t>(tile) * kKeys + key0;
+    const int j0 = tile * kKeys + key0;
     const bool edge = j0 + 8 * NT > see_first;  // some row does not see all of these keys
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int limit = static_cast<int>(max(static_cast<int64_t>(-1), min(static_cast<int64_t>(kKeys), sees[i] - j0)));
+      const int limit = sees[i] - j0;
       float mx = top[i];
 #pragma unroll
       for (int n = 0; n < NT; ++n)

@@ -181,24 +181,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   Chunk c;
   if (!chunk_of_seq(p, rt.seq, c)) return;
-  const int64_t m = c.end - c.begin, token0 = rt.index * 2 * tp.tokens;
-  if (token0 >= m) return;
+  const int m = c.end - c.begin;
+  if (rt.index * 2 * tp.tokens >= m) return;
+  const int token0 = static_cast<int>(rt.index) * 2 * tp.tokens;
   // tokens of the two row tiles, the keys that their last token sees, and tiles of keys of this CTA
   int tok[2], n[2];
-  int64_t see_last[2], see_all = 0;
+  int see_last[2], see_all = 0;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    tok[i] = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(tp.tokens), m - token0 - i * tp.tokens)));
-    see_last[i] = tok[i] ? visible_keys(c.begin + token0 + i * tp.tokens + tok[i] - 1, c.begin, c.end, c.kv_len) : 0;
+    tok[i] = max(0, min(tp.tokens, m - token0 - i * tp.tokens));
+    see_last[i] = tok[i] ? seen_by(c, c.begin + token0 + i * tp.tokens + tok[i] - 1) : 0;
     see_all = max(see_all, see_last[i]);
   }
-  const int tiles = static_cast<int>((see_all + kTileKeys - 1) / kTileKeys);
+  const int tiles = (see_all + kTileKeys - 1) / kTileKeys;
   const int tile_begin = static_cast<int>(static_cast<int64_t>(tiles) * rank / splits);
   const int tile_end = static_cast<int>(static_cast<int64_t>(tiles) * (rank + 1) / splits);
   const int count = tile_end - tile_begin;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    n[i] = max(0, min(tile_end, static_cast<int>((see_last[i] + kTileKeys - 1) / kTileKeys)) - tile_begin);
+    n[i] = max(0, min(tile_end, (see_last[i] + kTileKeys - 1) / kTileKeys) - tile_begin);
 
   const uint32_t raw = smem_addr(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* q_s = smem_raw + (base - raw);
@@ -233,15 +234,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < live; ++i)
           for (int h = 0; h < kPanels; ++h)
             tma_load_3d(q_s + (i * kPanels + h) * kPanel, &map_q, 64 * h, kvh * p.group,
-                        static_cast<int32_t>(c.begin + token0 + i * tp.tokens), &q_full);
+                        c.begin + token0 + i * tp.tokens, &q_full);
       }
       const int boxes = kTileKeys / tp.box_rows, b = lane % boxes, panel = lane / boxes;
       const bool mine = lane < boxes * kPanels;
       // first row of this lane's box in the tensor; outside of it (zero fill) behind the last position
       auto row_of = [&](int tile) -> int32_t {
-        const int64_t pos = static_cast<int64_t>(tile) * kTileKeys + b * tp.box_rows;
+        const int pos = tile * kTileKeys + b * tp.box_rows;
         if (!mine || tile >= tile_end) return 0;
-        if (!p.kv_len) return static_cast<int32_t>(c.begin + pos);
+        if (!p.kv_len) return c.begin + pos;
         const int64_t none = p.n_pages * p.page_size;
         const int64_t row = pos < see_all ? key_row(p, c, pos) : -1;
         return static_cast<int32_t>(row >= 0 ? row : none);
@@ -331,10 +332,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_addr = tmem + lanes + 128 * i, o_addr = tmem + lanes + 256 + D * i;
     const int token = r / p.group;  // of the row tile
     const bool live = token < tok[i];
-    const int64_t sees =
-        live ? visible_keys(c.begin + token0 + i * tp.tokens + token, c.begin, c.end, c.kv_len) : int64_t{0};
-    const int64_t see_first =
-        tok[i] ? visible_keys(c.begin + token0 + i * tp.tokens, c.begin, c.end, c.kv_len) : int64_t{0};
+    const int sees = live ? seen_by(c, c.begin + token0 + i * tp.tokens + token) : 0;
+    const int see_first = tok[i] ? seen_by(c, c.begin + token0 + i * tp.tokens) : 0;
     const float scale2 = p.scale * 1.4426950408889634f;
     const uint64_t scale_pair = pair(scale2, scale2);
     uint64_t total = pair(0.f, 0.f);
@@ -350,10 +349,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_wait_ld();
 #pragma unroll
       for (int q = 0; q < 4; ++q) after_wait(s + 32 * q);
-      const int64_t key0 = static_cast<int64_t>(tile_begin + j) * kTileKeys;
+      const int key0 = (tile_begin + j) * kTileKeys;
       const bool edge = key0 + kTileKeys > see_first;
       if (edge) {
-        const int limit = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(kTileKeys), sees - key0)));
+        const int limit = sees - key0;
 #pragma unroll
         for (int k = 0; k < 128; ++k)
           if (k >= limit) s[k] = 0xFF800000u;  // -inf
@@ -551,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int rr = r_lo + x, ti = rr >> 7, tr = rr & 127, tt = tr / p.group;
         if (tt >= tok[ti] || !redo_s[rr]) continue;
         const int64_t row = c.begin + token0 + ti * tp.tokens + tt;
-        if (visible_keys(row, c.begin, c.end, c.kv_len) < see_all && reached_from_behind<T>(p, c, row, kvh, see_all))
+        if (seen_by(c, static_cast<int>(row)) < see_all && reached_from_behind<T>(p, c, row, kvh, see_all))
           attend_row<T>(p, c, row, kvh * p.group + tr - tt * p.group, scratch);
       }
     }

@@ -44,11 +44,11 @@ EFG_HD bool seq_served(const SeqNeed& n, int64_t first, int64_t n_free) {
 
 EFG_HD bool page_ok(int32_t page, int64_t n_pages) { return page >= 0 && page < n_pages; }
 
-// The keys that row `row` of the packed batch sees: positions [0, count) of its sequence, whose
-// chunk is rows [begin, end) and whose cache holds kv_len positions with the chunk at the end.
+// The keys that row `row` of the packed batch sees: positions [0, count) of its sequence, whose chunk
+// ends before row `end` and whose cache holds kv_len positions with the chunk at the end.
 // 0 when the row sees nothing (more rows than positions).
-EFG_HD int64_t visible_keys(int64_t row, int64_t begin, int64_t end, int64_t kv_len) {
-  const int64_t n = kv_len - (end - begin) + (row - begin) + 1;
+EFG_HD int32_t visible_keys(int32_t row, int32_t end, int32_t kv_len) {
+  const int32_t n = kv_len - (end - row) + 1;  // 0 <= kv_len <= 2^31 - 256, row < end
   return n > 0 ? n : 0;
 }
 

@@ -326,6 +326,12 @@ def test_bad_pages_lengths_and_chunks_are_recorded(cuda, kind, m):
     q, kc, vc, table, cu, kv_len = args
     good = out.clone()
 
+    def _check_rows(o, which):
+        for s in which:
+            k, v = seqs[s]
+            want = attend(_d(q[m * s : m * s + m]), _d(k), _d(v), float(np.float32(64**-0.5)))
+            _held(kind, _d(o)[m * s : m * s + m], *want)
+
     def again(table=table, cu=cu, kv_len=kv_len, max_new=m):
         o = torch.full_like(out, 7.0)
         efg.attn_paged(o, q, kc, vc, table, cu, kv_len, max_new)
@@ -341,7 +347,8 @@ def test_bad_pages_lengths_and_chunks_are_recorded(cuda, kind, m):
     for n in (-3, 10**6, 2**31 - 1):
         l = kv_len.clone()
         l[0] = n
-        assert torch.equal(again(kv_len=l)[m:], good[m:])
+        # (the work is cut up differently without the first sequence: the same values, not the same bits)
+        _check_rows(again(kv_len=l), (1, 2))
     if m > 1:
         again(max_new=m - 1)
     again(cu=_i(torch, [0, m, 5 * m, 3 * m]))

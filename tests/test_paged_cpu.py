@@ -24,7 +24,7 @@ int served(int64_t need, int valid, int64_t first, int64_t n_free) {
   return seq_served(SeqNeed{0, 0, need, valid != 0}, first, n_free);
 }
 int ok(int32_t page, int64_t n) { return page_ok(page, n); }
-int64_t visible(int64_t r, int64_t b, int64_t e, int64_t k) { return visible_keys(r, b, e, k); }
+int32_t visible(int32_t r, int32_t e, int32_t k) { return visible_keys(r, e, k); }
 int64_t find(const int32_t* cu, int64_t n, int64_t row) { return find_sequence(cu, n, row); }
 }
 """
@@ -42,7 +42,7 @@ def host(tmp_path_factory):
     lib.need.argtypes = [C.c_int32, C.c_int32, i64, i64, C.c_void_p]
     lib.served.argtypes = [i64, C.c_int, i64, i64]
     lib.ok.argtypes = [C.c_int32, i64]
-    lib.visible.argtypes, lib.visible.restype = [i64] * 4, i64
+    lib.visible.argtypes, lib.visible.restype = [C.c_int32] * 3, C.c_int32
     lib.find.argtypes, lib.find.restype = [C.c_void_p, i64, i64], i64
     return lib
 
@@ -69,11 +69,14 @@ def test_needs(host):
 
 def test_pages_and_visible_positions(host):
     assert host.ok(0, 1) and not host.ok(1, 1) and not host.ok(-1, 5) and not host.ok(0, 0)
-    assert host.visible(0, 0, 1, 1) == 1
-    assert host.visible(12, 10, 14, 100) == 99
-    assert host.visible(10, 10, 14, 3) == 0  # a chunk longer than its cache: the first rows see nothing
-    assert host.visible(13, 10, 14, 3) == 3
-    assert host.visible(10, 10, 14, 0) == 0
+    assert host.visible(0, 1, 1) == 1
+    assert host.visible(12, 14, 100) == 99
+    assert host.visible(10, 14, 3) == 0  # a chunk longer than its cache: the first rows see nothing
+    assert host.visible(13, 14, 3) == 3
+    assert host.visible(10, 14, 0) == 0
+    top = 2**31 - 256
+    assert host.visible(0, top, 0) == 0 and host.visible(0, 1, top) == top  # no 32-bit overflow at the limits
+    assert host.visible(top - 1, top, top) == top and host.visible(0, top, top) == 1
 
 
 def test_find_sequence_stays_in_bounds(host):
