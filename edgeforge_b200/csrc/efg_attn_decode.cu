@@ -54,8 +54,9 @@ struct Shape {
 
 // A cut key head's pieces are slot `first` of CTA i (1: the last part of its run, 0: all of it) and
 // slot 0 of the CTAs behind it.
-struct JoinDesc {
+struct alignas(16) JoinDesc {
   int32_t seq, kvh, first, parts;  // parts 0: nothing begins here that is cut
+  int32_t begin, end, kv_len, pad;  // the sequence's chunk
 };
 
 struct DecodeParams {
@@ -104,6 +105,17 @@ __device__ __forceinline__ void redo_rows(const AttnParams& p, const Rows& w, in
   }
 }
 
+// Place of dim d in a warp's row r of the exchange area: pieces of a row exchanged so that a fragment's
+// eight rows fall into different banks (F32: 16-byte pieces, otherwise 8-byte ones).
+template <bool kF32>
+__device__ __forceinline__ int slab_at(int r, int d) {
+  return kF32 ? (((d >> 2) ^ ((r & 1) << 2)) << 2) | (d & 3) : (((d >> 1) ^ ((r & 3) << 2)) << 1) | (d & 1);
+}
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
+}
+
 // The consumer warps alone.
 __device__ __forceinline__ void consumer_barrier() {
   __syncwarp();
@@ -119,21 +131,32 @@ __device__ __forceinline__ int tiles_of(const Rows& w) {
 // Weight of a sequence on the line: of each key head its begin and end, then its tiles; 1 per key head when
 // they are never cut. 0 without new tokens.
 template <typename T, int D>
-__device__ __forceinline__ int64_t weight_of(const DecodeParams& dp, int64_t seq) {
+__device__ __forceinline__ int weight_of(const DecodeParams& dp, int64_t seq) {
   Rows w;
   if (!rows_of(dp.a, seq, w)) return 0;
-  return static_cast<int64_t>(dp.slots ? kHeadCost + tiles_of<T, D>(w) : 1) * dp.a.kv_heads;
+  return (dp.slots ? kHeadCost + tiles_of<T, D>(w) : 1) * dp.a.kv_heads;
 }
+
+// The line cut into `runs` runs whose weights differ by one at most.
+struct Runs {
+  uint32_t runs, size, longer;  // the first `longer` runs weigh size + 1
+  __device__ __forceinline__ Runs(uint32_t line, uint32_t n) : runs(n), size(line / n), longer(line - line / n * n) {}
+  __device__ __forceinline__ uint32_t begin(uint32_t i) const { return i * size + min(i, longer); }
+  __device__ __forceinline__ uint32_t at(uint32_t place) const {  // the run that holds a place
+    const uint32_t split = longer * (size + 1);
+    return place < split ? place / (size + 1) : longer + (place - split) / size;
+  }
+};
 
 // Walks the parts of a run: for each, the sequence, the key head and the tiles [from, to) of it.
 template <typename T, int D>
 struct Walk {
-  int64_t left, at;  // what is left of the run, and the place inside the sequence's weight
+  int left, at;  // what is left of the run, and the place inside the sequence's weight
   int seq, kvh, from, to, all;
   Rows w;
   bool loaded;
-  __device__ __forceinline__ void start(int64_t s, int64_t place, int64_t count) {
-    seq = static_cast<int>(s);
+  __device__ __forceinline__ void start(int s, int place, int count) {
+    seq = s;
     at = place;
     left = count;
     loaded = false;
@@ -147,15 +170,14 @@ struct Walk {
         if (loaded) all = tiles_of<T, D>(w);
       }
       const int weight = cut ? kHeadCost + all : 1;
-      if (!loaded || at >= static_cast<int64_t>(weight) * dp.a.kv_heads) {
+      if (!loaded || at >= weight * dp.a.kv_heads) {
         ++seq;
         at = 0;
         loaded = false;
         continue;
       }
-      kvh = static_cast<int>(at / weight);
-      const int off = static_cast<int>(at - static_cast<int64_t>(kvh) * weight);
-      const int step = static_cast<int>(min(static_cast<int64_t>(weight - off), left));
+      kvh = at / weight;
+      const int off = at - kvh * weight, step = min(weight - off, left);
       left -= step;
       at += step;
       from = cut ? max(0, off - kHeadCost) : 0;
@@ -177,47 +199,54 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[S::kStages], empty[S::kStages];
   __shared__ float top_s[kConsumers][16], sum_s[kConsumers][16];
-  __shared__ int64_t scan_s[kThreads / 32], place_s[3];
+  __shared__ int scan_s[kThreads / 32], place_s[2];
   __shared__ int redo_s[16];
   const AttnParams& p = dp.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const bool cut = dp.slots != nullptr;
-  pdl_launch_dependents();
-
-  // ---- this CTA's run of the line: every thread adds up a block of sequences, then the one whose block
-  // holds the run's beginning finds the sequence
-  const int64_t per = (p.n_seqs + kThreads - 1) / kThreads, s_lo = min(p.n_seqs, tid * per), s_hi = min(p.n_seqs, s_lo + per);
-  int64_t mine = 0;
-  for (int64_t s = s_lo; s < s_hi; ++s) mine += weight_of<T, D>(dp, s);
-  int64_t inc = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t up = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-    if (lane >= o) inc += up;
-  }
-  if (lane == 31) scan_s[warp] = inc;
-  if (tid == 0) {
+  if (tid == 32 * kConsumers) {
+    prefetch_map(&map_k);
+    prefetch_map(&map_v);
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], kConsumers);
     }
     fence_barrier_init();
   }
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // ---- this CTA's run of the line: every thread adds up a block of sequences, then the one whose block
+  // holds the run's beginning finds the sequence
+  const int n_seqs = static_cast<int>(p.n_seqs), per = (n_seqs + kThreads - 1) / kThreads;
+  const int s_lo = min(n_seqs, tid * per), s_hi = min(n_seqs, s_lo + per);
+  int mine = 0;
+  for (int s = s_lo; s < s_hi; ++s) mine += weight_of<T, D>(dp, s);
+  int inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+    if (lane >= o) inc += up;
+  }
+  if (lane == 31) scan_s[warp] = inc;
   __syncthreads();
-  int64_t line = 0, before = inc - mine;
+  int line = 0, before = inc - mine;
+#pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) before += scan_s[w];
     line += scan_s[w];
   }
-  const int64_t runs = min(static_cast<int64_t>(gridDim.x), cut ? max(int64_t{1}, line / kMinRun) : line);
-  if (blockIdx.x >= runs || line == 0) {
+  const int n_runs = min(static_cast<int>(gridDim.x), cut ? max(1, line / kMinRun) : line);
+  if (static_cast<int>(blockIdx.x) >= n_runs || line == 0) {
     if (cut && tid == 0) dp.desc[blockIdx.x].parts = 0;
     return;
   }
-  const int64_t begin = blockIdx.x * line / runs, end = (blockIdx.x + 1) * line / runs;
+  const Runs runs(line, n_runs);
+  const int begin = static_cast<int>(runs.begin(blockIdx.x)), end = static_cast<int>(runs.begin(blockIdx.x + 1));
   if (begin >= before && begin < before + mine) {
-    int64_t at = begin - before, s = s_lo;
-    for (int64_t n; (n = weight_of<T, D>(dp, s)) <= at; ++s) at -= n;
+    int at = begin - before, s = s_lo;
+    if (per > 1)
+      for (int n; (n = weight_of<T, D>(dp, s)) <= at; ++s) at -= n;
     place_s[0] = s;
     place_s[1] = at;
   }
@@ -509,13 +538,19 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
         sum_s[warp][g + 8 * i] = v;
       }
       float* o = o_s + (warp * kSlabRows + g + 8 * i) * D;
+      const auto value = [&](int n, int e) { return kStack ? acc[n][e] + acc[n][e + 2] : acc[n][2 * i + e]; };
+      if constexpr (kF32) {  // dims 32 dc + 4 t + 16 e ..  + 3
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n)
+        for (int n = 0; n < D / 8; n += 4)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int d = kF32 ? 32 * (n / 4) + 4 * t + 16 * e + n % 4 : 8 * n + 2 * t + e;
-          o[d] = kStack ? acc[n][e] + acc[n][e + 2] : acc[n][2 * i + e];
-        }
+          for (int e = 0; e < 2; ++e)
+            *reinterpret_cast<float4*>(o + slab_at<kF32>(g, 8 * n + 4 * t + 16 * e)) =
+                make_float4(value(n, e), value(n + 1, e), value(n + 2, e), value(n + 3, e));
+      } else {  // dims 8 n + 2 t, + 1
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+          *reinterpret_cast<float2*>(o + slab_at<kF32>(g, 8 * n + 2 * t)) = make_float2(value(n, 0), value(n, 1));
+      }
     }
     const bool whole = walk.from == 0 && walk.to == walk.all, uneven = whole && w.see_first < w.see_all;
     if (uneven && tid < 16) redo_s[tid] = 0;
@@ -531,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
 #pragma unroll
       for (int x = 0; x < kConsumers; ++x) {
         const float f = ex2(top_s[x][r] - ref);
-        v += f * o_s[x * kSlabRows * D + e];
+        v += f * o_s[(x * kSlabRows + r) * D + slab_at<kF32>(r, d)];
         l += f * sum_s[x][r];
       }
       if (!whole) {
@@ -550,12 +585,11 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
     }
     if (warp == 0) {
       if (!whole && walk.from == 0) {  // a key head that is cut begins here: its last piece is in another run
-        const int64_t last = end - 1 + (walk.all - walk.to);
-        const int64_t cta = ((last + 1) * runs - 1) / line;
+        const int cta = static_cast<int>(runs.at(end - 1 + (walk.all - walk.to)));
         owner = true;
         if (lane == 0)
-          dp.desc[blockIdx.x] = JoinDesc{static_cast<int32_t>(walk.seq), kvh, first_part ? 0 : 1,
-                                         static_cast<int32_t>(cta - blockIdx.x + 1)};
+          dp.desc[blockIdx.x] = JoinDesc{walk.seq, kvh, first_part ? 0 : 1, cta - static_cast<int>(blockIdx.x) + 1,
+                                         w.c.begin, w.c.end, w.c.kv_len, 0};
       }
     }
     first_part = false;
@@ -565,9 +599,11 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
 
 // Joins the pieces of the key head whose first piece is at the end of CTA blockIdx.x's run:
 // out = sum_x 2^(top_x - top) o_x / sum_x 2^(top_x - top) l_x. Rows blockIdx.y, blockIdx.y + gridDim.y, ..
+// A group of threads takes every kGroups-th piece; its first kAhead pieces are loaded before the weights
+// are known, so that few pieces cost one round of loads.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ DecodeParams dp) {
-  constexpr int kGroups = 128 / (D / 4);  // threads of one group read one piece's row, 16 bytes each
+  constexpr int kGroups = 128 / (D / 4), kAhead = 2;  // a group reads one piece's row, 16 bytes a thread
   __shared__ float weight[kMaxCtas], part[kGroups][D], red[8];
   __shared__ int redo_s[16];
   const AttnParams& p = dp.a;
@@ -577,12 +613,22 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
   const JoinDesc j = dp.desc[blockIdx.x];
   if (j.parts <= 1) return;
   Rows w;
-  if (!rows_of(p, j.seq, w)) return;
+  w.c = Chunk{j.seq, j.begin, j.end, j.kv_len};
+  w.rows = (j.end - j.begin) * p.group;
+  w.see_first = seen_by(w.c, j.begin);
+  w.see_all = seen_by(w.c, j.end - 1);
   constexpr int64_t kSlot = 16 * (D + 2);
-  auto slot = [&](int x) { return dp.slots + ((static_cast<int64_t>(blockIdx.x) + x) * 2 + (x == 0 ? j.first : 0)) * kSlot; };
+  const float* slots = dp.slots + static_cast<int64_t>(blockIdx.x) * 2 * kSlot;
+  auto slot = [&](int x) { return slots + (2 * x + (x == 0 ? j.first : 0)) * kSlot; };
   for (int r = blockIdx.y; r < w.rows; r += gridDim.y) {
+    float4 ahead[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int x = group + k * kGroups;
+      ahead[k] = x < j.parts ? *reinterpret_cast<const float4*>(slot(x) + 32 + r * D + d) : make_float4(0, 0, 0, 0);
+    }
     float mx = -INFINITY, l = 0.f;
-    for (int x = tid; x < j.parts; x += 128) mx = fmaxf(mx, slot(x)[r]);
+    for (int x = tid; x < j.parts; x += 128) mx = fmaxf(mx, weight[x] = slot(x)[r]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
     if (lane == 0) red[warp] = mx;
@@ -590,7 +636,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
     mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     const float ref = mx == -INFINITY ? 0.f : mx;
     for (int x = tid; x < j.parts; x += 128) {
-      const float f = ex2(slot(x)[r] - ref);
+      const float f = ex2(weight[x] - ref);
       weight[x] = f;
       l += f * slot(x)[16 + r];
     }
@@ -599,12 +645,16 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
     __syncthreads();
     l = (red[4] + red[5]) + (red[6] + red[7]);
     float4 acc = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-    for (int x = group; x < j.parts; x += kGroups) {
-      const float4 v = *reinterpret_cast<const float4*>(slot(x) + 32 + r * D + d);
+    const auto add = [&](int x, const float4& v) {
       const float f = weight[x];
       acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
-    }
+    };
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (group + k * kGroups < j.parts) add(group + k * kGroups, ahead[k]);
+#pragma unroll 4
+    for (int x = group + kAhead * kGroups; x < j.parts; x += kGroups)
+      add(x, *reinterpret_cast<const float4*>(slot(x) + 32 + r * D + d));
     *reinterpret_cast<float4*>(&part[group][d]) = acc;
     __syncthreads();
     if (tid < D && tid < p.head_dim) {
@@ -614,12 +664,11 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
       if (store_row<T>(p, w, j.kvh, r, tid, v, l)) redo_s[r] = 1;
     }
     __syncthreads();
-    if (warp == 0 && redo_s[r]) {
-      redo_rows<T>(p, w, j.kvh, redo_s, weight);
-      __syncwarp();
-      if (lane == 0) redo_s[r] = 0;
+    if (redo_s[r] && w.see_first < w.see_all) {  // the same for every thread
+      if (warp == 0) redo_rows<T>(p, w, j.kvh, redo_s, weight);
+      __syncthreads();
+      if (tid == 0) redo_s[r] = 0;
     }
-    __syncthreads();
   }
 }
 
@@ -629,19 +678,22 @@ int launch(const DecodeParams& dp, const CUtensorMap& mk, const CUtensorMap& mv,
   const auto fn = attn_decode_kernel<T, D, kStack>;
   if (int st = ensure_smem_attr(reinterpret_cast<const void*>(fn), S::smem(kStack ? 8 : 16))) return st;
   const AttnParams& p = dp.a;
-  fn<<<static_cast<unsigned>(ctas), kThreads, S::smem(kStack ? 8 : 16), s>>>(dp, mk, mv);
-  EFG_TRY_CUDA(cudaGetLastError(), "attention launch");
-  if (!dp.slots) return EFG_OK;
   cudaLaunchConfig_t cf{};
-  const int64_t rows = std::min<int64_t>(kDecodeRows, std::min(p.kv_len ? p.max_new : p.n_rows, p.n_rows) * p.group);
-  cf.gridDim = dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(std::min<int64_t>(rows, 4)));
-  cf.blockDim = dim3(128);
-  cf.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cf.attrs = attr;
   cf.numAttrs = 1;
+  cf.stream = s;
+  cf.gridDim = dim3(static_cast<unsigned>(ctas));
+  cf.blockDim = dim3(kThreads);
+  cf.dynamicSmemBytes = S::smem(kStack ? 8 : 16);
+  EFG_TRY_CUDA(cudaLaunchKernelEx(&cf, fn, dp, mk, mv), "attention launch");
+  if (!dp.slots) return EFG_OK;
+  const int64_t rows = std::min<int64_t>(kDecodeRows, std::min(p.kv_len ? p.max_new : p.n_rows, p.n_rows) * p.group);
+  cf.gridDim = dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(std::min<int64_t>(rows, 8)));
+  cf.blockDim = dim3(128);
+  cf.dynamicSmemBytes = 0;
   EFG_TRY_CUDA(cudaLaunchKernelEx(&cf, attn_join_kernel<T, D>, dp), "attention launch");
   return EFG_OK;
 }
@@ -680,6 +732,8 @@ bool attn_decode_takes(int type, const AttnParams& p) {
   if (p.k_stride == 0 || p.v_stride == 0) return false;
   if (p.kv_len && (p.n_pages == 0 || p.page_size < 8 || (p.page_size & (p.page_size - 1)))) return false;
   const int64_t max_new = std::min(p.kv_len ? p.max_new : p.n_rows, p.n_rows);
+  // the line's weight is a 32-bit number
+  if (p.n_seqs * p.kv_heads > 0x7FFFFFFFll / (max_keys_of(p) / 32 + 1 + kHeadCost)) return false;
   return attn_mma_takes(type, p) && max_new * p.group <= kDecodeRows;
 }
 
