@@ -7,6 +7,7 @@ CPU or PyTorch path.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -14,6 +15,7 @@ LIB_PATH = PKG / "libefg.so"
 
 _vp, _sz, _i = C.c_void_p, C.c_size_t, C.c_int
 _u64, _i32p = C.c_uint64, C.POINTER(C.c_int32)
+_args = C.c_char_p  # an argument block in C layout, packed by ArgBlock
 
 
 class EdgeForgeError(RuntimeError):
@@ -43,6 +45,26 @@ class ModelInfo(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("hidden", "intermediate", "layers", "heads", "kv_heads", "head_dim", "vocab",
                                           "max_seq", "n_q4", "n_q8", "embed_type")] + [("bytes_per_token", C.c_uint64)]
 
+
+class ArgBlock:
+    """Packs the fields of an efg_*_args struct (include/efg.h): one pointer to pass instead of two dozen
+    converted arguments."""
+
+    def __init__(self, fields: str):
+        kinds = [f.split(":") for f in fields.split()]
+        self.names = [k[0] for k in kinds]
+        code = {"p": "P", "n": "N", "i": "i", "f": "f"}
+        self.pack = struct.Struct("@" + "".join(code[k[1] if len(k) > 1 else "n"] for k in kinds)).pack
+
+
+PAGE_PLAN = ArgBlock("block_table:p max_pages slots:p positions:p n_rows cu:p kv_len:p taken:p cached:p new:p n_seqs "
+                     "free:p n_free n_pages page_size")
+PAGE_STORE = ArgBlock("type:i cache_type:i q_out:p k_cache:p v_cache:p n_slots q:p q_stride k:p k_stride v:p v_stride "
+                      "slots:p positions:p n_rows cos:p sin:p max_pos heads kv_heads head_dim")
+ATTN_PROMPT = ArgBlock("type:i scale:f out:p q:p q_stride k:p k_stride v:p v_stride cu:p n_seqs n_rows heads kv_heads "
+                       "head_dim")
+ATTN_PAGED = ArgBlock("type:i scale:f out:p q:p q_stride k_cache:p v_cache:p n_pages page_size block_table:p max_pages "
+                      "cu:p kv_len:p n_seqs n_rows max_new heads kv_heads head_dim workspace:p workspace_bytes")
 
 # name -> (restype, argtypes); every symbol include/efg.h declares.
 SIGNATURES = {
@@ -86,13 +108,11 @@ SIGNATURES = {
     "efg_matvec_sharded": (_i, [_i, _vp, _vp, _vp, _sz, _sz, _vp, _vp]),
     "efg_argmax": (_i, [_vp, _sz, _vp, _vp]),
     "efg_lm_head_argmax_sharded": (_i, [C.c_int, _vp, _vp, _vp, _vp, _vp, C.c_float, _sz, _sz, _vp, _vp]),
-    "efg_page_plan": (_i, [_vp, _sz, _vp, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _sz, _sz, _vp]),
-    "efg_page_store": (_i, [_i, _i, _vp, _vp, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _sz, _sz,
-                            _sz, _sz, _vp]),
-    "efg_attn_prompt": (_i, [_i, _vp, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _sz, _sz, _sz, _sz, C.c_float, _vp]),
-    "efg_attn_paged": (_i, [_i, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz,
-                            C.c_float, _vp, _sz, _vp]),
-    "efg_attn_paged_workspace": (_u64, [_i, _sz, _sz, _sz, _sz, _sz, _sz, _sz, _sz]),
+    "efg_page_plan": (_i, [_args, _vp]),
+    "efg_page_store": (_i, [_args, _vp]),
+    "efg_attn_prompt": (_i, [_args, _vp]),
+    "efg_attn_paged": (_i, [_args, _vp]),
+    "efg_attn_paged_workspace": (_u64, [_args]),
     "efg_efq_check": (_i, [_vp, _u64]),
     "efg_quantize_model": (_i, [C.c_char_p, C.c_char_p, C.c_char_p, C.c_char_p, C.POINTER(QuantizeReport)]),
     "efg_decoder_open": (_i, [C.c_char_p, _sz, C.POINTER(_vp)]),

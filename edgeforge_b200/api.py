@@ -17,7 +17,8 @@ from enum import IntEnum
 
 import numpy as np
 
-from ._lib import EdgeForgeError, MatvecJob, ModelInfo, QuantizeReport, check, load
+from ._lib import (ATTN_PAGED, ATTN_PROMPT, PAGE_PLAN, PAGE_STORE, EdgeForgeError, MatvecJob, ModelInfo,
+                   QuantizeReport, check, load)
 
 
 class QType(IntEnum):
@@ -337,68 +338,78 @@ def lm_head_argmax_sharded(qtype: int, logits_shard, token, W_shard, x, norm_w, 
 
 
 # ---------------------------------------------------------------- paged serving
+# These run once per layer of a decode step, so the wrappers count: one look at every tensor, one
+# packed argument block, no stream or device objects.
+
+_KINDS: dict = {}  # torch dtype -> EFG code of the plain storage types, and -1 for int32
 
 
-def _plain_type(t, what: str) -> int:
-    """The EFG code of a plain storage type."""
+def _kinds():
     import torch
 
-    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}.get(t.dtype)
-    if code is None:
-        raise EdgeForgeError(1, f"{what}: expected float32, float16 or bfloat16, got {t.dtype}")
-    return code
+    _KINDS.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int32: -1})
+    return _KINDS
 
 
-def _here(what: str, *tensors) -> None:
-    """Every tensor lies on the current CUDA device, where the call is queued."""
+def _look(what: str, ints, floats) -> tuple[int, int]:
+    """Every tensor lies on the current CUDA device, where the call is queued; `ints` are contiguous
+    int32, `floats` of one plain type. Returns (its EFG code, the current stream)."""
     import torch
 
-    dev = torch.cuda.current_device() if torch.cuda.is_available() else -1
-    for t in tensors:
-        if t.get_device() != dev or dev < 0:
-            raise EdgeForgeError(1, f"{what}: expected a tensor on the current CUDA device, got one on {t.device}")
-
-
-def _ints(what: str, *tensors) -> None:
-    import torch
-
-    for t in tensors:
-        if t.dtype != torch.int32 or not t.is_contiguous():
+    kinds = _KINDS or _kinds()
+    dev = ints[0].get_device()
+    for t in ints:
+        if t.get_device() != dev:
+            raise EdgeForgeError(1, f"{what}: tensors on different devices")
+        if kinds.get(t.dtype) != -1 or not t.is_contiguous():
             raise EdgeForgeError(1, f"{what}: lengths, offsets, slots and pages are contiguous int32 tensors")
+    kind = None
+    for t in floats:
+        if t.get_device() != dev:
+            raise EdgeForgeError(1, f"{what}: tensors on different devices")
+        if t.dtype is not kind:
+            if kind is not None:
+                raise EdgeForgeError(1, f"{what}: tensors of different types, {kind} and {t.dtype}")
+            kind = t.dtype
+    code = kinds.get(kind, -1) if floats else 0
+    if code < 0:
+        raise EdgeForgeError(1, f"{what}: expected float32, float16 or bfloat16, got {kind}")
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        raise EdgeForgeError(1, f"{what}: expected tensors on the current CUDA device, got {ints[0].device}")
+    return code, torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _rows3(what: str, t, n_rows: int, dim: int) -> tuple[int, int]:
-    """(heads, row stride) of [n_rows][heads][dim] rows; heads back to back within a row."""
-    if t.dim() != 3 or t.shape[0] != n_rows or t.shape[2] != dim:
-        raise EdgeForgeError(1, f"{what}: expected [{n_rows}][heads][{dim}], got {list(t.shape)}")
-    heads = t.shape[1]
-    if (t.stride(2) != 1 and dim > 1) or (t.stride(1) != dim and heads > 1):
+def _rows3(what: str, t) -> tuple[int, int, int, int]:
+    """(rows, heads, dim, row stride) of [rows][heads][dim]; heads back to back within a row."""
+    if t.dim() != 3:
+        raise EdgeForgeError(1, f"{what}: expected [rows][heads][dim], got {list(t.shape)}")
+    rows, heads, dim = t.shape
+    s0, s1, s2 = t.stride()
+    if (s2 != 1 and dim > 1) or (s1 != dim and heads > 1):
         raise EdgeForgeError(1, f"{what}: the heads of a row lie back to back")
-    return heads, t.stride(0) if n_rows > 1 else heads * dim
-
-
-def _whole(what: str, *tensors) -> None:
-    for t in tensors:
-        if not t.is_contiguous():
-            raise EdgeForgeError(1, f"{what}: expected a contiguous tensor")
+    return rows, heads, dim, s0 if rows > 1 else heads * dim
 
 
 def page_plan(block_table, slots, positions, cu, kv_len, taken, cached, new, free, n_pages: int, page_size: int) -> None:
     """One serving step's block tables and slot map on the GPU (efg_page_plan). In: cached and new
     token counts per sequence [n], the free list. In and out: block_table [n][max_pages]. Out:
     slots and positions [rows], cu [n + 1], kv_len [n], taken [1]; all int32 CUDA tensors."""
-    _here("page_plan", block_table, slots, positions, cu, kv_len, taken, cached, new, free)
-    _ints("page_plan", block_table, slots, positions, cu, kv_len, taken, cached, new, free)
-    n = new.numel()
+    _, stream = _look("page_plan", (block_table, slots, positions, cu, kv_len, taken, cached, new, free), ())
+    n, rows = new.numel(), slots.numel()
     if block_table.dim() != 2 or block_table.shape[0] != n:
         raise EdgeForgeError(1, f"page_plan: expected a block table [{n}][max_pages], got {list(block_table.shape)}")
     if cached.numel() != n or kv_len.numel() != n or cu.numel() != n + 1 or taken.numel() != 1 \
-            or positions.numel() != slots.numel():
+            or positions.numel() != rows:
         raise EdgeForgeError(1, "page_plan: cached, new and kv_len have one entry per sequence, cu one more, taken one, "
                                 "slots and positions one per row")
-    check(load().efg_page_plan(block_table.data_ptr(), block_table.shape[1], slots.data_ptr(), positions.data_ptr(),
-                               slots.numel(), cu.data_ptr(), kv_len.data_ptr(), taken.data_ptr(), cached.data_ptr(),
-                               new.data_ptr(), n, free.data_ptr(), free.numel(), int(n_pages), int(page_size), _stream()))
+    if n_pages < 0 or page_size < 0:
+        raise EdgeForgeError(1, f"page_plan: {n_pages} pages of {page_size} slots")
+    status = load().efg_page_plan(PAGE_PLAN.pack(
+        block_table.data_ptr(), block_table.shape[1], slots.data_ptr(), positions.data_ptr(), rows, cu.data_ptr(),
+        kv_len.data_ptr(), taken.data_ptr(), cached.data_ptr(), new.data_ptr(), n, free.data_ptr(), free.numel(),
+        n_pages, page_size), stream)
+    if status:
+        check(status)
 
 
 def page_store(q_out, k_cache, v_cache, q, k, v, slots, positions, cos=None, sin=None) -> None:
@@ -407,62 +418,67 @@ def page_store(q_out, k_cache, v_cache, q, k, v, slots, positions, cos=None, sin
     [rows][kv_heads][dim] into k_cache and v_cache [pages][page_size][kv_heads][dim]; cos and sin
     float32 [max_pos][dim / 2] (both None: no rotation). The caches and q_out have the rows'
     type, or float16 / bfloat16 for float32 rows."""
-    n_rows, dim = k.shape[0], k.shape[-1]
-    kv_heads, k_stride = _rows3("page_store: k", k, n_rows, dim)
-    _, v_stride = _rows3("page_store: v", v, n_rows, dim)
-    rows, outs = [k, v], [k_cache, v_cache]
-    heads = q_stride = 0
+    n_rows, kv_heads, dim, k_stride = _rows3("page_store: k", k)
+    v_stride = _rows3("page_store: v", v)[3]
+    heads = q_stride = max_pos = 0
     if (q is None) != (q_out is None) or (cos is None) != (sin is None):
         raise EdgeForgeError(1, "page_store: q and q_out, and cos and sin, come together")
+    rows, outs = (k, v), (k_cache, v_cache)
     if q is not None:
-        heads, q_stride = _rows3("page_store: q", q, n_rows, dim)
-        if q_out.shape != q.shape:
-            raise EdgeForgeError(1, f"page_store: q_out {list(q_out.shape)} for q {list(q.shape)}")
-        rows.append(q)
-        outs.append(q_out)
-    tables = [] if cos is None else [cos, sin]
-    _here("page_store", *rows, *outs, *tables, slots, positions)
-    _ints("page_store", slots, positions)
-    _whole("page_store", *outs, *tables)
-    if v.shape != k.shape or k_cache.dim() != 4 or tuple(k_cache.shape[2:]) != (kv_heads, dim) \
-            or v_cache.shape != k_cache.shape:
+        _, heads, _, q_stride = _rows3("page_store: q", q)
+        if q_out.shape != q.shape or q.shape[0] != n_rows or q.shape[2] != dim:
+            raise EdgeForgeError(1, f"page_store: q {list(q.shape)} and q_out {list(q_out.shape)} for k {list(k.shape)}")
+        rows, outs = (k, v, q), (k_cache, v_cache, q_out)
+    ints = (slots, positions)
+    kind, stream = _look("page_store", ints, rows)
+    cache_kind, _ = _look("page_store", ints, outs)
+    if v.shape != k.shape or k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
         raise EdgeForgeError(1, f"page_store: caches {list(k_cache.shape)} and {list(v_cache.shape)} for rows "
                                 f"{list(k.shape)} and {list(v.shape)}")
-    if any(t.dtype != k.dtype for t in rows) or any(t.dtype != k_cache.dtype for t in outs):
-        raise EdgeForgeError(1, "page_store: q, k and v have one type, q_out and the caches one type")
+    pages, page_size, cache_heads, cache_dim = k_cache.shape
+    if cache_heads != kv_heads or cache_dim != dim:
+        raise EdgeForgeError(1, f"page_store: caches {list(k_cache.shape)} for rows {list(k.shape)}")
     if slots.numel() != n_rows or positions.numel() != n_rows:
         raise EdgeForgeError(1, "page_store: one slot and one position per row")
-    max_pos = 0
-    if tables:
+    if cos is not None:
         max_pos = cos.shape[0]
-        if any(str(t.dtype) != "torch.float32" or tuple(t.shape) != (max_pos, dim // 2) for t in tables):
+        if _look("page_store", ints, (cos, sin))[0] != 0 or tuple(cos.shape) != (max_pos, dim // 2) or sin.shape != cos.shape:
             raise EdgeForgeError(1, f"page_store: cos and sin are float32 [max_pos][{dim // 2}]")
-    check(load().efg_page_store(
-        _plain_type(k, "page_store"), _plain_type(k_cache, "page_store"), None if q is None else q_out.data_ptr(),
-        k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0] * k_cache.shape[1],
-        None if q is None else q.data_ptr(), q_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, slots.data_ptr(),
-        positions.data_ptr(), n_rows, cos.data_ptr() if tables else None, sin.data_ptr() if tables else None, max_pos,
-        heads, kv_heads, dim, _stream()))
+        outs += (cos, sin)
+    for t in outs:
+        if not t.is_contiguous():
+            raise EdgeForgeError(1, "page_store: q_out, the caches and the tables are contiguous")
+    status = load().efg_page_store(PAGE_STORE.pack(
+        kind, cache_kind, 0 if q is None else q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pages * page_size,
+        0 if q is None else q.data_ptr(), q_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, slots.data_ptr(),
+        positions.data_ptr(), n_rows, 0 if cos is None else cos.data_ptr(), 0 if cos is None else sin.data_ptr(), max_pos,
+        heads, kv_heads, dim), stream)
+    if status:
+        check(status)
 
 
 def attn_prompt(out, q, k, v, cu, scale: float | None = None) -> None:
     """Causal attention over packed prompts (efg_attn_prompt): out and q [rows][heads][dim], k and
     v [rows][kv_heads][dim], cu int32 [n + 1] the first row of each prompt; scale 1 / sqrt(dim) by
     default. q, k and v may be strided rows (views of one projection's output)."""
-    _here("attn_prompt", out, q, k, v, cu)
-    _ints("attn_prompt", cu)
-    _whole("attn_prompt", out)
-    n_rows, dim = q.shape[0], q.shape[-1]
-    heads, q_stride = _rows3("attn_prompt: q", q, n_rows, dim)
-    kv_heads, k_stride = _rows3("attn_prompt: k", k, n_rows, dim)
-    _, v_stride = _rows3("attn_prompt: v", v, n_rows, dim)
-    if out.shape != q.shape or v.shape != k.shape or not (out.dtype == q.dtype == k.dtype == v.dtype):
-        raise EdgeForgeError(1, "attn_prompt: out is like q, v like k, all of one type")
-    if cu.numel() < 1:
-        raise EdgeForgeError(1, "attn_prompt: cu has one entry per prompt and one more")
-    check(load().efg_attn_prompt(_plain_type(q, "attn_prompt"), out.data_ptr(), q.data_ptr(), q_stride, k.data_ptr(),
-                                 k_stride, v.data_ptr(), v_stride, cu.data_ptr(), cu.numel() - 1, n_rows, heads, kv_heads,
-                                 dim, max(dim, 1)**-0.5 if scale is None else scale, _stream()))
+    kind, stream = _look("attn_prompt", (cu,), (out, q, k, v))
+    n_rows, heads, dim, q_stride = _rows3("attn_prompt: q", q)
+    k_rows, kv_heads, k_dim, k_stride = _rows3("attn_prompt: k", k)
+    v_stride = _rows3("attn_prompt: v", v)[3]
+    if out.shape != q.shape or v.shape != k.shape or k_rows != n_rows or k_dim != dim:
+        raise EdgeForgeError(1, f"attn_prompt: out {list(out.shape)}, q {list(q.shape)}, k {list(k.shape)}, v "
+                                f"{list(v.shape)}")
+    n = cu.numel() - 1
+    if n < 0 or not out.is_contiguous():
+        raise EdgeForgeError(1, "attn_prompt: cu has one entry per prompt and one more, and out is contiguous")
+    status = load().efg_attn_prompt(ATTN_PROMPT.pack(
+        kind, max(dim, 1)**-0.5 if scale is None else scale, out.data_ptr(), q.data_ptr(), q_stride, k.data_ptr(), k_stride,
+        v.data_ptr(), v_stride, cu.data_ptr(), n, n_rows, heads, kv_heads, dim), stream)
+    if status:
+        check(status)
+
+
+_workspace_bytes: dict = {}  # (device, sizes of a call) -> bytes, a function of these numbers alone
 
 
 def attn_paged(out, q, k_cache, v_cache, block_table, cu, kv_len, max_new: int, scale: float | None = None) -> None:
@@ -470,29 +486,37 @@ def attn_paged(out, q, k_cache, v_cache, block_table, cu, kv_len, max_new: int, 
     [rows][heads][dim], caches [pages][page_size][kv_heads][dim], block_table [n][max_pages], cu
     [n + 1] and kv_len [n] as page_plan writes them; max_new: no chunk is longer (1 for decode).
     The workspace that long sequences need comes from torch's allocator, for this call."""
-    import torch
-
-    _here("attn_paged", out, q, k_cache, v_cache, block_table, cu, kv_len)
-    _ints("attn_paged", block_table, cu, kv_len)
-    _whole("attn_paged", out, k_cache, v_cache)
-    n_rows, dim = q.shape[0], q.shape[-1]
-    heads, q_stride = _rows3("attn_paged: q", q, n_rows, dim)
-    n, max_new = kv_len.numel(), int(max_new)
-    if k_cache.dim() != 4 or k_cache.shape[3] != dim or v_cache.shape != k_cache.shape:
-        raise EdgeForgeError(1, f"attn_paged: caches {list(k_cache.shape)} and {list(v_cache.shape)} for head size {dim}")
-    if out.shape != q.shape or not (out.dtype == q.dtype == k_cache.dtype == v_cache.dtype):
-        raise EdgeForgeError(1, "attn_paged: out is like q, and the caches are of its type")
-    if block_table.dim() != 2 or block_table.shape[0] != n or cu.numel() != n + 1:
+    kind, stream = _look("attn_paged", (block_table, cu, kv_len), (out, q, k_cache, v_cache))
+    n_rows, heads, dim, q_stride = _rows3("attn_paged: q", q)
+    n = kv_len.numel()
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or out.shape != q.shape:
+        raise EdgeForgeError(1, f"attn_paged: caches {list(k_cache.shape)} and {list(v_cache.shape)}, out "
+                                f"{list(out.shape)}, q {list(q.shape)}")
+    pages, page_size, kv_heads, cache_dim = k_cache.shape
+    if cache_dim != dim or not (out.is_contiguous() and k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise EdgeForgeError(1, f"attn_paged: caches {list(k_cache.shape)} for head size {dim}; out and the caches are "
+                                "contiguous")
+    if block_table.dim() != 2 or block_table.shape[0] != n or cu.numel() != n + 1 or max_new < 0:
         raise EdgeForgeError(1, f"attn_paged: block table {list(block_table.shape)} and {cu.numel()} offsets for {n} "
-                                "sequences")
-    pages, page_size, kv_heads, _ = k_cache.shape
-    kind, wide, lib = _plain_type(q, "attn_paged"), block_table.shape[1], load()
-    need = lib.efg_attn_paged_workspace(kind, page_size, wide, n, n_rows, max_new, heads, kv_heads, dim)
-    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    check(lib.efg_attn_paged(kind, out.data_ptr(), q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(), pages,
-                             page_size, block_table.data_ptr(), wide, cu.data_ptr(), kv_len.data_ptr(), n, n_rows, max_new,
-                             heads, kv_heads, dim, max(dim, 1)**-0.5 if scale is None else scale,
-                             work.data_ptr() if need else None, need, _stream()))
+                                f"sequences, max_new {max_new}")
+    wide, lib = block_table.shape[1], load()
+    sizes = (n_rows, max_new, heads, kv_heads, dim)
+    args = (kind, max(dim, 1)**-0.5 if scale is None else scale, out.data_ptr(), q.data_ptr(), q_stride,
+            k_cache.data_ptr(), v_cache.data_ptr(), pages, page_size, block_table.data_ptr(), wide, cu.data_ptr(),
+            kv_len.data_ptr(), n, *sizes)
+    key = (q.get_device(), kind, page_size, wide, n, sizes)
+    need = _workspace_bytes.get(key)
+    if need is None:
+        if len(_workspace_bytes) > 4096:
+            _workspace_bytes.clear()
+        need = _workspace_bytes[key] = lib.efg_attn_paged_workspace(ATTN_PAGED.pack(*args, 0, 0))
+    if need:
+        work = q.new_empty(need // q.element_size() + 8)
+        status = lib.efg_attn_paged(ATTN_PAGED.pack(*args, work.data_ptr(), need), stream)
+    else:
+        status = lib.efg_attn_paged(ATTN_PAGED.pack(*args, 0, 0), stream)
+    if status:
+        check(status)
 
 
 # ---------------------------------------------------------------- .efq and the decode step

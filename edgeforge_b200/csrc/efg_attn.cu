@@ -78,9 +78,10 @@ using efg::fail;
 
 extern "C" {
 
-int efg_attn_prompt(int type, void* d_out, const void* d_q, size_t q_stride, const void* d_k, size_t k_stride,
-                    const void* d_v, size_t v_stride, const int32_t* d_cu, size_t n_seqs, size_t n_rows, size_t heads,
-                    size_t kv_heads, size_t head_dim, float scale, void* stream) {
+int efg_attn_prompt(const efg_attn_prompt_args* args, void* stream) {
+  if (!args) return fail(EFG_EINVAL, "attn_prompt: null pointer");
+  const auto& [type, scale, d_out, d_q, q_stride, d_k, k_stride, d_v, v_stride, d_cu, n_seqs, n_rows, heads, kv_heads,
+               head_dim] = *args;
   if (int st = efg::check_attn("attn_prompt", type, n_seqs, n_rows, heads, kv_heads, head_dim, q_stride, scale))
     return st;
   if (k_stride < kv_heads * head_dim || v_stride < kv_heads * head_dim)
@@ -109,8 +110,10 @@ int efg_attn_prompt(int type, void* d_out, const void* d_q, size_t q_stride, con
   return efg::launch_attn(type, p, dev->sm_count, nullptr, 0, static_cast<cudaStream_t>(stream));
 }
 
-uint64_t efg_attn_paged_workspace(int type, size_t page_size, size_t max_pages, size_t n_seqs, size_t n_rows,
-                                  size_t max_new, size_t heads, size_t kv_heads, size_t head_dim) {
+uint64_t efg_attn_paged_workspace(const efg_attn_paged_args* args) {
+  if (!args) return 0;
+  const size_t n_seqs = args->n_seqs, max_pages = args->max_pages, page_size = args->page_size, heads = args->heads,
+               kv_heads = args->kv_heads, head_dim = args->head_dim, max_new = args->max_new, n_rows = args->n_rows;
   efg::AttnParams p{};
   p.kv_len = reinterpret_cast<const int32_t*>(1);  // a paged call; never read
   p.n_seqs = static_cast<int64_t>(n_seqs);
@@ -121,14 +124,13 @@ uint64_t efg_attn_paged_workspace(int type, size_t page_size, size_t max_pages, 
   if (kv_heads == 0 || n_seqs == 0 || std::min(max_new, n_rows) * (heads / kv_heads) > efg::kDecodeRows || head_dim > 128)
     return 0;
   efg::DeviceInfo* dev = efg::current_device();
-  return dev ? efg::attn_decode_workspace(type, p, dev->sm_count) : 0;
+  return dev ? efg::attn_decode_workspace(args->type, p, dev->sm_count) : 0;
 }
 
-int efg_attn_paged(int type, void* d_out, const void* d_q, size_t q_stride, const void* d_k_cache,
-                   const void* d_v_cache, size_t n_pages, size_t page_size, const int32_t* d_block_table,
-                   size_t max_pages, const int32_t* d_cu, const int32_t* d_kv_len, size_t n_seqs, size_t n_rows,
-                   size_t max_new, size_t heads, size_t kv_heads, size_t head_dim, float scale, void* d_workspace,
-                   size_t workspace_bytes, void* stream) {
+int efg_attn_paged(const efg_attn_paged_args* args, void* stream) {
+  if (!args) return fail(EFG_EINVAL, "attn_paged: null pointer");
+  const auto& [type, scale, d_out, d_q, q_stride, d_k_cache, d_v_cache, n_pages, page_size, d_block_table, max_pages,
+               d_cu, d_kv_len, n_seqs, n_rows, max_new, heads, kv_heads, head_dim, d_workspace, workspace_bytes] = *args;
   if (int st = efg::check_attn("attn_paged", type, n_seqs, n_rows, heads, kv_heads, head_dim, q_stride, scale))
     return st;
   if (page_size == 0 || page_size > (1u << 30)) return fail(EFG_EINVAL, "attn_paged: page size %zu", page_size);

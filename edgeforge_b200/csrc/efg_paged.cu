@@ -252,10 +252,10 @@ using efg::fail;
 
 extern "C" {
 
-int efg_page_plan(int32_t* d_block_table, size_t max_pages, int32_t* d_slots, int32_t* d_positions, size_t n_rows,
-                  int32_t* d_cu, int32_t* d_kv_len, int32_t* d_taken, const int32_t* d_cached, const int32_t* d_new,
-                  size_t n_seqs, const int32_t* d_free, size_t n_free, size_t n_pages, size_t page_size,
-                  void* stream) {
+int efg_page_plan(const efg_page_plan_args* args, void* stream) {
+  if (!args) return fail(EFG_EINVAL, "page_plan: null pointer");
+  const auto& [d_block_table, max_pages, d_slots, d_positions, n_rows, d_cu, d_kv_len, d_taken, d_cached, d_new, n_seqs,
+               d_free, n_free, n_pages, page_size] = *args;
   if (!d_cu || !d_taken || (n_rows && (!d_slots || !d_positions)) || (n_free && !d_free) ||
       (n_seqs && (!d_kv_len || !d_cached || !d_new || (max_pages && !d_block_table))))
     return fail(EFG_EINVAL, "page_plan: null pointer");
@@ -290,11 +290,10 @@ int efg_page_plan(int32_t* d_block_table, size_t max_pages, int32_t* d_slots, in
   return EFG_OK;
 }
 
-int efg_page_store(int type, int cache_type, void* d_q_out, void* d_k_cache, void* d_v_cache, size_t n_slots,
-                   const void* d_q, size_t q_stride, const void* d_k, size_t k_stride, const void* d_v,
-                   size_t v_stride, const int32_t* d_slots, const int32_t* d_positions, size_t n_rows,
-                   const float* d_cos, const float* d_sin, size_t max_pos, size_t heads, size_t kv_heads,
-                   size_t head_dim, void* stream) {
+int efg_page_store(const efg_page_store_args* args, void* stream) {
+  if (!args) return fail(EFG_EINVAL, "page_store: null pointer");
+  const auto& [type, cache_type, d_q_out, d_k_cache, d_v_cache, n_slots, d_q, q_stride, d_k, k_stride, d_v, v_stride,
+               d_slots, d_positions, n_rows, d_cos, d_sin, max_pos, heads, kv_heads, head_dim] = *args;
   if (type < EFG_F32 || type > EFG_BF16) return fail(EFG_EINVAL, "page_store: unknown type %d", type);
   if (cache_type != type && (type != EFG_F32 || cache_type < EFG_F32 || cache_type > EFG_BF16))
     return fail(EFG_EINVAL, "page_store: the cache has the rows' type, or F16 or BF16 for F32 rows (got %d for %d)",

@@ -313,10 +313,18 @@ int efg_lm_head_argmax_sharded(int qtype, float* d_logits_shard, int32_t* d_toke
  * than max_pages hold is not served either (EFG_EINVAL). The rows of a sequence that is not
  * served get slot and position -1 and its kv_len is 0. More new tokens than n_rows: the rows
  * behind n_rows are dropped and d_cu stops at n_rows (EFG_EINVAL). */
-int efg_page_plan(int32_t* d_block_table, size_t max_pages, int32_t* d_slots, int32_t* d_positions, size_t n_rows,
-                  int32_t* d_cu, int32_t* d_kv_len, int32_t* d_taken, const int32_t* d_cached, const int32_t* d_new,
-                  size_t n_seqs, const int32_t* d_free, size_t n_free, size_t n_pages, size_t page_size,
-                  void* stream);
+typedef struct {
+  int32_t* d_block_table; /* [n_seqs][max_pages], in and out */
+  size_t max_pages;
+  int32_t *d_slots, *d_positions; /* [n_rows] */
+  size_t n_rows;
+  int32_t *d_cu, *d_kv_len, *d_taken; /* [n_seqs + 1], [n_seqs], [1] */
+  const int32_t *d_cached, *d_new;    /* [n_seqs] */
+  size_t n_seqs;
+  const int32_t* d_free; /* [n_free] */
+  size_t n_free, n_pages, page_size;
+} efg_page_plan_args;
+int efg_page_plan(const efg_page_plan_args* args, void* stream);
 
 /* For every row r: q_out[r] = RoPE(q[r]) at d_positions[r], the cache's slot d_slots[r] gets
  * RoPE(k[r]) and v[r]. d_cos and d_sin are [max_pos][head_dim / 2] tables (the rotation of
@@ -326,19 +334,41 @@ int efg_page_plan(int32_t* d_block_table, size_t max_pages, int32_t* d_slots, in
  * rotation is in FP32 and rounds once, to nearest even. A row with position -1 is left out, one
  * with slot -1 has its query rotated and stores nothing. The slots of a call must be distinct.
  * head_dim even, at most 256. */
-int efg_page_store(int type, int cache_type, void* d_q_out, void* d_k_cache, void* d_v_cache, size_t n_slots,
-                   const void* d_q, size_t q_stride, const void* d_k, size_t k_stride, const void* d_v,
-                   size_t v_stride, const int32_t* d_slots, const int32_t* d_positions, size_t n_rows,
-                   const float* d_cos, const float* d_sin, size_t max_pos, size_t heads, size_t kv_heads,
-                   size_t head_dim, void* stream);
+typedef struct {
+  int type, cache_type;
+  void *d_q_out, *d_k_cache, *d_v_cache; /* [n_rows][heads][head_dim], [n_slots][kv_heads][head_dim] */
+  size_t n_slots;
+  const void* d_q;
+  size_t q_stride;
+  const void* d_k;
+  size_t k_stride;
+  const void* d_v;
+  size_t v_stride;
+  const int32_t *d_slots, *d_positions; /* [n_rows] */
+  size_t n_rows;
+  const float *d_cos, *d_sin; /* [max_pos][head_dim / 2] */
+  size_t max_pos, heads, kv_heads, head_dim;
+} efg_page_store_args;
+int efg_page_store(const efg_page_store_args* args, void* stream);
 
 /* Causal attention over packed prompts: row r of sequence s attends to rows d_cu[s] .. r.
  * out [n_rows][heads][head_dim] = softmax(scale q k^T) v, query head h reading key head
  * h / (heads / kv_heads). Inputs and output of one type; scores, softmax and sums in FP32 (F32
  * inputs keep FP32 accuracy). head_dim up to 256. out must not overlap an input. */
-int efg_attn_prompt(int type, void* d_out, const void* d_q, size_t q_stride, const void* d_k, size_t k_stride,
-                    const void* d_v, size_t v_stride, const int32_t* d_cu, size_t n_seqs, size_t n_rows, size_t heads,
-                    size_t kv_heads, size_t head_dim, float scale, void* stream);
+typedef struct {
+  int type;
+  float scale;
+  void* d_out;
+  const void* d_q;
+  size_t q_stride;
+  const void* d_k;
+  size_t k_stride;
+  const void* d_v;
+  size_t v_stride;
+  const int32_t* d_cu; /* [n_seqs + 1] */
+  size_t n_seqs, n_rows, heads, kv_heads, head_dim;
+} efg_attn_prompt_args;
+int efg_attn_prompt(const efg_attn_prompt_args* args, void* stream);
 
 /* Attention of each sequence's new tokens over its pages: row i of the chunk of sequence s (of
  * m = d_cu[s + 1] - d_cu[s] rows) attends to positions 0 .. d_kv_len[s] - m + i, so the chunk's
@@ -347,16 +377,26 @@ int efg_attn_prompt(int type, void* d_out, const void* d_q, size_t q_stride, con
  * efg_device_error). A row that sees no position gets zeros. What lies in the pages behind the
  * last position is never used. Types as efg_attn_prompt, the caches of `type` too.
  * Long sequences with few new tokens are cut into parts that meet in d_workspace (16-byte aligned
- * device memory of at least efg_attn_paged_workspace bytes for the same arguments, contents of no
+ * device memory of at least efg_attn_paged_workspace bytes for the same sizes, contents of no
  * account before and after; NULL when that is 0). */
-int efg_attn_paged(int type, void* d_out, const void* d_q, size_t q_stride, const void* d_k_cache,
-                   const void* d_v_cache, size_t n_pages, size_t page_size, const int32_t* d_block_table,
-                   size_t max_pages, const int32_t* d_cu, const int32_t* d_kv_len, size_t n_seqs, size_t n_rows,
-                   size_t max_new, size_t heads, size_t kv_heads, size_t head_dim, float scale, void* d_workspace,
-                   size_t workspace_bytes, void* stream);
-/* Bytes of d_workspace for such a call on the current device. */
-uint64_t efg_attn_paged_workspace(int type, size_t page_size, size_t max_pages, size_t n_seqs, size_t n_rows,
-                                  size_t max_new, size_t heads, size_t kv_heads, size_t head_dim);
+typedef struct {
+  int type;
+  float scale;
+  void* d_out;
+  const void* d_q;
+  size_t q_stride;
+  const void *d_k_cache, *d_v_cache;
+  size_t n_pages, page_size;
+  const int32_t* d_block_table; /* [n_seqs][max_pages] */
+  size_t max_pages;
+  const int32_t *d_cu, *d_kv_len; /* [n_seqs + 1], [n_seqs] */
+  size_t n_seqs, n_rows, max_new, heads, kv_heads, head_dim;
+  void* d_workspace;
+  size_t workspace_bytes;
+} efg_attn_paged_args;
+int efg_attn_paged(const efg_attn_paged_args* args, void* stream);
+/* Bytes of d_workspace for a call with these sizes on the current device (pointers are not looked at). */
+uint64_t efg_attn_paged_workspace(const efg_attn_paged_args* args);
 
 /* ================================================================ .efq and the decode step */
 

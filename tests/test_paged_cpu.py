@@ -104,56 +104,63 @@ def test_c_refusals(efg_lib):
         assert code == 1
         assert text in lib.efg_last_error().decode(), lib.efg_last_error()
 
-    plan = lambda **k: lib.efg_page_plan(*{**dict(t=P, mp=4, s=P, p=P, r=8, cu=P, kv=P, tk=P, c=P, n=P, ns=2, f=P, nf=8,  # noqa: E731
-                                                  np=16, ps=16, st=None), **k}.values())
+    from edgeforge_b200._lib import ATTN_PAGED, ATTN_PROMPT, PAGE_PLAN, PAGE_STORE
+
+    def call(fn, block, **fields):
+        return lambda **k: fn(block.pack(*({**fields, **k}[n] or 0 for n in block.names)), None)
+
+    plan = call(lib.efg_page_plan, PAGE_PLAN, block_table=P, max_pages=4, slots=P, positions=P, n_rows=8, cu=P, kv_len=P,
+                taken=P, cached=P, new=P, n_seqs=2, free=P, n_free=8, n_pages=16, page_size=16)
+    assert lib.efg_page_plan(None, None) == 1
     said(plan(cu=None), "null pointer")
-    said(plan(f=None), "null pointer")
-    said(plan(t=None), "null pointer")
-    said(plan(s=None), "null pointer")
-    said(plan(ps=0), "page size 0")
-    said(plan(np=2**30), "2^31 slots")
-    said(plan(r=2**31), "out of range")
+    said(plan(free=None), "null pointer")
+    said(plan(block_table=None), "null pointer")
+    said(plan(slots=None), "null pointer")
+    said(plan(page_size=0), "page size 0")
+    said(plan(n_pages=2**30), "2^31 slots")
+    said(plan(n_rows=2**31), "out of range")
 
-    store = lambda **k: lib.efg_page_store(*{**dict(ty=2, ct=2, qo=P, kc=P, vc=P, ns=64, q=P, qs=512, k=P, ks=128, v=P,  # noqa: E731
-                                                    vs=128, sl=P, po=P, r=3, co=P, si=P, mp=64, h=8, kv=2, d=64,
-                                                    st=None), **k}.values())
-    said(store(ty=3), "unknown type 3")
-    said(store(ct=1), "the cache has the rows' type")
-    said(store(ty=1, ct=0), "the cache has the rows' type")
-    said(store(d=63), "not an even number")
-    said(store(d=0), "not an even number")
-    said(store(kv=0), "key heads")
+    store = call(lib.efg_page_store, PAGE_STORE, type=2, cache_type=2, q_out=P, k_cache=P, v_cache=P, n_slots=64, q=P,
+                 q_stride=512, k=P, k_stride=128, v=P, v_stride=128, slots=P, positions=P, n_rows=3, cos=P, sin=P,
+                 max_pos=64, heads=8, kv_heads=2, head_dim=64)
+    said(store(type=3), "unknown type 3")
+    said(store(cache_type=1), "the cache has the rows' type")
+    said(store(type=1, cache_type=0), "the cache has the rows' type")
+    said(store(head_dim=63), "not an even number")
+    said(store(head_dim=0), "not an even number")
+    said(store(kv_heads=0), "key heads")
     said(store(q=None), "come together")
-    said(store(si=None), "come together")
-    said(store(ks=127), "shorter than a row")
-    said(store(sl=None), "null pointer")
-    assert store(r=0) == 0  # nothing to do
+    said(store(sin=None), "come together")
+    said(store(k_stride=127), "shorter than a row")
+    said(store(slots=None), "null pointer")
+    assert store(n_rows=0) == 0  # nothing to do
 
-    prompt = lambda **k: lib.efg_attn_prompt(*{**dict(ty=2, o=P, q=P, qs=512, k=P, ks=128, v=P, vs=128, cu=P, n=1, r=5,  # noqa: E731
-                                                      h=8, kv=2, d=64, sc=0.125, st=None), **k}.values())
-    said(prompt(ty=4), "unknown type 4")
-    said(prompt(d=257), "not in 1..256")
-    said(prompt(h=7), "do not divide")
-    said(prompt(kv=0), "do not divide")
-    said(prompt(qs=511), "shorter than a row")
-    said(prompt(vs=100), "shorter than a row")
-    said(prompt(sc=float("nan")), "not finite")
-    said(prompt(sc=float("inf")), "not finite")
+    prompt = call(lib.efg_attn_prompt, ATTN_PROMPT, type=2, scale=0.125, out=P, q=P, q_stride=512, k=P, k_stride=128, v=P,
+                  v_stride=128, cu=P, n_seqs=1, n_rows=5, heads=8, kv_heads=2, head_dim=64)
+    said(prompt(type=4), "unknown type 4")
+    said(prompt(head_dim=257), "not in 1..256")
+    said(prompt(heads=7), "do not divide")
+    said(prompt(kv_heads=0), "do not divide")
+    said(prompt(q_stride=511), "shorter than a row")
+    said(prompt(v_stride=100), "shorter than a row")
+    said(prompt(scale=float("nan")), "not finite")
+    said(prompt(scale=float("inf")), "not finite")
     said(prompt(cu=None), "null pointer")
-    said(prompt(r=2**31), "out of range")
-    assert prompt(r=0) == 0 and prompt(n=0) == 0
+    said(prompt(n_rows=2**31), "out of range")
+    assert prompt(n_rows=0) == 0 and prompt(n_seqs=0) == 0
 
-    paged = lambda **k: lib.efg_attn_paged(*{**dict(ty=2, o=P, q=P, qs=512, k=P, v=P, np=16, ps=16, t=P, mp=4, cu=P, kl=P,  # noqa: E731
-                                                    n=1, r=5, mn=5, h=8, kv=2, d=64, sc=0.125, w=None, wb=0,
-                                                    st=None), **k}.values())
-    said(paged(ps=0), "page size 0")
-    said(paged(np=2**28), "2^31 slots")
-    said(paged(mp=2**28), "2^31 slots")
-    said(paged(mn=2**31), "max_new")
-    said(paged(t=None), "null pointer")
-    said(paged(v=None), "null pointer")
-    said(paged(h=9), "do not divide")
-    assert paged(r=0) == 0 and paged(mn=0) == 0
+    paged = call(lib.efg_attn_paged, ATTN_PAGED, type=2, scale=0.125, out=P, q=P, q_stride=512, k_cache=P, v_cache=P,
+                 n_pages=16, page_size=16, block_table=P, max_pages=4, cu=P, kv_len=P, n_seqs=1, n_rows=5, max_new=5,
+                 heads=8, kv_heads=2, head_dim=64, workspace=0, workspace_bytes=0)
+    said(paged(page_size=0), "page size 0")
+    said(paged(n_pages=2**28), "2^31 slots")
+    said(paged(max_pages=2**28), "2^31 slots")
+    said(paged(max_new=2**31), "max_new")
+    said(paged(block_table=None), "null pointer")
+    said(paged(v_cache=None), "null pointer")
+    said(paged(heads=9), "do not divide")
+    assert paged(n_rows=0) == 0 and paged(max_new=0) == 0
+    assert lib.efg_attn_paged_workspace(None) == 0
 
 
 def test_python_refusals(efg_lib):
