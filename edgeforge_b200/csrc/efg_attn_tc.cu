@@ -62,6 +62,44 @@ constexpr uint32_t idesc_of(uint32_t N, bool b_mn) {
   return (1u << 4) | (fmt << 7) | (fmt << 10) | ((b_mn ? 1u : 0u) << 16) | ((N >> 3) << 17) | ((kTileRows >> 4) << 24);
 }
 
+// ---- MMA forms for a warp-uniform issue loop: executed by the thread whose `one` is set
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xFFFFFFFF;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r;
+}
+template <bool kAdd>
+__device__ __forceinline__ void mma_ss(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %0, 0;\n\t"
+      "setp.ne.u32 p, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], %2, %3, %4, p;\n\t}" ::"r"(one),
+      "r"(d), "l"(a), "l"(b), "r"(idesc), "n"(kAdd ? 1 : 0)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %0, 0;\n\t"
+      "setp.ne.u32 p, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], %3, %4, p;\n\t}" ::"r"(one),
+      "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add)
+      : "memory");
+}
+__device__ __forceinline__ void commit_if(uint32_t one, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.u32 q, %0, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}" ::"r"(one),
+      "r"(smem_addr(bar))
+      : "memory");
+}
+
 // ---- packed FP32 pairs
 __device__ __forceinline__ uint64_t pair(float a, float b) {
   uint64_t r;
@@ -271,52 +309,63 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int item = max(0, issued - kStages); item < issued; ++item)
           wait_own(&kv_full[item % kStages], (item / kStages) & 1, p.err);
       }
-    } else if (warp == 9 && lane == 0 && count > 0) {
+    } else if (warp == 9 && count > 0) {
       // -------------------------------------------------------------- MMA
+      // The whole warp walks this code, so that addresses and descriptors stay warp-uniform (in uniform
+      // registers); one elected thread issues. All 512 columns are this CTA's: TMEM addresses start at 0.
       constexpr uint32_t id_s = idesc_of<T>(kTileKeys, false), id_o = idesc_of<T>(D, true);
-      auto scores = [&](int i, uint32_t k_addr) {
-        const uint64_t dq = smem_desc_sw128(smem_addr(q_s) + i * kTileBytes), dk = smem_desc_sw128(k_addr);
+      const uint32_t one = elect_one();
+      const uint32_t q_addr = base, ring_addr = base + 2 * kTileBytes;
+      auto scores = [&](int i, int item) {
+        const uint64_t dq = smem_desc_sw128(q_addr + i * kTileBytes);
+        const uint64_t dk = smem_desc_sw128(ring_addr + (item % kStages) * kTileBytes);
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
           const uint64_t adv = (ks / 4) * (kPanel >> 4) + (ks % 4) * 2;
-          mma_bf16(tmem + 128 * i, dq + adv, dk + adv, id_s, ks != 0);
+          if (ks == 0)
+            mma_ss<false>(one, 128 * i, dq + adv, dk + adv, id_s);
+          else
+            mma_ss<true>(one, 128 * i, dq + adv, dk + adv, id_s);
         }
-        mma_commit(&s_full[i]);
+        commit_if(one, &s_full[i]);
       };
-      auto values = [&](int i, uint32_t v_addr, bool add) {
-        const uint64_t dv = desc_values(v_addr);
+      auto values = [&](int i, int item, uint32_t add) {
+        const uint64_t dv = desc_values(ring_addr + (item % kStages) * kTileBytes);
+        mma_ts(one, 256 + D * i, 128 * i, dv, id_o, add);
 #pragma unroll
-        for (int ks = 0; ks < kTileKeys / 16; ++ks)
-          mma_bf16_ts(tmem + 256 + D * i, tmem + 128 * i + 8 * ks, dv + ks * (2048 >> 4), id_o, add || ks != 0);
+        for (int ks = 1; ks < kTileKeys / 16; ++ks)
+          mma_ts(one, 256 + D * i, 128 * i + 8 * ks, dv + ks * (2048 >> 4), id_o, 1u);
       };
-      auto stage_addr = [&](int item) { return smem_addr(ring) + (item % kStages) * kTileBytes; };
       bool ok = wait_own(&q_full, 0, p.err) && wait_own(&kv_full[0], 0, p.err);
       if (ok) {
         tc_fence_after();
+#pragma unroll
         for (int i = 0; i < 2; ++i)
-          if (n[i] > 0) scores(i, stage_addr(0));
-        mma_commit(&kv_empty[0]);
+          if (n[i] > 0) scores(i, 0);
+        commit_if(one, &kv_empty[0]);
       }
       for (int j = 0; j < count && ok; ++j) {
         const int vi = 2 * j + 1, ki = 2 * j + 2;
         ok = wait_own(&kv_full[vi % kStages], (vi / kStages) & 1, p.err);
         if (ok && j + 1 < count) ok = wait_own(&kv_full[ki % kStages], (ki / kStages) & 1, p.err);
-        for (int i = 0; i < 2 && ok; ++i) {
-          if (j >= n[i]) continue;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (!ok || j >= n[i]) continue;
           ok = wait_own(&p_ready[i], j & 1, p.err);
-          if (!ok) break;
+          if (!ok) continue;
           tc_fence_after();
-          values(i, stage_addr(vi), j > 0);
+          values(i, vi, j > 0);
           if (j + 1 < n[i])
-            scores(i, stage_addr(ki));
+            scores(i, ki);
           else
-            mma_commit(&o_full[i]);
+            commit_if(one, &o_full[i]);
         }
         if (!ok) break;
-        mma_commit(&kv_empty[vi % kStages]);
-        if (j + 1 < count) mma_commit(&kv_empty[ki % kStages]);
+        commit_if(one, &kv_empty[vi % kStages]);
+        if (j + 1 < count) commit_if(one, &kv_empty[ki % kStages]);
       }
-      mma_commit(&drained);  // no MMA runs on when the TMEM is given back, also after a wait gave up
+      commit_if(one, &drained);  // no MMA runs on when the TMEM is given back, also after a wait gave up
+      __syncwarp();
       mbar_drain(&drained, 0, p.err);
     }
     if (splits > 1) {  // the joining of the softmax warps below
