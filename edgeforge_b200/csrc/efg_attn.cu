@@ -22,7 +22,6 @@ constexpr int kRowWarps = 4;
 // Any head size, stride and alignment: one warp per row and query head.
 template <typename T>
 __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(const AttnParams p) {
-  __shared__ float q_s[kRowWarps][256];
   const int warp = threadIdx.x >> 5;
   if (blockIdx.x == 0) check_offsets(p);
   const int64_t item = static_cast<int64_t>(blockIdx.x) * kRowWarps + warp;
@@ -32,7 +31,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(const AttnPar
   if (s < 0 || s >= p.n_seqs) return;  // behind the last sequence
   Chunk c;
   if (!chunk_of_seq(p, s, c)) return;
-  attend_row<T>(p, c, row, static_cast<int>(item % p.heads), q_s[warp]);
+  attend_row<T>(p, c, row, static_cast<int>(item % p.heads));
 }
 
 template <typename T>
@@ -51,7 +50,12 @@ int launch_attn(int type, const AttnParams& p, int sms, void* work, size_t work_
       return fail(EFG_EINVAL, "attention: a workspace of %zu bytes is needed, got %zu", need, work_bytes);
     return launch_attn_decode(type, p, sms, work, s);
   }
-  if (attn_tc_takes(type, p)) return launch_attn_tc(type, p, sms, s);
+  if (attn_tc_takes(type, p)) {
+    const size_t need = attn_tc_workspace(p, sms);
+    if (need > work_bytes || (need && !work))
+      return fail(EFG_EINVAL, "attention: a workspace of %zu bytes is needed, got %zu", need, work_bytes);
+    return launch_attn_tc(type, p, sms, need ? work : nullptr, s);
+  }
   if (attn_mma_takes(type, p)) return launch_attn_mma(type, p, sms, s);
   if (type == EFG_F32) return launch_rows<float>(p, s);
   if (type == EFG_F16) return launch_rows<__half>(p, s);
@@ -121,10 +125,15 @@ uint64_t efg_attn_paged_workspace(const efg_attn_paged_args* args) {
   p.page_size = static_cast<int64_t>(page_size);
   p.kv_heads = static_cast<int>(kv_heads);
   p.head_dim = static_cast<int>(head_dim);
-  if (kv_heads == 0 || n_seqs == 0 || std::min(max_new, n_rows) * (heads / kv_heads) > efg::kDecodeRows || head_dim > 128)
-    return 0;
+  p.max_new = static_cast<int64_t>(max_new);
+  p.n_rows = static_cast<int64_t>(n_rows);
+  if (kv_heads == 0 || n_seqs == 0 || heads < kv_heads || head_dim > 128) return 0;
+  p.group = static_cast<int>(heads / kv_heads);
   efg::DeviceInfo* dev = efg::current_device();
-  return dev ? efg::attn_decode_workspace(args->type, p, dev->sm_count) : 0;
+  if (!dev) return 0;
+  if (std::min(max_new, n_rows) * p.group <= static_cast<size_t>(efg::kDecodeRows))
+    return efg::attn_decode_workspace(args->type, p, dev->sm_count);
+  return args->type == EFG_F32 || p.group > 128 ? 0 : efg::attn_tc_workspace(p, dev->sm_count);
 }
 
 int efg_attn_paged(const efg_attn_paged_args* args, void* stream) {

@@ -131,6 +131,17 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
+// A line of `line` weights cut into n runs that differ by one at most.
+struct Runs {
+  uint32_t runs, size, longer;  // the first `longer` runs weigh size + 1
+  __device__ __forceinline__ Runs(uint32_t line, uint32_t n) : runs(n), size(line / n), longer(line - line / n * n) {}
+  __device__ __forceinline__ uint32_t begin(uint32_t i) const { return i * size + min(i, longer); }
+  __device__ __forceinline__ uint32_t at(uint32_t place) const {  // the run that holds a place
+    const uint32_t split = longer * (size + 1);
+    return place < split ? place / (size + 1) : longer + (place - split) / size;
+  }
+};
+
 // The tile of rows a CTA owns: its sequence and its place among the sequence's tiles.
 struct RowTile {
   int64_t seq, index;
@@ -182,26 +193,31 @@ __device__ bool find_tile(const AttnParams& p, int64_t want, int64_t mul, int64_
 // One warp computes one row of one query head: 32 keys at a time, a lane per key for the scores
 // (running maximum and sum of the softmax in FP32), then a lane per dim for the values. A key
 // behind the row's last visible one is never read, so what lies there (stale, infinite or NaN)
-// cannot reach the row. head_dim <= 256; q_s holds the row's query as FP32, scaled to base 2.
+// cannot reach the row. head_dim <= 256; lane l holds dims l, l + 32, .. of the query.
 template <typename T>
-__device__ __noinline__ void attend_row(const AttnParams& p, const Chunk& c, int64_t row, int head, float* q_s) {
+__device__ __noinline__ void attend_row(const AttnParams& p, const Chunk& c, int64_t row, int head) {
   const int lane = threadIdx.x & 31, D = p.head_dim, kvh = head / p.group;
   const int32_t count = seen_by(c, static_cast<int32_t>(row));
   const T* q = static_cast<const T*>(p.q) + row * p.q_stride + static_cast<int64_t>(head) * D;
-  for (int d = lane; d < D; d += 32) q_s[d] = attn_widen(q[d]);
-  __syncwarp();
+  float qv[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) qv[i] = lane + 32 * i < D ? attn_widen(q[lane + 32 * i]) : 0.f;
   const float to_base2 = p.scale * 1.4426950408889634f;
   float acc[8] = {}, top = -INFINITY, sum = 0.f;
   for (int32_t j0 = 0; j0 < count; j0 += 32) {
     int64_t kr = -1;
-    float sc = -INFINITY;
+    float sc = -INFINITY, dot = 0.f;
     if (j0 + lane < count) kr = key_row(p, c, j0 + lane);
-    if (kr >= 0) {
-      const T* k = static_cast<const T*>(p.k) + kr * p.k_stride + static_cast<int64_t>(kvh) * D;
-      float dot = 0.f;
-      for (int d = 0; d < D; ++d) dot = fmaf(q_s[d], attn_widen(k[d]), dot);
-      sc = dot * to_base2;
+    const T* k = static_cast<const T*>(p.k) + max(kr, int64_t{0}) * p.k_stride + static_cast<int64_t>(kvh) * D;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int n = min(32, D - 32 * i);
+      for (int d = 0; d < n; ++d) {
+        const float x = __shfl_sync(0xFFFFFFFFu, qv[i], d);
+        if (kr >= 0) dot = fmaf(x, attn_widen(k[32 * i + d]), dot);
+      }
     }
+    if (kr >= 0) sc = dot * to_base2;
     float m = sc;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -233,7 +249,6 @@ __device__ __noinline__ void attend_row(const AttnParams& p, const Chunk& c, int
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     if (lane + 32 * i < D) out[lane + 32 * i] = attn_narrow<T>(acc[i] * inv);
-  __syncwarp();
 }
 
 // Whether a non-finite value of the KV head lies at a position that the row does not see, but

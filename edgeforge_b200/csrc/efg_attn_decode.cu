@@ -94,14 +94,14 @@ __device__ __forceinline__ bool store_row(const AttnParams& p, const Rows& w, in
 }
 
 // Rows marked in `redo` once more, alone, where something behind their last position reached them.
-// One warp; scratch holds one query.
+// One warp.
 template <typename T>
-__device__ __forceinline__ void redo_rows(const AttnParams& p, const Rows& w, int kvh, const int* redo, float* scratch) {
+__device__ __forceinline__ void redo_rows(const AttnParams& p, const Rows& w, int kvh, const int* redo) {
   for (int r = 0; r < w.rows; ++r) {
     const int token = r / p.group;
     if (redo[r] && seen_by(w.c, w.c.begin + token) < w.see_all &&
         reached_from_behind<T>(p, w.c, w.c.begin + token, kvh, w.see_all))
-      attend_row<T>(p, w.c, w.c.begin + token, kvh * p.group + r - token * p.group, scratch);
+      attend_row<T>(p, w.c, w.c.begin + token, kvh * p.group + r - token * p.group);
   }
 }
 
@@ -136,17 +136,6 @@ __device__ __forceinline__ int weight_of(const DecodeParams& dp, int64_t seq) {
   if (!rows_of(dp.a, seq, w)) return 0;
   return (dp.slots ? kHeadCost + tiles_of<T, D>(w) : 1) * dp.a.kv_heads;
 }
-
-// The line cut into `runs` runs whose weights differ by one at most.
-struct Runs {
-  uint32_t runs, size, longer;  // the first `longer` runs weigh size + 1
-  __device__ __forceinline__ Runs(uint32_t line, uint32_t n) : runs(n), size(line / n), longer(line - line / n * n) {}
-  __device__ __forceinline__ uint32_t begin(uint32_t i) const { return i * size + min(i, longer); }
-  __device__ __forceinline__ uint32_t at(uint32_t place) const {  // the run that holds a place
-    const uint32_t split = longer * (size + 1);
-    return place < split ? place / (size + 1) : longer + (place - split) / size;
-  }
-};
 
 // Walks the parts of a run: for each, the sequence, the key head and the tiles [from, to) of it.
 template <typename T, int D>
@@ -581,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
     }
     if (uneven) {
       consumer_barrier();
-      if (warp == 0) redo_rows<T>(p, w, kvh, redo_s, o_s);
+      if (warp == 0) redo_rows<T>(p, w, kvh, redo_s);
     }
     if (warp == 0) {
       if (!whole && walk.from == 0) {  // a key head that is cut begins here: its last piece is in another run
@@ -665,7 +654,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
     }
     __syncthreads();
     if (redo_s[r] && w.see_first < w.see_all) {  // the same for every thread
-      if (warp == 0) redo_rows<T>(p, w, j.kvh, redo_s, weight);
+      if (warp == 0) redo_rows<T>(p, w, j.kvh, redo_s);
       __syncthreads();
       if (tid == 0) redo_s[r] = 0;
     }

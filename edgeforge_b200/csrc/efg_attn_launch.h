@@ -22,6 +22,9 @@ int launch_attn_decode(int type, const AttnParams& p, int sms, void* work, cudaS
 
 // 5th-generation tensor cores (efg_attn_tc.cu): 16-bit types and more than 64 rows per key head.
 bool attn_tc_takes(int type, const AttnParams& p);
-int launch_attn_tc(int type, const AttnParams& p, int sms, cudaStream_t s);
+// With a workspace of attn_tc_workspace bytes the work is cut evenly along the keys; without one (or where
+// that is 0) row tiles stay whole.
+size_t attn_tc_workspace(const AttnParams& p, int sms);
+int launch_attn_tc(int type, const AttnParams& p, int sms, void* work, cudaStream_t s);
 
 }  // namespace efg

@@ -79,7 +79,6 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
   __shared__ int64_t scan_s[kThreads / 32 + 2];
   __shared__ float top_s[4][16], sum_s[4][16];  // per warp, then (row order) per CTA
   __shared__ float part_top[64], part_sum[64];
-  __shared__ float q_s[4][256];
   __shared__ int redo_s[64];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   cg::cluster_group cluster = cg::this_cluster();
@@ -409,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
       const int64_t token = (row0 + r) / p.group;
       const int head = kvh * p.group + static_cast<int>(row0 + r - token * p.group);
       if (reached_from_behind<T>(p, c, c.begin + token, kvh, see_all))
-        attend_row<T>(p, c, c.begin + token, head, q_s[warp]);
+        attend_row<T>(p, c, c.begin + token, head);
     }
   }
   if (splits > 1) cluster.sync();  // the peers read this CTA's shared memory until here

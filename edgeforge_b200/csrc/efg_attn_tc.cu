@@ -6,31 +6,36 @@
 // every key and value tile (128 positions) that TMA brings into a ring. Per tile of keys and row tile:
 //   S = Q K^T       tcgen05.mma, Q and K from shared memory, S (FP32) in TMEM;
 //   P = 2^(S - ref) one softmax thread per row: TMEM -> 128 registers -> exponentials -> 16-bit P back
-//                   into S's own TMEM columns;
+//                   into TMEM;
 //   O += P V        tcgen05.mma with A = P from TMEM, O (FP32) in TMEM.
 // The two row tiles alternate: while one is in its softmax, the tensor cores work for the other.
 // The reference value ref follows the running maximum lazily: it moves (and O is multiplied) only when
 // the maximum has grown by more than 2^8, so weights stay below 256 and O is touched rarely.
 //
 // What bounds it: at head size 128 the two products of a 128 x 128 tile take 1024 tensor-core cycles and
-// its 16384 exponentials 1024 cycles of the special function units; at 64 the exponentials are the
-// bound. Part of them is therefore computed as polynomials on the FMA pipes (kPolyEvery below).
+// its 16384 exponentials 1024 cycles of the special function units, so neither may wait for the other;
+// at 64 the exponentials (and the instructions around them) are the bound. Measured: one 8192-token
+// prompt, 32 query and 8 key heads of 128, BF16: 476 us, 1155 TFLOP/s, 0.70 of the measured GEMM rate;
+// the same with heads of 64 in groups of 8: 383 us, 718 TFLOP/s. Measured and not kept: a part of the
+// exponentials as a degree-4 polynomial on the FMA pipes (no gain at any share), turns at the
+// exponentials for the two warps of a scheduler (491 against 430 us at 64: one warp alone does not fill
+// the special function units), sums and packing one quarter behind the exponentials (540 against 486).
 //
-// Roles (12 warps): 0-3 and 4-7 softmax and epilogue of row tiles 0 and 1, 8 TMA, 9 MMA (10 and 11 only
-// complete the warpgroup that gives its registers to the softmax: 2 x 128 x 208 + 128 x 80 of the
-// launch's 384 x 168). TMEM (512 columns): S0 | S1 | O0 | O1. With few row tiles a cluster of CTAs splits the keys and joins the
-// partial rows through distributed shared memory, in rank order.
+// Roles (12 warps): 0-3 and 4-7 softmax and epilogue of row tiles 0 and 1, 8 TMA, 9 (and 11) MMA, 10 scheduler: a CTA
+// walks many pairs of row tiles, and loads and products of the next one run during the epilogue of the
+// one before. (Registers: 2 x 128 x 224 for the softmax, 128 x 56 for the other warpgroup, of the launch's
+// 384 x 168.) TMEM (512 columns): S0 | S1 | O0 | O1, at head size 64 then P0 | P1: the next S is there before
+// the softmax asks for it. At 128 P overwrites S, and the other row tile's work fills the wait. With a workspace
+// (paged chunks) the work is one line of key tiles cut into equal runs, and a second launch joins the
+// rows of items that were cut, in order.
 #include <algorithm>
 
-#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
 #include "efg_attn.cuh"
 #include "efg_attn_launch.h"
 #include "efg_host.h"
 #include "efg_tcgen05.cuh"
-
-namespace cg = cooperative_groups;
 
 namespace efg {
 namespace {
@@ -125,28 +130,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// 2^x of two values on the FMA pipes: x = n + r with r in [-1/2, 1/2] (adding and subtracting 1.5 * 2^23
-// rounds to an integer), 2^r as the degree-4 polynomial of least relative error on that interval
-// (fitted for this kernel, error 2.6e-6, below the 16-bit rounding of the weight), n added to the
-// exponent. x is held at -126 and above: smaller weights come out as 2^-126 instead.
-__device__ __forceinline__ void poly_ex2(uint64_t x, float& a, float& b) {
-  float xa, xb;
-  unpair(x, xa, xb);
-  x = pair(fmaxf(xa, -126.f), fmaxf(xb, -126.f));
-  const uint64_t magic = pair(12582912.f, 12582912.f), t = add2(x, magic);
-  const uint64_t n = add2(t, pair(-12582912.f, -12582912.f));
-  const uint64_t r = fma2(n, pair(-1.f, -1.f), x);
-  uint64_t y = fma2(pair(0.009570102207362652f, 0.009570102207362652f), r, pair(0.05591785907745361f, 0.05591785907745361f));
-  y = fma2(y, r, pair(0.240247443318367f, 0.240247443318367f));
-  y = fma2(y, r, pair(0.6931217908859253f, 0.6931217908859253f));
-  y = fma2(y, r, pair(0.9999992847442627f, 0.9999992847442627f));
-  float ya, yb, ta, tb;
-  unpair(y, ya, yb);
-  unpair(t, ta, tb);
-  a = __uint_as_float(__float_as_uint(ya) + (__float_as_uint(ta) << 23));
-  b = __uint_as_float(__float_as_uint(yb) + (__float_as_uint(tb) << 23));
-}
-
 // Ties the registers of a TMEM load to the point after its wait.
 __device__ __forceinline__ void after_wait(uint32_t* r) {
 #pragma unroll
@@ -155,26 +138,18 @@ __device__ __forceinline__ void after_wait(uint32_t* r) {
                  "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 
-// One pair in kPolyEvery goes to the FMA pipes.
-template <int D>
-constexpr int kPolyEvery = D == 64 ? 2 : 4;
-
-// Weights of 32 columns, packed to 16 bits; `total` collects the unrounded weights.
-template <typename T, int D, bool kEdge>
-__device__ __forceinline__ void weights32(const uint32_t* s, uint64_t scale, uint64_t nref, uint64_t& total,
+// Weights of 32 columns, packed to 16 bits; `total` collects the unrounded weights. Masked places (-inf) come
+// out as exact zeros.
+template <typename T>
+__device__ __forceinline__ void weights32(const uint32_t* s, uint64_t scale, uint64_t nref, uint64_t (&total)[2],
                                           uint32_t (&out)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const uint64_t x = fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale, nref);
     float a, b;
-    if (!kEdge && i % kPolyEvery<D> == kPolyEvery<D> - 1) {
-      poly_ex2(x, a, b);
-    } else {  // masked places (-inf) come out as exact zeros here
-      unpair(x, a, b);
-      a = ex2(a);
-      b = ex2(b);
-    }
-    total = add2(total, pair(a, b));
+    unpair(fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale, nref), a, b);
+    a = ex2(a);
+    b = ex2(b);
+    total[i % 2] = add2(total[i % 2], pair(a, b));
     out[i] = pack2<T>(a, b);
   }
 }
@@ -185,139 +160,261 @@ __device__ __forceinline__ void cta_barrier() {
   asm volatile("bar.sync 0, %0;" ::"n"(kThreads) : "memory");
 }
 
+// Asks the hardware for a CTA of this grid that has not started: its place is taken over by this CTA
+// (cluster launch control). The answer, 16 bytes, completes on `bar`.
+__device__ __forceinline__ void ask_next_cta(uint4* answer, uint64_t* bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+          smem_addr(answer)),
+      "r"(smem_addr(bar))
+      : "memory");
+}
+// The taken CTA's blockIdx.x, or -1 when every CTA has started (nothing may be asked for after that).
+__device__ __forceinline__ int next_cta(const uint4* answer) {
+  uint32_t got, x, y, z;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 a;\n\t"
+      "ld.shared.b128 a, [%4];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, %3, _}, a;\n\t}"
+      : "=&r"(got), "=&r"(x), "=&r"(y), "=&r"(z)
+      : "r"(smem_addr(answer))
+      : "memory");
+  return got ? static_cast<int>(x) : -1;
+}
+
+// An item that is cut along its keys: its pieces are slot `first` of CTA i (1: the last part of its run, 0: all
+// of it) and slot 0 of the CTAs behind it.
+struct alignas(16) TcJoin {
+  Chunk c;
+  int32_t kvh, token0, first, parts;  // parts 0: nothing begins here that is cut
+};
+
 struct TcParams {
   AttnParams a;
+  TcJoin* joins;      // [ctas]; null: whole items, handed out by the hardware
+  float* slots;       // [ctas][2]{top[256], sum[256], o[D / 4][256][4]}
   int tokens;         // tokens of a row tile
-  int tiles_per_seq;  // pairs of row tiles per sequence at fixed places, or 0: found by a scan
+  int tiles;          // pairs of row tiles of one key head, some of which may turn out to be empty
+  int tiles_per_seq;  // of them at fixed places for every sequence, or 0: found by a scan
   int box_rows;       // rows of one key / value box
 };
+
+constexpr int kItemCost = 3;  // what the begin and end of an item cost, in key tiles
+constexpr int kMinRun = 4;    // weight of a run, at least
+
+// A pair of row tiles of one key head, or a run of its key tiles, as the scheduler warp hands it to the roles.
+struct Item {
+  Chunk c;
+  int32_t kvh, token0;
+  int32_t first, count;  // key tiles
+  int32_t slot;          // -1: all of them, the rows are written out; else the workspace slot of this CTA
+  int32_t stop;
+};
+
+// What a role derives from an item: tokens of the two row tiles, the keys that the last one sees, and how many
+// of the item's key tiles row tile i uses.
+struct Plan {
+  int tok[2], n[2], see_all;
+};
+__device__ __forceinline__ int keys_of(const Chunk& c, int token_end) { return seen_by(c, c.begin + token_end - 1); }
+__device__ __forceinline__ Plan plan_of(const Item& w, int tokens) {
+  Plan a;
+  a.see_all = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    a.tok[i] = max(0, min(tokens, w.c.end - w.c.begin - w.token0 - i * tokens));
+    const int last = a.tok[i] ? keys_of(w.c, w.token0 + i * tokens + a.tok[i]) : 0;
+    a.see_all = max(a.see_all, last);
+    a.n[i] = max(0, min(w.first + w.count, (last + kTileKeys - 1) / kTileKeys) - w.first);
+  }
+  return a;
+}
+// Key tiles of the pair of row tiles that begins at token0.
+__device__ __forceinline__ int tiles_of_pair(const Chunk& c, int token0, int pair_tokens) {
+  return (keys_of(c, min(c.end - c.begin, token0 + pair_tokens)) + kTileKeys - 1) / kTileKeys;
+}
+// Weight of a sequence under one key head: of each pair its begin and end, then its key tiles.
+__device__ __forceinline__ int weight_of(const AttnParams& p, int64_t seq, int pair_tokens) {
+  Chunk c;
+  if (!chunk_of_seq(p, seq, c)) return 0;
+  int sum = 0;
+  for (int t = 0; t < c.end - c.begin; t += pair_tokens) sum += kItemCost + tiles_of_pair(c, t, pair_tokens);
+  return sum;
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_tc_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ CUtensorMap map_q,
                    const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   constexpr int kPanels = D / 64, kStages = kv_stages<D>();
+  constexpr bool kApart = D == 64;  // P beside S in TMEM: the next S does not wait for the value product
   constexpr uint32_t kTileBytes = kPanels * kPanel;
+  constexpr uint32_t kColO = 256, kColP = kApart ? 384 : 0, kStepP = kApart ? 64 : 128;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t q_full, kv_full[kStages], kv_empty[kStages], s_full[2], p_ready[2], o_full[2], drained;
+  __shared__ uint64_t q_full, q_empty, kv_full[kStages], kv_empty[kStages], s_full[2], s_free[2], p_ready[2], pv_done[2],
+      drained[2], item_full[2], item_empty[2], fetch, asked;
+  __shared__ uint4 answer;
+  __shared__ int scan_s[kThreads / 32], run_s[5];
+  __shared__ Item items[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ int64_t scan_s[kThreads / 32 + 2];
   const AttnParams& p = tp.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int splits = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
-  const int kvh = blockIdx.y;
-  const int64_t tile_id = blockIdx.x / splits;
-
-  if (tp.tiles_per_seq == 0 && blockIdx.x == 0 && kvh == 0) check_offsets(p);
-  RowTile rt;
-  if (tp.tiles_per_seq > 0) {
-    rt.seq = tile_id / tp.tiles_per_seq;
-    rt.index = tp.tiles_per_seq - 1 - (tile_id - rt.seq * tp.tiles_per_seq);
-  } else if (!find_tile<kThreads>(p, tile_id, 1, 2 * tp.tokens, scan_s, rt)) {
-    return;  // uniform over the cluster, as the returns below
-  }
-  Chunk c;
-  if (!chunk_of_seq(p, rt.seq, c)) return;
-  const int m = c.end - c.begin;
-  if (rt.index * 2 * tp.tokens >= m) return;
-  const int token0 = static_cast<int>(rt.index) * 2 * tp.tokens;
-  // tokens of the two row tiles, the keys that their last token sees, and tiles of keys of this CTA
-  int tok[2], n[2];
-  int see_last[2], see_all = 0;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    tok[i] = max(0, min(tp.tokens, m - token0 - i * tp.tokens));
-    see_last[i] = tok[i] ? seen_by(c, c.begin + token0 + i * tp.tokens + tok[i] - 1) : 0;
-    see_all = max(see_all, see_last[i]);
-  }
-  const int tiles = (see_all + kTileKeys - 1) / kTileKeys;
-  const int tile_begin = static_cast<int>(static_cast<int64_t>(tiles) * rank / splits);
-  const int tile_end = static_cast<int>(static_cast<int64_t>(tiles) * (rank + 1) / splits);
-  const int count = tile_end - tile_begin;
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    n[i] = max(0, min(tile_end, (see_last[i] + kTileKeys - 1) / kTileKeys) - tile_begin);
-
   const uint32_t raw = smem_addr(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* q_s = smem_raw + (base - raw);
   uint8_t* ring = q_s + 2 * kTileBytes;
   if (tid == 0) {
     mbar_init(&q_full, 1);
-    mbar_init(&drained, 1);
+    mbar_init(&q_empty, kApart ? 2 : 1);
+    mbar_init(&fetch, 1);
+    mbar_init(&asked, 1);
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&kv_empty[i], kApart ? 2 : 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], 128);
       mbar_init(&p_ready[i], 128);
-      mbar_init(&o_full[i], 1);
+      mbar_init(&pv_done[i], 1);
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], kApart ? 11 : 10);  // 8 softmax warps (when they are done with it), TMA, MMA
+      mbar_init(&drained[i], 1);
     }
     fence_barrier_init();
   }
   if (warp == 9) tmem_alloc(&tmem_slot, 512);
+  if (tp.tiles_per_seq == 0 && blockIdx.x == 0) check_offsets(p);
+  if (tp.joins) {
+    // This CTA's run of the line of all items' key tiles: every thread adds up a block of sequences, the one
+    // whose block holds the beginning finds the sequence.
+    const int n_seqs = static_cast<int>(p.n_seqs), per = (n_seqs + kThreads - 1) / kThreads;
+    const int s_lo = min(n_seqs, tid * per), s_hi = min(n_seqs, s_lo + per), pair_tokens = 2 * tp.tokens;
+    int mine = 0;
+    for (int x = s_lo; x < s_hi; ++x) mine += weight_of(p, x, pair_tokens) * p.kv_heads;
+    int inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    if (lane == 31) scan_s[warp] = inc;
+    __syncthreads();
+    int line = 0, before = inc - mine;
+#pragma unroll
+    for (int x = 0; x < kThreads / 32; ++x) {
+      if (x < warp) before += scan_s[x];
+      line += scan_s[x];
+    }
+    const int n_runs = min(static_cast<int>(gridDim.x), max(1, line / kMinRun));
+    if (tid == 0) {
+      tp.joins[blockIdx.x].parts = 0;
+      run_s[2] = line;
+      run_s[3] = n_runs;
+    }
+    if (line > 0 && static_cast<int>(blockIdx.x) < n_runs) {
+      const Runs runs(line, n_runs);
+      const int begin = static_cast<int>(runs.begin(blockIdx.x));
+      if (begin >= before && begin < before + mine) {
+        int at = begin - before, x = s_lo;
+        for (int n; (n = weight_of(p, x, pair_tokens) * p.kv_heads) <= at; ++x) at -= n;
+        run_s[0] = x;
+        run_s[1] = at;
+      }
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
+  // The next item for a role: false at the end of the work or after a wait gave up (recorded). One warp.
+  int turn = 0;
+  auto next_item = [&](Item& w) {
+    const int slot = turn & 1;
+    const bool ok = __all_sync(0xFFFFFFFFu, wait_own(&item_full[slot], (turn >> 1) & 1, p.err));
+    if (!ok) return false;
+    w = items[slot];
+    ++turn;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&item_empty[slot]);
+    return !w.stop;
+  };
+
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == 8 && count > 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 8) {
       // -------------------------------------------------------------- TMA
-      if (lane == 0) {
-        const int live = n[1] > 0 ? 2 : 1;
-        mbar_arrive_expect_tx(&q_full, static_cast<uint32_t>(live * kPanels * tp.tokens * p.group) * 128u);
-        for (int i = 0; i < live; ++i)
-          for (int h = 0; h < kPanels; ++h)
-            tma_load_3d(q_s + (i * kPanels + h) * kPanel, &map_q, 64 * h, kvh * p.group,
-                        c.begin + token0 + i * tp.tokens, &q_full);
-      }
       const int boxes = kTileKeys / tp.box_rows, b = lane % boxes, panel = lane / boxes;
       const bool mine = lane < boxes * kPanels;
-      // first row of this lane's box in the tensor; outside of it (zero fill) behind the last position
-      auto row_of = [&](int tile) -> int32_t {
-        const int pos = tile * kTileKeys + b * tp.box_rows;
-        if (!mine || tile >= tile_end) return 0;
-        if (!p.kv_len) return c.begin + pos;
-        const int64_t none = p.n_pages * p.page_size;
-        const int64_t row = pos < see_all ? key_row(p, c, pos) : -1;
-        return static_cast<int32_t>(row >= 0 ? row : none);
-      };
-      int32_t row = row_of(tile_begin);
+      Item w;
       bool ok = true;
-      int issued = 0;
-      for (int j = 0; j < count && ok; ++j) {
-        const int32_t next = row_of(tile_begin + j + 1);
-        for (int kv = 0; kv < 2 && ok; ++kv) {
-          const int item = 2 * j + kv, st = item % kStages;
-          if (item >= kStages) ok = wait_own(&kv_empty[st], ((item / kStages) - 1) & 1, p.err);
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], kTileBytes);
-          __syncwarp();
-          if (mine)
-            tma_load_3d(ring + st * kTileBytes + panel * kPanel + b * tp.box_rows * 128, kv ? &map_v : &map_k, 64 * panel,
-                        kvh, row, &kv_full[st]);
-          ++issued;
+      int issued = 0, tiles = 0;
+      while (ok && next_item(w)) {
+        const Plan a = plan_of(w, tp.tokens);
+        if (w.count == 0) {
+          if (lane == 0) mbar_arrive(&fetch);
+          continue;
         }
-        row = next;
+        if (tiles > 0) ok = wait_own(&q_empty, (tiles - 1) & 1, p.err);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
+        ++tiles;
+        if (lane == 0) {
+          const int live = a.n[1] > 0 ? 2 : 1;
+          mbar_arrive_expect_tx(&q_full, static_cast<uint32_t>(live * kPanels * tp.tokens * p.group) * 128u);
+          for (int i = 0; i < live; ++i)
+            for (int h = 0; h < kPanels; ++h)
+              tma_load_3d(q_s + (i * kPanels + h) * kPanel, &map_q, 64 * h, w.kvh * p.group,
+                          w.c.begin + w.token0 + i * tp.tokens, &q_full);
+        }
+        // first row of this lane's box in the tensor; outside of it (zero fill) behind the last position
+        auto row_of = [&](int tile) -> int32_t {
+          const int pos = tile * kTileKeys + b * tp.box_rows;
+          if (!mine || tile >= w.first + w.count) return 0;
+          if (!p.kv_len) return w.c.begin + pos;
+          const int64_t row = pos < a.see_all ? key_row(p, w.c, pos) : -1;
+          return static_cast<int32_t>(row >= 0 ? row : p.n_pages * p.page_size);
+        };
+        int32_t row = row_of(w.first);
+        for (int j = 0; j < w.count && ok; ++j) {
+          const int32_t next = row_of(w.first + j + 1);
+          if (j == max(0, w.count - 2) && lane == 0) mbar_arrive(&fetch);  // time to look for the next item
+          for (int kv = 0; kv < 2 && ok; ++kv) {
+            const int st = issued % kStages;
+            if (issued >= kStages) ok = wait_own(&kv_empty[st], ((issued / kStages) - 1) & 1, p.err);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], kTileBytes);
+            __syncwarp();
+            if (mine)
+              tma_load_3d(ring + st * kTileBytes + panel * kPanel + b * tp.box_rows * 128, kv ? &map_v : &map_k,
+                          64 * panel, w.kvh, row, &kv_full[st]);
+            ++issued;
+          }
+          row = next;
+        }
       }
       // the copies in flight land before the shared memory is given back (all have, unless a wait gave up)
-      if (!ok) {
-        wait_own(&q_full, 0, p.err);
-        for (int item = max(0, issued - kStages); item < issued; ++item)
-          wait_own(&kv_full[item % kStages], (item / kStages) & 1, p.err);
-      }
-    } else if (warp == 9 && count > 0) {
+      if (tiles > 0) wait_own(&q_full, (tiles - 1) & 1, p.err);
+      for (int i = max(0, issued - kStages); i < issued; ++i) wait_own(&kv_full[i % kStages], (i / kStages) & 1, p.err);
+    } else if (warp == 9 || (kApart && warp == 11)) {
       // -------------------------------------------------------------- MMA
-      // The whole warp walks this code, so that addresses and descriptors stay warp-uniform (in uniform
-      // registers); one elected thread issues. All 512 columns are this CTA's: TMEM addresses start at 0.
+      // Where P lies apart, each row tile has a warp of its own (9 and 11): a softmax that is ready is never
+      // behind the other's. Where P lies in S, one warp serves both in turn, which keeps the row tiles half
+      // a step apart: at head size 128 the products are the bound, and both at once would leave the tensor
+      // cores idle during both softmaxes. Each whole warp walks this code, so that addresses and
+      // descriptors stay warp-uniform (in uniform registers); one elected thread issues. All 512 columns
+      // are this CTA's: TMEM addresses start at 0.
       constexpr uint32_t id_s = idesc_of<T>(kTileKeys, false), id_o = idesc_of<T>(D, true);
+      constexpr int kMine = kApart ? 1 : 2;  // row tiles of this warp: from `mine` on
+      const int mine = kApart && warp == 11 ? 1 : 0;
       const uint32_t one = elect_one();
-      const uint32_t q_addr = base, ring_addr = base + 2 * kTileBytes;
+      const uint32_t ring_addr = base + 2 * kTileBytes;
       auto scores = [&](int i, int item) {
-        const uint64_t dq = smem_desc_sw128(q_addr + i * kTileBytes);
+        const uint64_t dq = smem_desc_sw128(base + i * kTileBytes);
         const uint64_t dk = smem_desc_sw128(ring_addr + (item % kStages) * kTileBytes);
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
@@ -331,277 +428,405 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       auto values = [&](int i, int item, uint32_t add) {
         const uint64_t dv = desc_values(ring_addr + (item % kStages) * kTileBytes);
-        mma_ts(one, 256 + D * i, 128 * i, dv, id_o, add);
+        const uint32_t o = kColO + D * i, pp = kColP + kStepP * i;
+        mma_ts(one, o, pp, dv, id_o, add);
 #pragma unroll
-        for (int ks = 1; ks < kTileKeys / 16; ++ks)
-          mma_ts(one, 256 + D * i, 128 * i + 8 * ks, dv + ks * (2048 >> 4), id_o, 1u);
+        for (int ks = 1; ks < kTileKeys / 16; ++ks) mma_ts(one, o, pp + 8 * ks, dv + ks * (2048 >> 4), id_o, 1u);
+        commit_if(one, &pv_done[i]);
       };
-      bool ok = wait_own(&q_full, 0, p.err) && wait_own(&kv_full[0], 0, p.err);
-      if (ok) {
-        tc_fence_after();
+      // The tile has landed. (A stage is given back only after that, also by a row tile that has no use for it:
+      // the other one's use of the stage before is over then.)
+      auto landed = [&](int item) { return wait_own(&kv_full[item % kStages], (item / kStages) & 1, p.err); };
+      Item w;
+      bool ok = true;
+      int ring_at = 0, tiles = 0;     // ring items and items with keys before this one
+      int step[kMine] = {};           // key tiles of each row tile before this item
+      while (ok && next_item(w)) {
+        const Plan a = plan_of(w, tp.tokens);
+        if (w.count == 0) continue;
+        int n[kMine];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (n[i] > 0) scores(i, 0);
-        commit_if(one, &kv_empty[0]);
-      }
-      for (int j = 0; j < count && ok; ++j) {
-        const int vi = 2 * j + 1, ki = 2 * j + 2;
-        ok = wait_own(&kv_full[vi % kStages], (vi / kStages) & 1, p.err);
-        if (ok && j + 1 < count) ok = wait_own(&kv_full[ki % kStages], (ki / kStages) & 1, p.err);
+        for (int x = 0; x < kMine; ++x) n[x] = kApart && mine == 1 ? a.n[1] : a.n[x];
+        ok = wait_own(&q_full, tiles & 1, p.err) && landed(ring_at);
+        ++tiles;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (!ok || j >= n[i]) continue;
-          ok = wait_own(&p_ready[i], j & 1, p.err);
+        for (int x = 0; x < kMine; ++x) {
+          if (n[x] == 0) continue;
+          // S of the item before has been read (where P lies in S, its value product precedes these MMAs)
+          if (kApart && step[x] > 0) ok = ok && wait_own(&s_free[mine + x], (step[x] - 1) & 1, p.err);
           if (!ok) continue;
           tc_fence_after();
-          values(i, vi, j > 0);
-          if (j + 1 < n[i])
-            scores(i, ki);
-          else
-            commit_if(one, &o_full[i]);
+          scores(mine + x, ring_at);
         }
         if (!ok) break;
-        commit_if(one, &kv_empty[vi % kStages]);
-        if (j + 1 < count) commit_if(one, &kv_empty[ki % kStages]);
+        commit_if(one, &kv_empty[ring_at % kStages]);
+        if (w.count == 1) commit_if(one, &q_empty);
+        for (int j = 0; j < w.count && ok; ++j) {
+          const int vi = ring_at + 2 * j + 1, ki = vi + 1;
+          const bool more = j + 1 < w.count;
+          if (kApart && more) {
+            ok = landed(ki);
+            if (j + 1 < n[0]) {
+              ok = ok && wait_own(&s_free[mine], (step[0] + j) & 1, p.err);
+              if (!ok) break;
+              tc_fence_after();
+              scores(mine, ki);
+            }
+            commit_if(one, &kv_empty[ki % kStages]);
+            if (j + 2 == w.count) commit_if(one, &q_empty);
+          }
+          ok = ok && landed(vi);
+          if (!kApart && more) ok = ok && landed(ki);
+#pragma unroll
+          for (int x = 0; x < kMine; ++x) {
+            if (j >= n[x]) continue;
+            ok = ok && wait_own(&p_ready[mine + x], (step[x] + j) & 1, p.err);
+            if (!ok) continue;
+            tc_fence_after();
+            values(mine + x, vi, j > 0);
+            if (!kApart && j + 1 < n[x]) scores(x, ki);
+          }
+          if (!ok) break;
+          commit_if(one, &kv_empty[vi % kStages]);
+          if (!kApart && more) {
+            commit_if(one, &kv_empty[ki % kStages]);
+            if (j + 2 == w.count) commit_if(one, &q_empty);
+          }
+        }
+        ring_at += 2 * w.count;
+#pragma unroll
+        for (int x = 0; x < kMine; ++x) step[x] += n[x];
       }
-      commit_if(one, &drained);  // no MMA runs on when the TMEM is given back, also after a wait gave up
+      commit_if(one, &drained[mine]);  // no MMA runs on when the TMEM is given back, also after a wait gave up
       __syncwarp();
-      mbar_drain(&drained, 0, p.err);
-    }
-    if (splits > 1) {  // the joining of the softmax warps below
-      cta_barrier();
-      cluster.sync();
-      cluster.sync();
+      mbar_drain(&drained[mine], 0, p.err);
+    } else if (warp == 10) {
+      // -------------------------------------------------------------- scheduler
+      // Items are numbered key head by key head, the pairs of row tiles of a sequence last to first (the last see
+      // the most keys). A CTA begins with the item of its own number; when its loads are nearly issued it
+      // takes over the next CTA that the hardware has not started, so the GPU stays balanced whatever the
+      // items take. Sequences are counted 32 at a time.
+      // With a workspace (few items for the GPU, or ragged ones) the line of all key tiles is cut into equal runs
+      // instead, one per CTA, and items are cut where the runs end.
+      const int total = tp.tiles * p.kv_heads, pair_tokens = 2 * tp.tokens;
+      int sent = 0;
+      bool ok = true;
+      auto send = [&](const Item& w) {
+        const int slot = sent & 1;
+        if (sent >= 2) ok = wait_own(&item_empty[slot], ((sent >> 1) - 1) & 1, p.err);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) return;
+        if (lane == 0) {
+          items[slot] = w;
+          mbar_arrive(&item_full[slot]);
+        }
+        __syncwarp();
+        ++sent;
+      };
+      Item w;
+      w.stop = 0;
+      if (tp.joins) {
+        const int line = run_s[2], n_runs = run_s[3];
+        if (line > 0 && static_cast<int>(blockIdx.x) < n_runs) {
+          const Runs runs(line, n_runs);
+          const int end = static_cast<int>(runs.begin(blockIdx.x + 1));
+          int seq = run_s[0], at = run_s[1], left = end - static_cast<int>(runs.begin(blockIdx.x)), parts = 0;
+          while (left > 0 && ok && seq < p.n_seqs) {
+            const int weight = weight_of(p, seq, pair_tokens);  // 0: nothing to do there
+            if (at >= weight * p.kv_heads) {
+              ++seq;
+              at = 0;
+              continue;
+            }
+            chunk_of_seq(p, seq, w.c);
+            w.kvh = at / weight;
+            int off = at - w.kvh * weight, tiles = 0;
+            for (w.token0 = 0;; w.token0 += pair_tokens) {  // the pair that holds the place
+              tiles = tiles_of_pair(w.c, w.token0, pair_tokens);
+              if (off < kItemCost + tiles) break;
+              off -= kItemCost + tiles;
+            }
+            const int step = min(kItemCost + tiles - off, left), to = off + step - kItemCost;
+            left -= step;
+            at += step;
+            // (a run that ends before the item's first key tile leaves it to the next; rows that see nothing
+            // belong to the run that holds the end of their item)
+            if (to <= 0 && !(tiles == 0 && to == 0)) continue;
+            w.first = max(0, off - kItemCost);
+            w.count = to - w.first;
+            const bool whole = w.count == tiles;
+            w.slot = whole ? -1 : min(parts, 1);
+            ++parts;
+            if (!whole && w.first == 0 && lane == 0)  // its last piece is in the run that holds its end
+              tp.joins[blockIdx.x] = TcJoin{w.c, w.kvh, w.token0, w.slot,
+                                            static_cast<int>(runs.at(end - 1 + (tiles - to))) - static_cast<int>(blockIdx.x) + 1};
+            send(w);
+          }
+        }
+      } else {
+        int asks = 0, s0 = 0, before = 0, last_tile = 0;  // the scan stands at sequence s0 with `before` tiles before it
+        // the number of the next item, -1 behind the last
+        auto next_number = [&]() -> int {
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&asked, 16);
+            ask_next_cta(&answer, &asked);
+          }
+          __syncwarp();
+          ok = __all_sync(0xFFFFFFFFu, wait_own(&asked, asks & 1, p.err));
+          ++asks;
+          if (!ok) return -1;
+          const int x = next_cta(&answer);
+          fence_proxy_async();  // the answer has been read before the next one may be written
+          __syncwarp();
+          return x;
+        };
+        for (int wi = static_cast<int>(blockIdx.x); wi >= 0 && ok; wi = next_number()) {
+          const int kvh = wi / tp.tiles, tile = wi - kvh * tp.tiles;
+          if (wi >= total) continue;
+          int64_t seq = -1, index = 0;
+          if (tp.tiles_per_seq > 0) {
+            seq = tile / tp.tiles_per_seq;
+            index = tp.tiles_per_seq - 1 - (tile - seq * tp.tiles_per_seq);
+          } else {
+            if (tile < last_tile) s0 = before = 0;  // another key head
+            last_tile = tile;
+            for (; s0 < p.n_seqs; s0 += 32) {
+              int64_t m = s0 + lane < p.n_seqs ? static_cast<int64_t>(p.cu[s0 + lane + 1]) - p.cu[s0 + lane] : 0;
+              // lengths that make no sense get one tile, which records them
+              const int n = m < 0 || m > p.n_rows ? 1 : static_cast<int>((m + pair_tokens - 1) / pair_tokens);
+              int inc = n;
+#pragma unroll
+              for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+                if (lane >= o) inc += up;
+              }
+              const uint32_t hit = __ballot_sync(0xFFFFFFFFu, tile >= before + inc - n && tile < before + inc);
+              if (hit) {
+                const int l = __ffs(hit) - 1;
+                seq = s0 + l;
+                index = __shfl_sync(0xFFFFFFFFu, before + inc - 1 - tile, l);
+                break;
+              }
+              before += __shfl_sync(0xFFFFFFFFu, inc, 31);
+            }
+          }
+          if (seq < 0 || !chunk_of_seq(p, seq, w.c) || index * pair_tokens >= w.c.end - w.c.begin) continue;
+          w.kvh = kvh;
+          w.token0 = static_cast<int>(index) * pair_tokens;
+          w.first = 0;
+          w.count = tiles_of_pair(w.c, w.token0, pair_tokens);
+          w.slot = -1;
+          send(w);
+          if (ok) ok = __all_sync(0xFFFFFFFFu, wait_own(&fetch, (sent - 1) & 1, p.err));
+        }
+      }
+      if (ok) {
+        w.stop = 1;
+        send(w);
+      }
     }
   } else {
     // ---------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int i = warp >> 2, r = tid & 127;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-    const uint32_t s_addr = tmem + lanes + 128 * i, o_addr = tmem + lanes + 256 + D * i;
+    const uint32_t s_addr = tmem + lanes + 128 * i, o_addr = tmem + lanes + kColO + D * i;
+    const uint32_t p_addr = tmem + lanes + kColP + kStepP * i;
     const int token = r / p.group;  // of the row tile
-    const bool live = token < tok[i];
-    const int sees = live ? seen_by(c, c.begin + token0 + i * tp.tokens + token) : 0;
-    const int see_first = tok[i] ? seen_by(c, c.begin + token0 + i * tp.tokens) : 0;
     const float scale2 = p.scale * 1.4426950408889634f;
     const uint64_t scale_pair = pair(scale2, scale2);
-    uint64_t total = pair(0.f, 0.f);
-    float ref = 0.f;
     bool ok = true;
-    for (int j = 0; j < n[i]; ++j) {
-      ok = wait_own(&s_full[i], j & 1, p.err);
-      if (!__all_sync(0xFFFFFFFFu, ok)) break;
-      tc_fence_after();
-      uint32_t s[128];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) tmem_ld32(s_addr + 32 * q, s + 32 * q);
-      tmem_wait_ld();
-#pragma unroll
-      for (int q = 0; q < 4; ++q) after_wait(s + 32 * q);
-      const int key0 = (tile_begin + j) * kTileKeys;
-      const bool edge = key0 + kTileKeys > see_first;
-      if (edge) {
+    int ring_at = 0, step = 0;  // ring items, and key tiles of this row tile, before this item
+    for (;; ++turn) {
+      const int slot = turn & 1;
+      // (read again where needed: the registers are for S)
+      ok = ok && __all_sync(0xFFFFFFFFu, wait_own(&item_full[slot], (turn >> 1) & 1, p.err));
+      if (!ok || items[slot].stop) break;
+      int n, first, count, see_all, sees, see_first;
+      {
+        const Item w = items[slot];
+        const Plan a = plan_of(w, tp.tokens);
+        n = a.n[i];
+        first = w.first;
+        count = w.count;
+        see_all = a.see_all;
+        const int row0 = w.c.begin + w.token0 + i * tp.tokens;
+        sees = token < a.tok[i] ? seen_by(w.c, row0 + token) : 0;
+        see_first = a.tok[i] ? seen_by(w.c, row0) : 0;
+      }
+      uint64_t total[2] = {0, 0};  // pairs of FP32 zeros
+      float ref = 0.f;
+      for (int j = 0; j < n; ++j, ++step) {
+        ok = wait_own(&s_full[i], step & 1, p.err);
+        if (!__all_sync(0xFFFFFFFFu, ok)) break;
+        tc_fence_after();
+        uint32_t s[128];
+        const int key0 = (first + j) * kTileKeys;
+        const bool edge = key0 + kTileKeys > see_first;
         const int limit = sees - key0;
 #pragma unroll
-        for (int k = 0; k < 128; ++k)
-          if (k >= limit) s[k] = 0xFF800000u;  // -inf
-      }
-      float mx[4];
+        for (int q = 0; q < 4; ++q) tmem_ld32(s_addr + 32 * q, s + 32 * q);
+        tmem_wait_ld();
 #pragma unroll
-      for (int q = 0; q < 4; ++q) mx[q] = fmaxf(__uint_as_float(s[q]), __uint_as_float(s[q + 4]));
+        for (int q = 0; q < 4; ++q) after_wait(s + 32 * q);
+        if (kApart) {
+          tc_fence_before();
+          mbar_arrive(&s_free[i]);
+        }
+        if (edge) {
 #pragma unroll
-      for (int k = 8; k < 128; k += 8)
+          for (int k = 0; k < 128; ++k)
+            if (k >= limit) s[k] = 0xFF800000u;  // -inf
+        }
+        float mx[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) mx[q] = max3(mx[q], __uint_as_float(s[k + q]), __uint_as_float(s[k + q + 4]));
-      const float high = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
-      if (j == 0) {
-        ref = high == -INFINITY ? 0.f : high;
-      } else {
-        const bool move = high - ref > kLazy;
-        if (__any_sync(0xFFFFFFFFu, move)) {  // the MMAs of the tile before are done: S of this one follows them
-          const float back = move ? ex2(ref - high) : 1.f;
-          if (move) ref = high;
-          float ta, tb;
-          unpair(total, ta, tb);
-          total = pair(ta * back, tb * back);
+        for (int q = 0; q < 4; ++q) mx[q] = fmaxf(__uint_as_float(s[q]), __uint_as_float(s[q + 4]));
+#pragma unroll
+        for (int k = 8; k < 128; k += 8)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) mx[q] = max3(mx[q], __uint_as_float(s[k + q]), __uint_as_float(s[k + q + 4]));
+        const float high = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
+        // P and O of the key tile before are free once its value product is done
+        const auto before_done = [&] {
+          if (j > 0) ok = wait_own(&pv_done[i], (step - 1) & 1, p.err);
+          tc_fence_after();
+        };
+        if (j == 0) {
+          ref = high == -INFINITY ? 0.f : high;
+        } else {
+          const bool move = high - ref > kLazy;
+          if (__any_sync(0xFFFFFFFFu, move)) {
+            before_done();
+            const float back = move ? ex2(ref - high) : 1.f;
+            if (move) ref = high;
+            total[0] = fma2(total[0], pair(back, back), 0);
+            total[1] = fma2(total[1], pair(back, back), 0);
 #pragma unroll 1
-          for (int q = 0; q < D / 32; ++q) {
-            uint32_t o[32];
+            for (int q = 0; q < D / 32; ++q) {
+              uint32_t o[32];
+              tmem_ld32(o_addr + 32 * q, o);
+              tmem_wait_ld();
+              after_wait(o);
+              uint32_t lo[16], hi[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                lo[e] = __float_as_uint(__uint_as_float(o[e]) * back);
+                hi[e] = __float_as_uint(__uint_as_float(o[e + 16]) * back);
+              }
+              tmem_st16(o_addr + 32 * q, lo);
+              tmem_st16(o_addr + 32 * q + 16, hi);
+            }
+          }
+        }
+        const uint64_t nref = pair(-ref, -ref);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t x[16];
+          weights32<T>(s + 32 * q, scale_pair, nref, total, x);
+          if (q == 0) before_done();
+          tmem_st16(p_addr + 16 * q, x);
+        }
+        if (!__all_sync(0xFFFFFFFFu, ok)) break;
+        if (key0 + kTileKeys > see_all) {
+          // values behind the last position: whatever lies there would meet weights of zero, and 0 times
+          // infinity is NaN, so it becomes zero
+          const int item = ring_at + 2 * j + 1, st = item % kStages;
+          ok = wait_own(&kv_full[st], (item / kStages) & 1, p.err);
+          if (ok && key0 + r >= see_all) {
+#pragma unroll
+            for (int h = 0; h < kPanels; ++h) {
+              uint4* row = reinterpret_cast<uint4*>(ring + st * kTileBytes + h * kPanel + r * 128);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) row[e] = make_uint4(0, 0, 0, 0);
+            }
+          }
+          fence_proxy_async();
+          if (!__all_sync(0xFFFFFFFFu, ok)) break;
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_ready[i]);
+      }
+      ring_at += 2 * count;
+      float ta, tb;
+      unpair(add2(total[0], total[1]), ta, tb);
+      const float row_sum = ta + tb;
+      if (ok && n > 0) ok = wait_own(&pv_done[i], (step - 1) & 1, p.err);
+      tc_fence_after();
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      const Item w = items[slot];
+      const Plan a = plan_of(w, tp.tokens);
+      const int row0 = w.c.begin + w.token0 + i * tp.tokens;
+      const bool live = token < a.tok[i];
+
+      if (w.slot < 0) {
+        const float inv = sees > 0 && row_sum != 0.f ? 1.f / row_sum : 0.f;
+        const int64_t row = row0 + token;
+        const int head = w.kvh * p.group + r - token * p.group;
+        T* out = static_cast<T*>(p.out) + (row * p.heads + head) * p.head_dim;
+        bool finite = true;
+#pragma unroll 1
+        for (int q = 0; q < D / 32; ++q) {
+          uint32_t o[32];
+          if (n > 0) {
             tmem_ld32(o_addr + 32 * q, o);
             tmem_wait_ld();
             after_wait(o);
-            uint32_t lo[16], hi[16];
+          }
+          if (live && ok) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              lo[e] = __float_as_uint(__uint_as_float(o[e]) * back);
-              hi[e] = __float_as_uint(__uint_as_float(o[e + 16]) * back);
+            for (int e = 0; e < 32; e += 8) {
+              uint32_t x[4];
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                const float u = inv == 0.f ? 0.f : __uint_as_float(o[e + 2 * y]) * inv;
+                const float v = inv == 0.f ? 0.f : __uint_as_float(o[e + 2 * y + 1]) * inv;
+                finite = finite && fabsf(u) <= 3.402823466e38f && fabsf(v) <= 3.402823466e38f;
+                x[y] = pack2<T>(u, v);
+              }
+              if (32 * q + e < p.head_dim)
+                *reinterpret_cast<uint4*>(out + 32 * q + e) = make_uint4(x[0], x[1], x[2], x[3]);
             }
-            tmem_st16(o_addr + 32 * q, lo);
-            tmem_st16(o_addr + 32 * q + 16, hi);
           }
         }
-      }
-      const uint64_t nref = pair(-ref, -ref);
-      if (edge) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t w[16];
-          weights32<T, D, true>(s + 32 * q, scale_pair, nref, total, w);
-          tmem_st16(s_addr + 16 * q, w);
-        }
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t w[16];
-          weights32<T, D, false>(s + 32 * q, scale_pair, nref, total, w);
-          tmem_st16(s_addr + 16 * q, w);
-        }
-      }
-      if (key0 + kTileKeys > see_all) {
-        // values behind the last position: whatever lies there would meet weights of zero, and 0 times
-        // infinity is NaN, so it becomes zero
-        const int item = 2 * j + 1, st = item % kStages;
-        ok = wait_own(&kv_full[st], (item / kStages) & 1, p.err);
-        if (ok && key0 + r >= see_all) {
-#pragma unroll
-          for (int h = 0; h < kPanels; ++h) {
-            uint4* row = reinterpret_cast<uint4*>(ring + st * kTileBytes + h * kPanel + r * 128);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) row[e] = make_uint4(0, 0, 0, 0);
-          }
-        }
-        fence_proxy_async();
-        if (!__all_sync(0xFFFFFFFFu, ok)) break;
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&p_ready[i]);
-    }
-    float ta, tb;
-    unpair(total, ta, tb);
-    const float row_sum = ta + tb;
-    if (ok && n[i] > 0) ok = wait_own(&o_full[i], 0, p.err);
-    tc_fence_after();
-    ok = __all_sync(0xFFFFFFFFu, ok);
-
-    if (splits == 1) {
-      const float inv = sees > 0 && row_sum != 0.f ? 1.f / row_sum : 0.f;
-      const int64_t row = c.begin + token0 + i * tp.tokens + token;
-      const int head = kvh * p.group + r - token * p.group;
-      T* out = static_cast<T*>(p.out) + (row * p.heads + head) * p.head_dim;
-      bool finite = true;
-#pragma unroll 1
-      for (int q = 0; q < D / 32; ++q) {
-        uint32_t o[32];
-        if (n[i] > 0) {
-          tmem_ld32(o_addr + 32 * q, o);
-          tmem_wait_ld();
-          after_wait(o);
-        }
-        if (live && ok) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint32_t w[4];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const float a = inv == 0.f ? 0.f : __uint_as_float(o[e + 2 * x]) * inv;
-              const float b = inv == 0.f ? 0.f : __uint_as_float(o[e + 2 * x + 1]) * inv;
-              finite = finite && fabsf(a) <= 3.402823466e38f && fabsf(b) <= 3.402823466e38f;
-              w[x] = pack2<T>(a, b);
-            }
-            if (32 * q + e < p.head_dim)
-              *reinterpret_cast<uint4*>(out + 32 * q + e) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-      }
-      // a row may not be reached by what lies at positions it does not see
-      uint32_t redo = __ballot_sync(0xFFFFFFFFu, live && ok && !finite && sees < see_all);
-      if (redo) {
-        // scratch for one query: this warp's part of the Q area, whose MMAs are done
-        float* scratch = reinterpret_cast<float*>(q_s + i * kTileBytes) + (warp & 3) * 256;
-        __syncwarp();
+        // a row may not be reached by what lies at positions it does not see
+        uint32_t redo = __ballot_sync(0xFFFFFFFFu, live && ok && !finite && sees < see_all);
         while (redo) {
           const int l = __ffs(redo) - 1;
           redo &= redo - 1;
           const int64_t row_l = __shfl_sync(0xFFFFFFFFu, row, l);
           const int head_l = __shfl_sync(0xFFFFFFFFu, head, l);
-          if (reached_from_behind<T>(p, c, row_l, kvh, see_all)) attend_row<T>(p, c, row_l, head_l, scratch);
+          if (reached_from_behind<T>(p, w.c, row_l, w.kvh, see_all)) attend_row<T>(p, w.c, row_l, head_l);
         }
-      }
-    }
-    if (splits > 1) {
-      // partial rows to shared memory (every operand there has been used): row r of [256][D] FP32 with its
-      // 16-byte chunks rotated by r, so that a warp's rows fall into different banks
-      cta_barrier();
-      float* o_s = reinterpret_cast<float*>(q_s);
-      float *part_top = o_s + 256 * D, *part_sum = part_top + 256;
-      int* redo_s = reinterpret_cast<int*>(part_sum + 256);
-      redo_s[tid] = 0;
-      // a row that saw none of these keys takes no part
-      part_top[tid] = row_sum == 0.f ? -INFINITY : ref;
-      part_sum[tid] = row_sum;
+      } else {
+        // a piece: row `tid` of the slot; 16-byte pieces of the rows lie side by side, so that a warp's stores do
+        float* slot_o = tp.slots + (static_cast<int64_t>(blockIdx.x) * 2 + w.slot) * (256 * (D + 2));
+        if (live) {
+          slot_o[tid] = row_sum == 0.f ? -INFINITY : ref;  // a row that saw none of these keys takes no part
+          slot_o[256 + tid] = row_sum;
+        }
 #pragma unroll 1
-      for (int q = 0; q < D / 32; ++q) {
-        uint32_t o[32];
-        if (n[i] > 0) {
-          tmem_ld32(o_addr + 32 * q, o);
-          tmem_wait_ld();
-          after_wait(o);
-        } else {
+        for (int q = 0; q < D / 32; ++q) {
+          uint32_t o[32];
+          if (n > 0) {
+            tmem_ld32(o_addr + 32 * q, o);
+            tmem_wait_ld();
+            after_wait(o);
+          } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0u;
+            for (int e = 0; e < 32; ++e) o[e] = 0u;
+          }
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<uint4*>(slot_o + 512 + ((8 * q + e) * 256 + tid) * 4) =
+                  make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          *reinterpret_cast<uint4*>(o_s + tid * D + ((8 * q + e + r) % (D / 4)) * 4) =
-              make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
       }
+      tc_fence_before();  // O has been read before this warp's next p_ready lets the MMAs write it
       __syncwarp();
-      cluster.sync();
-      // this CTA's share of the rows, 8 dims a thread, partials in rank order
-      const int share = 256 / splits, r_lo = rank * share;
-      for (int e = tid; e < share * (D / 8); e += 256) {
-        const int rr = r_lo + e / (D / 8), d = (e % (D / 8)) * 8, ti = rr >> 7, tr = rr & 127, tt = tr / p.group;
-        if (tt >= tok[ti] || d >= p.head_dim) continue;
-        float mx = -INFINITY;
-        for (int w = 0; w < splits; ++w) mx = fmaxf(mx, cluster.map_shared_rank(part_top, w)[rr]);
-        const float high = mx == -INFINITY ? 0.f : mx;
-        float acc[8] = {}, l = 0.f;
-        for (int w = 0; w < splits; ++w) {
-          const float f = ex2(cluster.map_shared_rank(part_top, w)[rr] - high);
-          l += f * cluster.map_shared_rank(part_sum, w)[rr];
-          const float* o = cluster.map_shared_rank(o_s, w) + rr * D;
-          const float4 a = *reinterpret_cast<const float4*>(o + ((d / 4 + tr) % (D / 4)) * 4);
-          const float4 b = *reinterpret_cast<const float4*>(o + ((d / 4 + 1 + tr) % (D / 4)) * 4);
-          acc[0] += f * a.x, acc[1] += f * a.y, acc[2] += f * a.z, acc[3] += f * a.w;
-          acc[4] += f * b.x, acc[5] += f * b.y, acc[6] += f * b.z, acc[7] += f * b.w;
-        }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        uint32_t w[4];
-        bool finite = true;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          acc[2 * x] *= inv;
-          acc[2 * x + 1] *= inv;
-          finite = finite && fabsf(acc[2 * x]) <= 3.402823466e38f && fabsf(acc[2 * x + 1]) <= 3.402823466e38f;
-          w[x] = pack2<T>(acc[2 * x], acc[2 * x + 1]);
-        }
-        const int64_t row = c.begin + token0 + ti * tp.tokens + tt;
-        const int head = kvh * p.group + tr - tt * p.group;
-        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (row * p.heads + head) * p.head_dim + d) =
-            make_uint4(w[0], w[1], w[2], w[3]);
-        if (!finite) redo_s[rr] = 1;
-      }
-      __syncwarp();
-      cluster.sync();  // every peer has read this CTA's partials; redo_s is complete
-      float* scratch = o_s + warp * 256;
-      for (int x = warp; x < share; x += 8) {
-        const int rr = r_lo + x, ti = rr >> 7, tr = rr & 127, tt = tr / p.group;
-        if (tt >= tok[ti] || !redo_s[rr]) continue;
-        const int64_t row = c.begin + token0 + ti * tp.tokens + tt;
-        if (seen_by(c, static_cast<int>(row)) < see_all && reached_from_behind<T>(p, c, row, kvh, see_all))
-          attend_row<T>(p, c, row, kvh * p.group + tr - tt * p.group, scratch);
-      }
+      if (lane == 0) mbar_arrive(&item_empty[slot]);
     }
   }
   tc_fence_before();
@@ -609,8 +834,70 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
+// Joins the pieces of the item that begins at the end of CTA blockIdx.x's run. A block takes 32 of its 256 rows,
+// a lane per row; a warp takes every eighth 16 bytes of the rows.
 template <typename T, int D>
-int launch(const AttnParams& p, int64_t max_new, int64_t max_keys, int sms, cudaStream_t s) {
+__global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant__ TcParams tp) {
+  constexpr int kMine = D / 4 / 8;
+  __shared__ int redo_s[32];
+  const AttnParams& p = tp.a;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.y * 32 + lane;
+  if (threadIdx.x < 32) redo_s[threadIdx.x] = 0;
+  pdl_wait();
+  const TcJoin j = tp.joins[blockIdx.x];
+  if (j.parts <= 1) return;
+  __syncthreads();
+  constexpr int64_t kSlot = 256 * (D + 2);
+  const float* slots = tp.slots + static_cast<int64_t>(blockIdx.x) * 2 * kSlot;
+  auto slot = [&](int x) { return slots + (2 * x + (x == 0 ? j.first : 0)) * kSlot; };
+  const int i = r >> 7, token = (r & 127) / p.group, head = j.kvh * p.group + (r & 127) - token * p.group;
+  const int tok = min(tp.tokens, j.c.end - j.c.begin - j.token0 - i * tp.tokens);
+  const bool live = token < tok;
+  const int row = j.c.begin + j.token0 + i * tp.tokens + token;
+  if (live) {
+    float mx = -INFINITY;
+#pragma unroll 4
+    for (int x = 0; x < j.parts; ++x) mx = fmaxf(mx, slot(x)[r]);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float l = 0.f;
+    float4 acc[kMine];
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) acc[k] = make_float4(0, 0, 0, 0);
+#pragma unroll 2
+    for (int x = 0; x < j.parts; ++x) {
+      const float* o = slot(x);
+      const float f = ex2(o[r] - ref);
+      l += f * o[256 + r];
+#pragma unroll
+      for (int k = 0; k < kMine; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(o + 512 + ((warp + 8 * k) * 256 + r) * 4);
+        acc[k].x += f * v.x, acc[k].y += f * v.y, acc[k].z += f * v.z, acc[k].w += f * v.w;
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(row) * p.heads + head) * p.head_dim;
+    bool finite = true;
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      const float v[4] = {acc[k].x * inv, acc[k].y * inv, acc[k].z * inv, acc[k].w * inv};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) finite = finite && fabsf(v[e]) <= 3.402823466e38f;
+      const int d = 4 * (warp + 8 * k);
+      if (d < p.head_dim) *reinterpret_cast<uint2*>(out + d) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+    }
+    if (!finite) redo_s[lane] = 1;
+  }
+  __syncthreads();
+  const int see_all = keys_of(j.c, min(j.c.end - j.c.begin, j.token0 + 2 * tp.tokens));
+  for (int x = warp; x < 32; x += 8) {
+    const int rx = __shfl_sync(0xFFFFFFFFu, row, x), hx = __shfl_sync(0xFFFFFFFFu, head, x);
+    if (redo_s[x] && seen_by(j.c, rx) < see_all && reached_from_behind<T>(p, j.c, rx, j.kvh, see_all))
+      attend_row<T>(p, j.c, rx, hx);
+  }
+}
+
+template <typename T, int D>
+int launch(const AttnParams& p, int64_t max_new, int sms, void* work, cudaStream_t s) {
   TcParams tp;
   tp.a = p;
   tp.tokens = kTileRows / p.group;
@@ -625,24 +912,30 @@ int launch(const AttnParams& p, int64_t max_new, int64_t max_keys, int sms, cuda
   const int64_t pair_tokens = 2 * tp.tokens, per_seq = (max_new + pair_tokens - 1) / pair_tokens;
   const int64_t fixed = p.n_seqs * per_seq, bound = p.n_rows / pair_tokens + p.n_seqs;
   const int64_t tiles = std::min(fixed, bound);
+  if (tiles * p.kv_heads > 0x3FFFFFFFll) return fail(EFG_EINVAL, "attention: too many rows");
+  tp.tiles = static_cast<int>(tiles);
   tp.tiles_per_seq = fixed <= bound ? static_cast<int>(per_seq) : 0;
-  // Split the keys while the row tiles leave half of the SMs idle and every split keeps 4 key tiles.
-  int splits = 1;
-  while (splits < 8 && tiles * p.kv_heads * splits * 2 <= sms && max_keys >= 2 * splits * 4 * kTileKeys) splits *= 2;
-  if (tiles * splits > 0x7FFFFFFFll) return fail(EFG_EINVAL, "attention: too many rows");
   const auto fn = attn_tc_kernel<T, D>;
   if (int st = ensure_smem_attr(reinterpret_cast<const void*>(fn), smem_bytes<D>())) return st;
   cudaLaunchConfig_t cf{};
-  cf.gridDim = dim3(static_cast<unsigned>(tiles * splits), static_cast<unsigned>(p.kv_heads));
+  tp.joins = static_cast<TcJoin*>(work);
+  tp.slots = work ? reinterpret_cast<float*>(tp.joins + sms) : nullptr;
+  // a CTA per run, or per item; those that run take over the others
+  cf.gridDim = dim3(static_cast<unsigned>(work ? sms : tiles * p.kv_heads));
   cf.blockDim = dim3(kThreads);
   cf.dynamicSmemBytes = smem_bytes<D>();
   cf.stream = s;
+  EFG_TRY_CUDA(cudaLaunchKernelEx(&cf, fn, tp, mq, mk, mv), "attention launch");
+  if (!work) return EFG_OK;
+  cf.gridDim = dim3(static_cast<unsigned>(sms), 8);
+  cf.blockDim = dim3(256);
+  cf.dynamicSmemBytes = 0;
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {static_cast<unsigned>(splits), 1, 1};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cf.attrs = attr;
   cf.numAttrs = 1;
-  EFG_TRY_CUDA(cudaLaunchKernelEx(&cf, fn, tp, mq, mk, mv), "attention launch");
+  EFG_TRY_CUDA(cudaLaunchKernelEx(&cf, attn_tc_join_kernel<T, D>, tp), "attention launch");
   return EFG_OK;
 }
 
@@ -658,14 +951,23 @@ bool attn_tc_takes(int type, const AttnParams& p) {
   return attn_mma_takes(type, p) && max_new * p.group > 64;
 }
 
-int launch_attn_tc(int type, const AttnParams& p, int sms, cudaStream_t s) {
+size_t attn_tc_workspace(const AttnParams& p, int sms) {
+  // Prompts bring no workspace; many items keep the GPU busy without cutting any. The line's weight is a 32-bit
+  // number.
+  if (!p.kv_len) return 0;
+  const int64_t max_new = std::min(p.max_new, p.n_rows), pair_tokens = 2 * (kTileRows / p.group);
+  const int64_t tiles = std::min(p.n_seqs * ((max_new + pair_tokens - 1) / pair_tokens), p.n_rows / pair_tokens + p.n_seqs);
+  const int64_t max_keys = p.max_pages * p.page_size;
+  if (tiles * p.kv_heads > 6 * sms || tiles * p.kv_heads > 0x7FFFFFFFll / (max_keys / kTileKeys + 1 + kItemCost)) return 0;
+  return static_cast<size_t>(sms) * (sizeof(TcJoin) + 2 * 256 * ((p.head_dim <= 64 ? 64 : 128) + 2) * sizeof(float));
+}
+
+int launch_attn_tc(int type, const AttnParams& p, int sms, void* work, cudaStream_t s) {
   const int64_t max_new = p.kv_len ? std::min(p.max_new, p.n_rows) : p.n_rows;
-  const int64_t max_keys = p.kv_len ? p.max_pages * p.page_size : p.n_rows;
   if (type == EFG_F16)
-    return p.head_dim <= 64 ? launch<__half, 64>(p, max_new, max_keys, sms, s)
-                            : launch<__half, 128>(p, max_new, max_keys, sms, s);
-  return p.head_dim <= 64 ? launch<__nv_bfloat16, 64>(p, max_new, max_keys, sms, s)
-                          : launch<__nv_bfloat16, 128>(p, max_new, max_keys, sms, s);
+    return p.head_dim <= 64 ? launch<__half, 64>(p, max_new, sms, work, s) : launch<__half, 128>(p, max_new, sms, work, s);
+  return p.head_dim <= 64 ? launch<__nv_bfloat16, 64>(p, max_new, sms, work, s)
+                          : launch<__nv_bfloat16, 128>(p, max_new, sms, work, s);
 }
 
 }  // namespace efg

@@ -7,9 +7,8 @@ operands split for the tensor cores leave out at most 2^-21 of a product, counte
 weight by twice that plus 2^-21 (exponential, running maximum, normalisation), and a sum over n weights
 by (n / 8 + 40) 2^-24 of A: no kernel adds more than n / 8 products one after the other outside the
 tensor cores, whose sums over 16 or more products are at least as good as one FP32 chain over n / 8.
-The 16-bit kernels may take the exponential from a polynomial that is off by 2.6e-6 < 2^-18, which counts
-twice (weight and normalisation), and F16 holds a weight of at most 2^-14 of the largest within 2^-25 of it,
-which over n weights is at most n 2^-25 max |v|.
+F16 holds a weight of at most 2^-14 of the largest within 2^-25 of it, which over n weights is at most
+n 2^-25 max |v|.
 """
 from __future__ import annotations
 
@@ -48,7 +47,7 @@ def tolerance(kind, out, rel, A, tiny):
     u = EPS[kind] / 2
     if kind == "f32":
         return u * np.abs(out) + A * rel
-    return u * np.abs(out) + A * (rel + u + 2.0**-17) + (2.0**-25 * (1 + tiny) if kind == "f16" else 0.0)
+    return u * np.abs(out) + A * (rel + u) + (2.0**-25 * (1 + tiny) if kind == "f16" else 0.0)
 
 
 def plan(cached, new, table, free, page_size, n_rows):
