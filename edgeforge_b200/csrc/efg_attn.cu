@@ -133,7 +133,7 @@ uint64_t efg_attn_paged_workspace(const efg_attn_paged_args* args) {
   if (!dev) return 0;
   if (std::min(max_new, n_rows) * p.group <= static_cast<size_t>(efg::kDecodeRows))
     return efg::attn_decode_workspace(args->type, p, dev->sm_count);
-  return args->type == EFG_F32 || p.group > 128 ? 0 : efg::attn_tc_workspace(p, dev->sm_count);
+  return (args->type == EFG_F32 && head_dim > 64) || p.group > 128 ? 0 : efg::attn_tc_workspace(p, dev->sm_count);
 }
 
 int efg_attn_paged(const efg_attn_paged_args* args, void* stream) {

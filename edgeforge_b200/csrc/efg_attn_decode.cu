@@ -292,12 +292,13 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
   while (walk.next(dp)) {
     const Rows& w = walk.w;
     const int kvh = walk.kvh;
-    float acc[D / 8][4];
+    constexpr int kAcc = kStack ? 2 : 4;
+    float acc[D / 8][kAcc];
     float top[kHalves], sum[kHalves];
 #pragma unroll
     for (int n = 0; n < D / 8; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+      for (int i = 0; i < kAcc; ++i) acc[n][i] = 0.f;
 #pragma unroll
     for (int i = 0; i < kHalves; ++i) top[i] = -INFINITY, sum[i] = 0.f;
     // ---- queries as A fragments
@@ -359,13 +360,13 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
         fence_proxy_async();  // before the copy that fills this stage again
         __syncwarp();
       }
-      float s[NT][4], s2[kStack ? NT : 1][4];
+      float s[NT][4], s2[kF32 ? NT : 1][4];  // (F32: the small products apart)
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           s[n][i] = 0.f;
-          if constexpr (kStack) s2[n][i] = 0.f;
+          if constexpr (kF32) s2[n][i] = 0.f;
         }
       // ---- scores
 #pragma unroll
@@ -398,8 +399,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
               } else {
                 const uint32_t ah[4] = {qh[0][2 * h], qh[1][2 * h], qh[0][2 * h + 1], qh[1][2 * h + 1]};
                 const uint32_t al[4] = {ql[0][2 * h], ql[1][2 * h], ql[0][2 * h + 1], ql[1][2 * h + 1]};
-                mma_tf32(s[n], ah, kl[2 * h], kl[2 * h + 1]);
-                mma_tf32(s[n], al, kh[2 * h], kh[2 * h + 1]);
+                mma_tf32(s2[n], ah, kl[2 * h], kl[2 * h + 1]);
+                mma_tf32(s2[n], al, kh[2 * h], kh[2 * h + 1]);
                 mma_tf32(s[n], ah, kh[2 * h], kh[2 * h + 1]);
               }
             }
@@ -420,9 +421,15 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) s[n][e] = (s[n][e] + (s[n][e + 2] + s2[n][e])) + s2[n][e + 2];
+      } else if constexpr (kF32) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
       }
       // ---- softmax (base 2)
       const bool edge = j0 + kWarpKeys > w.see_first;
+      float back[kHalves];
 #pragma unroll
       for (int i = 0; i < kHalves; ++i) {
         const int limit = sees[i] - j0;
@@ -440,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
         mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
         const float ref = mx == -INFINITY ? 0.f : mx;
-        const float back = ex2(top[i] - ref);
+        back[i] = ex2(top[i] - ref);
         const bool moved = mx != top[i];
         top[i] = mx;
         float add = 0.f;
@@ -452,36 +459,38 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
             x = ex2(x - ref);
             add += x;
           }
-        sum[i] = sum[i] * back + add;
-        if (__any_sync(0xFFFFFFFFu, moved)) {
+        sum[i] = sum[i] * back[i] + add;
+        if (!kF32 && __any_sync(0xFFFFFFFFu, moved)) {
 #pragma unroll
           for (int n = 0; n < D / 8; ++n) {
-            acc[n][2 * i] *= back;
-            acc[n][2 * i + 1] *= back;
-            if constexpr (kStack) {
-              acc[n][2] *= back;
-              acc[n][3] *= back;
-            }
+            acc[n][2 * i] *= back[i];
+            acc[n][2 * i + 1] *= back[i];
           }
         }
       }
       // ---- weighted values
       if constexpr (kF32) {
+        // The products of one tile are summed from zero and added to the running sums by FP32 additions: the matrix
+        // instructions cut off instead of rounding, which over a long row would shrink it.
+        uint32_t ph[NT][4], pl[NT][4];  // A fragments: k = t is key t, k = t + 4 key t + 4 of the eight
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          uint32_t ph[4], pl[4];  // A fragment: k = t is key t, k = t + 4 key t + 4 of the eight
           if constexpr (kStack) {
-            split_tf32(s[n][0], ph[0], ph[1]);
-            split_tf32(s[n][1], ph[2], ph[3]);
+            split_tf32(s[n][0], ph[n][0], ph[n][1]);
+            split_tf32(s[n][1], ph[n][2], ph[n][3]);
           } else {
-            split_tf32(s[n][0], ph[0], pl[0]);
-            split_tf32(s[n][2], ph[1], pl[1]);
-            split_tf32(s[n][1], ph[2], pl[2]);
-            split_tf32(s[n][3], ph[3], pl[3]);
+            split_tf32(s[n][0], ph[n][0], pl[n][0]);
+            split_tf32(s[n][2], ph[n][1], pl[n][1]);
+            split_tf32(s[n][1], ph[n][2], pl[n][2]);
+            split_tf32(s[n][3], ph[n][3], pl[n][3]);
           }
-          const int r = key0 + 8 * n + t;  // and r + 4
+        }
 #pragma unroll
-          for (int dc = 0; dc < D / 32; ++dc) {  // column g of group (dc, i) is dim 32 dc + 4 perm + i
+        for (int dc = 0; dc < D / 32; ++dc) {  // column g of group (dc, i) is dim 32 dc + 4 perm + i
+          float big[4][4] = {}, small[4][4] = {};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const int r = key0 + 8 * n + t;  // and r + 4
             const uint32_t panel = vs + dc * S::kPanelBytes;
             const float4 v0 = lds128(panel + r * 128 + ((perm ^ (r & 7)) << 4));
             const float4 v1 = lds128(panel + (r + 4) * 128 + ((perm ^ ((r + 4) & 7)) << 4));
@@ -491,11 +500,21 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
               uint32_t h0, l0, h1, l1;
               split_tf32(a0[i], h0, l0);
               split_tf32(a1[i], h1, l1);
-              mma_tf32(acc[4 * dc + i], ph, l0, l1);
-              if constexpr (!kStack) mma_tf32(acc[4 * dc + i], pl, h0, h1);
-              mma_tf32(acc[4 * dc + i], ph, h0, h1);
+              mma_tf32(small[i], ph[n], l0, l1);
+              if constexpr (!kStack) mma_tf32(small[i], pl[n], h0, h1);
+              mma_tf32(big[i], ph[n], h0, h1);
             }
           }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < kAcc; ++e) {
+              float& o = acc[4 * dc + i][e];
+              if constexpr (kStack)
+                o = fmaf(o, back[0], big[i][e] + (big[i][e + 2] + (small[i][e] + small[i][e + 2])));
+              else
+                o = fmaf(o, back[e >> 1], big[i][e] + small[i][e]);
+            }
         }
       } else {
 #pragma unroll
@@ -527,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
         sum_s[warp][g + 8 * i] = v;
       }
       float* o = o_s + (warp * kSlabRows + g + 8 * i) * D;
-      const auto value = [&](int n, int e) { return kStack ? acc[n][e] + acc[n][e + 2] : acc[n][2 * i + e]; };
+      const auto value = [&](int n, int e) { return acc[n][2 * i + e]; };
       if constexpr (kF32) {  // dims 32 dc + 4 t + 16 e ..  + 3
 #pragma unroll
         for (int n = 0; n < D / 8; n += 4)

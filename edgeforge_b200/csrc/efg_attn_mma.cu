@@ -193,11 +193,14 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
 
     const uint32_t ks = base + static_cast<uint32_t>(buf) * (2 * kTile), vs = ks + kTile;
     const int key0 = MT == 1 ? warp * 16 : 0;
-    float s[NT][4];
+    float s[NT][4], s2[kF32 ? NT : 1][4];  // (F32: the small products apart)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
+      for (int i = 0; i < 4; ++i) {
+        s[n][i] = 0.f;
+        if constexpr (kF32) s2[n][i] = 0.f;
+      }
     // ---- scores
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
@@ -223,8 +226,8 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
           for (int h = 0; h < 2; ++h) {
             const uint32_t ah[4] = {qh[0][2 * h], qh[1][2 * h], qh[0][2 * h + 1], qh[1][2 * h + 1]};
             const uint32_t al[4] = {ql[0][2 * h], ql[1][2 * h], ql[0][2 * h + 1], ql[1][2 * h + 1]};
-            mma_tf32(s[n], ah, kl[2 * h], kl[2 * h + 1]);
-            mma_tf32(s[n], al, kh[2 * h], kh[2 * h + 1]);
+            mma_tf32(s2[n], ah, kl[2 * h], kl[2 * h + 1]);
+            mma_tf32(s2[n], al, kh[2 * h], kh[2 * h + 1]);
             mma_tf32(s[n], ah, kh[2 * h], kh[2 * h + 1]);
           }
         }
@@ -239,7 +242,14 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
         }
       }
     }
+    if constexpr (kF32) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
+    }
     // ---- softmax of this tile (base 2), rows g and g + 8
+    float back[2];
     const int j0 = tile * kKeys + key0;
     const bool edge = j0 + 8 * NT > see_first;  // some row does not see all of these keys
 #pragma unroll
@@ -258,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
       const float ref = mx == -INFINITY ? 0.f : mx;  // nothing seen yet: all weights 0
-      const float back = ex2(top[i] - ref);
+      back[i] = ex2(top[i] - ref);
       top[i] = mx;
       float add = 0.f;
 #pragma unroll
@@ -269,25 +279,30 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
           x = ex2(x - ref);
           add += x;
         }
-      sum[i] = sum[i] * back + add;
+      sum[i] = sum[i] * back[i] + add;
+      if constexpr (!kF32) {
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n) {
-        acc[n][2 * i] *= back;
-        acc[n][2 * i + 1] *= back;
+        for (int n = 0; n < D / 8; ++n) {
+          acc[n][2 * i] *= back[i];
+          acc[n][2 * i + 1] *= back[i];
+        }
       }
     }
     // ---- weighted values
     if constexpr (kF32) {
+      // The products of one tile are summed from zero and added to the running sums by FP32 additions: the matrix
+      // instructions cut off instead of rounding, which over a long row would shrink it (by 1.3e-5 at 8192 keys).
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        uint32_t ph[4], pl[4];  // A fragment: k = t is key 2t, k = t + 4 key 2t + 1
-        split_tf32(s[n][0], ph[0], pl[0]);
-        split_tf32(s[n][2], ph[1], pl[1]);
-        split_tf32(s[n][1], ph[2], pl[2]);
-        split_tf32(s[n][3], ph[3], pl[3]);
-        const int r = key0 + 8 * n + 2 * t;
+      for (int dc = 0; dc < D / 32; ++dc) {  // column g of group (dc, i) is dim 32 dc + 4 g + i
+        float big[4][4] = {}, small[4][4] = {};
 #pragma unroll
-        for (int dc = 0; dc < D / 32; ++dc) {  // column g of group (dc, i) is dim 32 dc + 4 g + i
+        for (int n = 0; n < NT; ++n) {
+          uint32_t ph[4], pl[4];  // A fragment: k = t is key 2t, k = t + 4 key 2t + 1
+          split_tf32(s[n][0], ph[0], pl[0]);
+          split_tf32(s[n][2], ph[1], pl[1]);
+          split_tf32(s[n][1], ph[2], pl[2]);
+          split_tf32(s[n][3], ph[3], pl[3]);
+          const int r = key0 + 8 * n + 2 * t;
           const float4 v0 = lds128(vs + r * kRowBytes + value_chunk<T>(r, 8 * dc + g) * 16);
           const float4 v1 = lds128(vs + (r + 1) * kRowBytes + value_chunk<T>(r + 1, 8 * dc + g) * 16);
           const float a0[4] = {v0.x, v0.y, v0.z, v0.w}, a1[4] = {v1.x, v1.y, v1.z, v1.w};
@@ -296,11 +311,15 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
             uint32_t h0, l0, h1, l1;
             split_tf32(a0[i], h0, l0);
             split_tf32(a1[i], h1, l1);
-            mma_tf32(acc[4 * dc + i], ph, l0, l1);
-            mma_tf32(acc[4 * dc + i], pl, h0, h1);
-            mma_tf32(acc[4 * dc + i], ph, h0, h1);
+            mma_tf32(small[i], ph, l0, l1);
+            mma_tf32(small[i], pl, h0, h1);
+            mma_tf32(big[i], ph, h0, h1);
           }
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[4 * dc + i][e] = fmaf(acc[4 * dc + i][e], back[e >> 1], big[i][e] + small[i][e]);
       }
     } else {
 #pragma unroll

@@ -40,18 +40,28 @@
 namespace efg {
 namespace {
 
-constexpr int kThreads = 384, kTileKeys = 128, kTileRows = 128;
+constexpr int kTileKeys = 128, kTileRows = 128;
+template <typename T>
+constexpr bool is_f32 = std::is_same_v<T, float>;
+template <typename T>
+constexpr int threads = is_f32<T> ? 512 : 384;
 constexpr uint32_t kPanel = 128 * 128;  // 128 rows of 64 16-bit values, 128-byte swizzled
-constexpr float kLazy = 8.f;            // powers of two that the maximum may grow before O is rescaled
+// Powers of two that the maximum may grow before O is rescaled; F32 weights are held 2^12 higher, so that both
+// their F16 parts stay in range and small ones keep their digits.
+template <typename T>
+constexpr float kLazy = is_f32<T> ? 3.f : 8.f;
+constexpr int kRaise = 12;
 
-template <int D>
-constexpr int kv_stages() {
-  return D == 64 ? 8 : 5;
-}
-template <int D>
-constexpr size_t smem_bytes() {
-  return 1024 + static_cast<size_t>(2 + kv_stages<D>()) * (D / 64) * kPanel;
-}
+// Panels of an operand tile (a row of 64 16-bit values each): the head's dims, or the hi and the lo part of 64 FP32
+// dims; operand stages, and stages of FP32 tiles on their way to the converters.
+template <typename T, int D>
+constexpr int panels = is_f32<T> ? 2 : D / 64;
+template <typename T, int D>
+constexpr int kv_stages = is_f32<T> ? 3 : D == 64 ? 8 : 5;
+template <typename T>
+constexpr int staging = is_f32<T> ? 2 : 0;
+template <typename T, int D>
+constexpr size_t smem_bytes = 1024 + static_cast<size_t>(2 + kv_stages<T, D> + staging<T>) * panels<T, D> * kPanel;
 
 // A value tile as the B operand of O += P V: keys run along K, so the tile (rows of keys, 64 dims of 128
 // bytes, 128-byte swizzle) is MN-major: 64-dim panels kPanel apart, groups of 8 keys 1024 bytes apart.
@@ -63,7 +73,7 @@ __device__ __forceinline__ uint64_t desc_values(uint32_t saddr) {
 // Instruction descriptor: FP32 accumulator, A and B F16 or BF16, A K-major, B K-major or MN-major.
 template <typename T>
 constexpr uint32_t idesc_of(uint32_t N, bool b_mn) {
-  const uint32_t fmt = std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;
+  const uint32_t fmt = std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;  // (F32: two F16 parts)
   return (1u << 4) | (fmt << 7) | (fmt << 10) | ((b_mn ? 1u : 0u) << 16) | ((N >> 3) << 17) | ((kTileRows >> 4) << 24);
 }
 
@@ -154,7 +164,68 @@ __device__ __forceinline__ void weights32(const uint32_t* s, uint64_t scale, uin
   }
 }
 
+// The same for F32: each weight as the sum of two F16 values.
+__device__ __forceinline__ void weights32_split(const uint32_t* s, uint64_t scale, uint64_t nref, uint64_t (&total)[2],
+                                                uint32_t (&hi)[16], uint32_t (&lo)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float a, b;
+    unpair(fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale, nref), a, b);
+    // (raised by a product, not in the exponent: next to 0 that keeps more of its digits)
+    constexpr float kUp = static_cast<float>(1 << kRaise);
+    const uint64_t w = fma2(pair(ex2(a), ex2(b)), pair(kUp, kUp), 0);
+    total[i % 2] = add2(total[i % 2], w);
+    unpair(w, a, b);
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 back = __half22float2(h);
+    hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+    lo[i] = pack2<__half>(a - back.x, b - back.y);
+  }
+}
+
+// Eight FP32 values times a power of two, as F16 hi and lo parts: x = hi + lo within 2^-22 |x| (or 2^-25
+// of the scaled unit).
+__device__ __forceinline__ void split8(const float4& x, const float4& y, float scale, uint4& hi, uint4& lo) {
+  const float v[8] = {x.x * scale, x.y * scale, x.z * scale, x.w * scale, y.x * scale, y.y * scale, y.z * scale, y.w * scale};
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 t = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    const float2 back = __half22float2(t);
+    h[i] = *reinterpret_cast<const uint32_t*>(&t);
+    l[i] = pack2<__half>(v[2 * i] - back.x, v[2 * i + 1] - back.y);
+  }
+  hi = make_uint4(h[0], h[1], h[2], h[3]);
+  lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+// Largest finite magnitude of a quad and what came before.
+__device__ __forceinline__ float finite_max(float m, const float4& v) {
+  const float a[4] = {fabsf(v.x), fabsf(v.y), fabsf(v.z), fabsf(v.w)};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = a[i] <= 3.402823466e38f ? fmaxf(m, a[i]) : m;
+  return m;
+}
+// Exponent of the largest magnitude (held at -100 and above), and 2^e.
+__device__ __forceinline__ int exponent_of(float m) { return max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -100); }
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+constexpr int kTop = 14;  // split operands are scaled so that their largest value is below 2^(kTop + 1)
+
+// Whether `ok` holds for all 128 converter threads; a barrier among them.
+__device__ __forceinline__ bool all_converters(bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, 2, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(ok ? 1u : 0u)
+      : "memory");
+  return r != 0;
+}
+
 // All threads of the CTA, from inside their roles.
+template <int kThreads>
 __device__ __forceinline__ void cta_barrier() {
   __syncwarp();
   asm volatile("bar.sync 0, %0;" ::"n"(kThreads) : "memory");
@@ -191,6 +262,24 @@ struct alignas(16) TcJoin {
   Chunk c;
   int32_t kvh, token0, first, parts;  // parts 0: nothing begins here that is cut
 };
+
+// 32 columns of O; F32: the products with V hi plus those with V lo, 64 columns on.
+template <bool kF32>
+__device__ __forceinline__ void load_o(uint32_t addr, uint32_t (&o)[32]) {
+  tmem_ld32(addr, o);
+  if constexpr (kF32) {
+    uint32_t lo[32];
+    tmem_ld32(addr + 64, lo);
+    tmem_wait_ld();
+    after_wait(o);
+    after_wait(lo);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) + __uint_as_float(lo[e]));
+  } else {
+    tmem_wait_ld();
+    after_wait(o);
+  }
+}
 
 struct TcParams {
   AttnParams a;
@@ -246,16 +335,24 @@ __device__ __forceinline__ int weight_of(const AttnParams& p, int64_t seq, int p
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(threads<T>, 1)
     attn_tc_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ CUtensorMap map_q,
                    const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
-  constexpr int kPanels = D / 64, kStages = kv_stages<D>();
-  constexpr bool kApart = D == 64;  // P beside S in TMEM: the next S does not wait for the value product
+  constexpr bool kF32 = is_f32<T>;
+  using E = std::conditional_t<kF32, __half, T>;  // of the MMA operands
+  constexpr int kThreads = threads<T>, kPanels = panels<T, D>, kStages = kv_stages<T, D>, kStaging = kF32 ? 2 : 1;
+  // P beside S in TMEM: the next S does not wait for the value product
+  constexpr bool kApart = !kF32 && D == 64;
   constexpr uint32_t kTileBytes = kPanels * kPanel;
-  constexpr uint32_t kColO = 256, kColP = kApart ? 384 : 0, kStepP = kApart ? 64 : 128;
+  // columns of O per row tile (F32: products with V hi, then with V lo), where P lies
+  constexpr uint32_t kColO = 256, kWideO = kF32 ? 128 : D, kColP = kApart ? 384 : 0, kStepP = kApart ? 64 : 128;
+  static_assert(!kF32 || D == 64);
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t q_full, q_empty, kv_full[kStages], kv_empty[kStages], s_full[2], s_free[2], p_ready[2], pv_done[2],
       drained[2], item_full[2], item_empty[2], fetch, asked;
+  __shared__ uint64_t stage_full[kStaging], stage_empty[kStaging], exp_full[8];
+  __shared__ int exp_s[8];  // exponents of the split tiles, by ring item
+  __shared__ float max_s[2][4];
   __shared__ uint4 answer;
   __shared__ int scan_s[kThreads / 32], run_s[5];
   __shared__ Item items[2];
@@ -265,13 +362,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t raw = smem_addr(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* q_s = smem_raw + (base - raw);
   uint8_t* ring = q_s + 2 * kTileBytes;
+  uint8_t* stage = ring + kStages * kTileBytes;
   if (tid == 0) {
-    mbar_init(&q_full, 1);
+    mbar_init(&q_full, kF32 ? 256 : 1);
     mbar_init(&q_empty, kApart ? 2 : 1);
     mbar_init(&fetch, 1);
     mbar_init(&asked, 1);
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_full[i], kF32 ? 128 : 1);
       mbar_init(&kv_empty[i], kApart ? 2 : 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -280,9 +378,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&p_ready[i], 128);
       mbar_init(&pv_done[i], 1);
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], kApart ? 11 : 10);  // 8 softmax warps (when they are done with it), TMA, MMA
+      // 8 softmax warps (when they are done with it), TMA, MMA, converters
+      mbar_init(&item_empty[i], kApart ? 11 : kF32 ? 14 : 10);
       mbar_init(&drained[i], 1);
     }
+    for (int i = 0; i < kStaging; ++i) {
+      mbar_init(&stage_full[i], 1);
+      mbar_init(&stage_empty[i], 128);
+    }
+    for (int i = 0; i < 8; ++i) mbar_init(&exp_full[i], 1);
     fence_barrier_init();
   }
   if (warp == 9) tmem_alloc(&tmem_slot, 512);
@@ -349,6 +453,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       // -------------------------------------------------------------- TMA
       const int boxes = kTileKeys / tp.box_rows, b = lane % boxes, panel = lane / boxes;
       const bool mine = lane < boxes * kPanels;
+      constexpr int kIn = kF32 ? kStaging : kStages;
+      uint64_t *in_full = kF32 ? stage_full : kv_full, *in_empty = kF32 ? stage_empty : kv_empty;
+      uint8_t* in = kF32 ? stage : ring;
       Item w;
       bool ok = true;
       int issued = 0, tiles = 0;
@@ -358,11 +465,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) mbar_arrive(&fetch);
           continue;
         }
-        if (tiles > 0) ok = wait_own(&q_empty, (tiles - 1) & 1, p.err);
+        if (!kF32 && tiles > 0) ok = wait_own(&q_empty, (tiles - 1) & 1, p.err);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;
         ++tiles;
-        if (lane == 0) {
+        if (!kF32 && lane == 0) {  // (F32 queries: the softmax warps)
           const int live = a.n[1] > 0 ? 2 : 1;
           mbar_arrive_expect_tx(&q_full, static_cast<uint32_t>(live * kPanels * tp.tokens * p.group) * 128u);
           for (int i = 0; i < live; ++i)
@@ -383,23 +490,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int32_t next = row_of(w.first + j + 1);
           if (j == max(0, w.count - 2) && lane == 0) mbar_arrive(&fetch);  // time to look for the next item
           for (int kv = 0; kv < 2 && ok; ++kv) {
-            const int st = issued % kStages;
-            if (issued >= kStages) ok = wait_own(&kv_empty[st], ((issued / kStages) - 1) & 1, p.err);
+            const int st = issued % kIn;
+            if (issued >= kIn) ok = wait_own(&in_empty[st], ((issued / kIn) - 1) & 1, p.err);
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) break;
-            if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], kTileBytes);
+            if (lane == 0) mbar_arrive_expect_tx(&in_full[st], kTileBytes);
             __syncwarp();
             if (mine)
-              tma_load_3d(ring + st * kTileBytes + panel * kPanel + b * tp.box_rows * 128, kv ? &map_v : &map_k,
-                          64 * panel, w.kvh, row, &kv_full[st]);
+              tma_load_3d(in + st * kTileBytes + panel * kPanel + b * tp.box_rows * 128, kv ? &map_v : &map_k,
+                          (128 / static_cast<int>(sizeof(T))) * panel, w.kvh, row, &in_full[st]);
             ++issued;
           }
           row = next;
         }
       }
       // the copies in flight land before the shared memory is given back (all have, unless a wait gave up)
-      if (tiles > 0) wait_own(&q_full, (tiles - 1) & 1, p.err);
-      for (int i = max(0, issued - kStages); i < issued; ++i) wait_own(&kv_full[i % kStages], (i / kStages) & 1, p.err);
+      if (!kF32 && tiles > 0) wait_own(&q_full, (tiles - 1) & 1, p.err);
+      for (int i = max(0, issued - kIn); i < issued; ++i) wait_own(&in_full[i % kIn], (i / kIn) & 1, p.err);
     } else if (warp == 9 || (kApart && warp == 11)) {
       // -------------------------------------------------------------- MMA
       // Where P lies apart, each row tile has a warp of its own (9 and 11): a softmax that is ready is never
@@ -408,7 +515,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       // cores idle during both softmaxes. Each whole warp walks this code, so that addresses and
       // descriptors stay warp-uniform (in uniform registers); one elected thread issues. All 512 columns
       // are this CTA's: TMEM addresses start at 0.
-      constexpr uint32_t id_s = idesc_of<T>(kTileKeys, false), id_o = idesc_of<T>(D, true);
+      constexpr uint32_t id_s = idesc_of<E>(kTileKeys, false), id_o = idesc_of<E>(kWideO, true);
+      constexpr uint32_t id_half = idesc_of<E>(64, true);
       constexpr int kMine = kApart ? 1 : 2;  // row tiles of this warp: from `mine` on
       const int mine = kApart && warp == 11 ? 1 : 0;
       const uint32_t one = elect_one();
@@ -416,10 +524,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto scores = [&](int i, int item) {
         const uint64_t dq = smem_desc_sw128(base + i * kTileBytes);
         const uint64_t dk = smem_desc_sw128(ring_addr + (item % kStages) * kTileBytes);
+        if constexpr (kF32) {  // hi lo and lo hi first: the accumulator cuts off digits at each step, of small sums less
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            if (ks == 0)
+              mma_ss<false>(one, 128 * i, dq, dk + (kPanel >> 4), id_s);
+            else
+              mma_ss<true>(one, 128 * i, dq + 2 * ks, dk + (kPanel >> 4) + 2 * ks, id_s);
+            mma_ss<true>(one, 128 * i, dq + (kPanel >> 4) + 2 * ks, dk + 2 * ks, id_s);
+          }
+        }
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
           const uint64_t adv = (ks / 4) * (kPanel >> 4) + (ks % 4) * 2;
-          if (ks == 0)
+          if (ks == 0 && !kF32)
             mma_ss<false>(one, 128 * i, dq + adv, dk + adv, id_s);
           else
             mma_ss<true>(one, 128 * i, dq + adv, dk + adv, id_s);
@@ -428,10 +546,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       auto values = [&](int i, int item, uint32_t add) {
         const uint64_t dv = desc_values(ring_addr + (item % kStages) * kTileBytes);
-        const uint32_t o = kColO + D * i, pp = kColP + kStepP * i;
-        mma_ts(one, o, pp, dv, id_o, add);
+        const uint32_t o = kColO + kWideO * i, pp = kColP + kStepP * i;
+        // F32: P hi times [V hi | V lo], then P lo times V hi onto the columns of the small products; of each half of
+        // the keys P hi lies in 32 columns and P lo in the next 32
+        const auto col = [&](int ks) { return pp + (kF32 ? (ks / 4) * 64 + (ks % 4) * 8 : 8 * ks); };
+        mma_ts(one, o, pp, dv, id_o, kF32 ? 0u : add);
 #pragma unroll
-        for (int ks = 1; ks < kTileKeys / 16; ++ks) mma_ts(one, o, pp + 8 * ks, dv + ks * (2048 >> 4), id_o, 1u);
+        for (int ks = 1; ks < kTileKeys / 16; ++ks) mma_ts(one, o, col(ks), dv + ks * (2048 >> 4), id_o, 1u);
+        if constexpr (kF32) {
+#pragma unroll
+          for (int ks = 0; ks < kTileKeys / 16; ++ks) mma_ts(one, o + 64, col(ks) + 32, dv + ks * (2048 >> 4), id_half, 1u);
+        }
         commit_if(one, &pv_done[i]);
       };
       // The tile has landed. (A stage is given back only after that, also by a row tile that has no use for it:
@@ -500,6 +625,56 @@ __global__ void __launch_bounds__(kThreads, 1)
       commit_if(one, &drained[mine]);  // no MMA runs on when the TMEM is given back, also after a wait gave up
       __syncwarp();
       mbar_drain(&drained[mine], 0, p.err);
+    } else if (kF32 && warp >= 12) {
+      // -------------------------------------------------------------- converters
+      // An FP32 tile (128 rows of 64 dims, two swizzled panels) becomes the hi and lo panels of an operand tile,
+      // scaled by a power of two after its largest magnitude; a thread per row. Rows behind the last
+      // position become zeros, whatever lies there.
+      const int r = tid - 384;
+      Item w;
+      bool ok = true;
+      int at = 0;
+      while (ok && next_item(w)) {
+        const Plan a = plan_of(w, tp.tokens);
+        for (int x = 0; x < 2 * w.count && ok; ++x, ++at) {
+          const int st = at % kStaging, op = at % kStages;
+          const bool valid = (w.first + (x >> 1)) * kTileKeys + r < a.see_all;
+          ok = wait_own(&stage_full[st], (at / kStaging) & 1, p.err);
+          if (ok && at >= kStages) ok = wait_own(&kv_empty[op], ((at / kStages) - 1) & 1, p.err);
+          const uint8_t* src = stage + st * kTileBytes + r * 128;
+          auto chunk = [&](int c) {
+            return *reinterpret_cast<const float4*>(src + (c >> 3) * kPanel + (((c & 7) ^ (r & 7)) << 4));
+          };
+          float m = 0.f;
+          if (valid) {
+#pragma unroll
+            for (int c = 0; c < 16; ++c) m = finite_max(m, chunk(c));
+          }
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+          if (lane == 0) max_s[at & 1][warp - 12] = m;
+          ok = all_converters(ok);  // also orders max_s
+          if (!ok) break;
+          const float* ms = max_s[at & 1];
+          const int e = exponent_of(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])));
+          const float scale = power_of_two(kTop - e);
+          uint8_t* dst = ring + op * kTileBytes + r * 128;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+            if (valid) split8(chunk(2 * c), chunk(2 * c + 1), scale, hi, lo);
+            *reinterpret_cast<uint4*>(dst + ((c ^ (r & 7)) << 4)) = hi;
+            *reinterpret_cast<uint4*>(dst + kPanel + ((c ^ (r & 7)) << 4)) = lo;
+          }
+          if (r == 0) {
+            exp_s[at & 7] = e;
+            mbar_arrive(&exp_full[at & 7]);
+          }
+          fence_proxy_async();
+          mbar_arrive(&kv_full[op]);
+          mbar_arrive(&stage_empty[st]);
+        }
+      }
     } else if (warp == 10) {
       // -------------------------------------------------------------- scheduler
       // Items are numbered key head by key head, the pairs of row tiles of a sequence last to first (the last see
@@ -627,16 +802,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ---------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    if constexpr (kF32)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    else
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int i = warp >> 2, r = tid & 127;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-    const uint32_t s_addr = tmem + lanes + 128 * i, o_addr = tmem + lanes + kColO + D * i;
+    const uint32_t s_addr = tmem + lanes + 128 * i, o_addr = tmem + lanes + kColO + kWideO * i;
     const uint32_t p_addr = tmem + lanes + kColP + kStepP * i;
     const int token = r / p.group;  // of the row tile
     const float scale2 = p.scale * 1.4426950408889634f;
-    const uint64_t scale_pair = pair(scale2, scale2);
     bool ok = true;
     int ring_at = 0, step = 0;  // ring items, and key tiles of this row tile, before this item
+    int tiles = 0;              // items with keys before this one
     for (;; ++turn) {
       const int slot = turn & 1;
       // (read again where needed: the registers are for S)
@@ -656,102 +834,218 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       uint64_t total[2] = {0, 0};  // pairs of FP32 zeros
       float ref = 0.f;
-      for (int j = 0; j < n; ++j, ++step) {
-        ok = wait_own(&s_full[i], step & 1, p.err);
-        if (!__all_sync(0xFFFFFFFFu, ok)) break;
-        tc_fence_after();
-        uint32_t s[128];
-        const int key0 = (first + j) * kTileKeys;
-        const bool edge = key0 + kTileKeys > see_first;
-        const int limit = sees - key0;
+      int exp_q = 0;                // F32: exponent of this row's query
+      float acc[kF32 ? D : 1] = {};  // F32: O of the key tiles before
+      if (kF32 && count > 0) {
+        // this row's query, scaled by a power of two, as the hi and lo rows of the Q operand
+        if (tiles > 0) ok = ok && wait_own(&q_empty, (tiles - 1) & 1, p.err);
+        const int64_t row = items[slot].c.begin + items[slot].token0 + i * tp.tokens + token;
+        const int head = items[slot].kvh * p.group + r - token * p.group;
+        const bool live = token < plan_of(items[slot], tp.tokens).tok[i];
+        const float* q = static_cast<const float*>(p.q) + row * p.q_stride + static_cast<int64_t>(head) * p.head_dim;
+        float4 v[16];
+        float m = 0.f;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) tmem_ld32(s_addr + 32 * q, s + 32 * q);
-        tmem_wait_ld();
-#pragma unroll
-        for (int q = 0; q < 4; ++q) after_wait(s + 32 * q);
-        if (kApart) {
-          tc_fence_before();
-          mbar_arrive(&s_free[i]);
+        for (int c = 0; c < 16; ++c) {
+          v[c] = live && 4 * c < p.head_dim ? *reinterpret_cast<const float4*>(q + 4 * c) : make_float4(0, 0, 0, 0);
+          m = finite_max(m, v[c]);
         }
-        if (edge) {
+        exp_q = exponent_of(m);
+        uint8_t* dst = q_s + i * kTileBytes + r * 128;
 #pragma unroll
-          for (int k = 0; k < 128; ++k)
-            if (k >= limit) s[k] = 0xFF800000u;  // -inf
+        for (int c = 0; c < 8; ++c) {
+          uint4 hi, lo;
+          split8(v[2 * c], v[2 * c + 1], power_of_two(kTop - exp_q), hi, lo);
+          *reinterpret_cast<uint4*>(dst + ((c ^ (r & 7)) << 4)) = hi;
+          *reinterpret_cast<uint4*>(dst + kPanel + ((c ^ (r & 7)) << 4)) = lo;
         }
-        float mx[4];
+        fence_proxy_async();
+        mbar_arrive(&q_full);
+      }
+      tiles += count > 0;
+      if constexpr (kF32) {
+        // O of one key tile at a time is added up here, in registers: the tensor cores' accumulators cut off instead
+        // of rounding, which over a long row would shrink it (by 5e-6 at 8192 keys). S is read by halves
+        // to leave room for that.
+        float unit = 0.f;  // of O of the key tile before
+        const auto take = [&](float back) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) mx[q] = fmaxf(__uint_as_float(s[q]), __uint_as_float(s[q + 4]));
+          for (int q = 0; q < D / 32; ++q) {
+            uint32_t o[32];
+            load_o<true>(o_addr + 32 * q, o);
 #pragma unroll
-        for (int k = 8; k < 128; k += 8)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) mx[q] = max3(mx[q], __uint_as_float(s[k + q]), __uint_as_float(s[k + q + 4]));
-        const float high = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
-        // P and O of the key tile before are free once its value product is done
-        const auto before_done = [&] {
-          if (j > 0) ok = wait_own(&pv_done[i], (step - 1) & 1, p.err);
-          tc_fence_after();
+            for (int e = 0; e < 32; ++e) acc[32 * q + e] = fmaf(__uint_as_float(o[e]), unit, acc[32 * q + e]) * back;
+          }
         };
-        if (j == 0) {
-          ref = high == -INFINITY ? 0.f : high;
-        } else {
-          const bool move = high - ref > kLazy;
-          if (__any_sync(0xFFFFFFFFu, move)) {
-            before_done();
+        for (int j = 0; j < n; ++j, ++step) {
+          ok = ok && wait_own(&s_full[i], step & 1, p.err);
+          if (!__all_sync(0xFFFFFFFFu, ok)) break;
+          tc_fence_after();
+          const int key0 = (first + j) * kTileKeys;
+          const bool edge = key0 + kTileKeys > see_first;
+          const int limit = sees - key0;
+          uint32_t s[64];
+          const auto load = [&](int h) {
+            tmem_ld32(s_addr + 64 * h, s);
+            tmem_ld32(s_addr + 64 * h + 32, s + 32);
+            tmem_wait_ld();
+            after_wait(s);
+            after_wait(s + 32);
+            if (edge) {
+#pragma unroll
+              for (int k = 0; k < 64; ++k)
+                if (k + 64 * h >= limit) s[k] = 0xFF800000u;  // -inf
+            }
+          };
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            load(h);
+#pragma unroll
+            for (int k = 0; k < 64; k += 8)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) mx[q] = max3(mx[q], __uint_as_float(s[k + q]), __uint_as_float(s[k + q + 4]));
+          }
+          const int ki = ring_at + 2 * j, vi = ki + 1;
+          ok = wait_own(&exp_full[ki & 7], (ki >> 3) & 1, p.err) && wait_own(&exp_full[vi & 7], (vi >> 3) & 1, p.err);
+          const float factor = scale2 * power_of_two(max(-120, min(120, exp_q + exp_s[ki & 7] - 2 * kTop)));
+          const float high = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * factor;
+          if (j == 0) {
+            ref = high == -INFINITY ? 0.f : high;
+          } else {
+            const bool move = high - ref > kLazy<T>;
             const float back = move ? ex2(ref - high) : 1.f;
             if (move) ref = high;
             total[0] = fma2(total[0], pair(back, back), 0);
             total[1] = fma2(total[1], pair(back, back), 0);
-#pragma unroll 1
-            for (int q = 0; q < D / 32; ++q) {
-              uint32_t o[32];
-              tmem_ld32(o_addr + 32 * q, o);
-              tmem_wait_ld();
-              after_wait(o);
-              uint32_t lo[16], hi[16];
+            ok = ok && wait_own(&pv_done[i], (step - 1) & 1, p.err);
+            if (!__all_sync(0xFFFFFFFFu, ok)) break;
+            tc_fence_after();
+            take(back);
+          }
+          unit = power_of_two(max(-126, exp_s[vi & 7] - kTop - kRaise));
+          const uint64_t scale_pair = pair(factor, factor), nref = pair(-ref, -ref);
 #pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                lo[e] = __float_as_uint(__uint_as_float(o[e]) * back);
-                hi[e] = __float_as_uint(__uint_as_float(o[e + 16]) * back);
-              }
-              tmem_st16(o_addr + 32 * q, lo);
-              tmem_st16(o_addr + 32 * q + 16, hi);
+          for (int h = 1; h >= 0; --h) {  // the second half is still there
+            if (h == 0) load(0);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              uint32_t hi[16], lo[16];
+              weights32_split(s + 32 * q, scale_pair, nref, total, hi, lo);
+              tmem_st16(p_addr + 64 * h + 16 * q, hi);
+              tmem_st16(p_addr + 64 * h + 32 + 16 * q, lo);
             }
           }
-        }
-        const uint64_t nref = pair(-ref, -ref);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t x[16];
-          weights32<T>(s + 32 * q, scale_pair, nref, total, x);
-          if (q == 0) before_done();
-          tmem_st16(p_addr + 16 * q, x);
-        }
-        if (!__all_sync(0xFFFFFFFFu, ok)) break;
-        if (key0 + kTileKeys > see_all) {
-          // values behind the last position: whatever lies there would meet weights of zero, and 0 times
-          // infinity is NaN, so it becomes zero
-          const int item = ring_at + 2 * j + 1, st = item % kStages;
-          ok = wait_own(&kv_full[st], (item / kStages) & 1, p.err);
-          if (ok && key0 + r >= see_all) {
-#pragma unroll
-            for (int h = 0; h < kPanels; ++h) {
-              uint4* row = reinterpret_cast<uint4*>(ring + st * kTileBytes + h * kPanel + r * 128);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) row[e] = make_uint4(0, 0, 0, 0);
-            }
-          }
-          fence_proxy_async();
           if (!__all_sync(0xFFFFFFFFu, ok)) break;
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&p_ready[i]);
         }
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&p_ready[i]);
+        if (n > 0) {
+          ok = ok && wait_own(&pv_done[i], (step - 1) & 1, p.err);
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          tc_fence_after();
+          take(1.f);
+        }
+      } else {
+        for (int j = 0; j < n; ++j, ++step) {
+          ok = wait_own(&s_full[i], step & 1, p.err);
+          if (!__all_sync(0xFFFFFFFFu, ok)) break;
+          tc_fence_after();
+          uint32_t s[128];
+          const int key0 = (first + j) * kTileKeys;
+          const bool edge = key0 + kTileKeys > see_first;
+          const int limit = sees - key0;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) tmem_ld32(s_addr + 32 * q, s + 32 * q);
+          tmem_wait_ld();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) after_wait(s + 32 * q);
+          if (kApart) {
+            tc_fence_before();
+            mbar_arrive(&s_free[i]);
+          }
+          if (edge) {
+#pragma unroll
+            for (int k = 0; k < 128; ++k)
+              if (k >= limit) s[k] = 0xFF800000u;  // -inf
+          }
+          float mx[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) mx[q] = fmaxf(__uint_as_float(s[q]), __uint_as_float(s[q + 4]));
+#pragma unroll
+          for (int k = 8; k < 128; k += 8)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) mx[q] = max3(mx[q], __uint_as_float(s[k + q]), __uint_as_float(s[k + q + 4]));
+          const uint64_t scale_pair = pair(scale2, scale2);
+          const float high = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
+          // P and O of the key tile before are free once its value product is done
+          const auto before_done = [&] {
+            if (j > 0) ok = ok && wait_own(&pv_done[i], (step - 1) & 1, p.err);
+            tc_fence_after();
+          };
+          if (j == 0) {
+            ref = high == -INFINITY ? 0.f : high;
+          } else {
+            const bool move = high - ref > kLazy<T>;
+            if (__any_sync(0xFFFFFFFFu, move)) {
+              before_done();
+              const float back = move ? ex2(ref - high) : 1.f;
+              if (move) ref = high;
+              total[0] = fma2(total[0], pair(back, back), 0);
+              total[1] = fma2(total[1], pair(back, back), 0);
+#pragma unroll 1
+              for (int q = 0; q < static_cast<int>(kWideO) / 32; ++q) {
+                uint32_t o[32];
+                tmem_ld32(o_addr + 32 * q, o);
+                tmem_wait_ld();
+                after_wait(o);
+                uint32_t lo[16], hi[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                  lo[e] = __float_as_uint(__uint_as_float(o[e]) * back);
+                  hi[e] = __float_as_uint(__uint_as_float(o[e + 16]) * back);
+                }
+                tmem_st16(o_addr + 32 * q, lo);
+                tmem_st16(o_addr + 32 * q + 16, hi);
+              }
+            }
+          }
+          const uint64_t nref = pair(-ref, -ref);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t x[16];
+            weights32<T>(s + 32 * q, scale_pair, nref, total, x);
+            if (q == 0) before_done();
+            tmem_st16(p_addr + 16 * q, x);
+          }
+          if (!__all_sync(0xFFFFFFFFu, ok)) break;
+          if (key0 + kTileKeys > see_all) {
+            // values behind the last position: whatever lies there would meet weights of zero, and 0 times
+            // infinity is NaN, so it becomes zero
+            const int item = ring_at + 2 * j + 1, st = item % kStages;
+            ok = wait_own(&kv_full[st], (item / kStages) & 1, p.err);
+            if (ok && key0 + r >= see_all) {
+#pragma unroll
+              for (int h = 0; h < kPanels; ++h) {
+                uint4* row = reinterpret_cast<uint4*>(ring + st * kTileBytes + h * kPanel + r * 128);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) row[e] = make_uint4(0, 0, 0, 0);
+              }
+            }
+            fence_proxy_async();
+            if (!__all_sync(0xFFFFFFFFu, ok)) break;
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&p_ready[i]);
+        }
       }
       ring_at += 2 * count;
       float ta, tb;
       unpair(add2(total[0], total[1]), ta, tb);
-      const float row_sum = ta + tb;
-      if (ok && n > 0) ok = wait_own(&pv_done[i], (step - 1) & 1, p.err);
+      const float row_sum = kF32 ? (ta + tb) * power_of_two(-kRaise) : ta + tb;
+      if (!kF32 && ok && n > 0) ok = wait_own(&pv_done[i], (step - 1) & 1, p.err);
       tc_fence_after();
       ok = __all_sync(0xFFFFFFFFu, ok);
       const Item w = items[slot];
@@ -765,27 +1059,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int head = w.kvh * p.group + r - token * p.group;
         T* out = static_cast<T*>(p.out) + (row * p.heads + head) * p.head_dim;
         bool finite = true;
-#pragma unroll 1
-        for (int q = 0; q < D / 32; ++q) {
-          uint32_t o[32];
-          if (n > 0) {
-            tmem_ld32(o_addr + 32 * q, o);
-            tmem_wait_ld();
-            after_wait(o);
-          }
+        if constexpr (kF32) {
           if (live && ok) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              uint32_t x[4];
+            for (int e = 0; e < D; e += 4) {
+              float v[4];
 #pragma unroll
               for (int y = 0; y < 4; ++y) {
-                const float u = inv == 0.f ? 0.f : __uint_as_float(o[e + 2 * y]) * inv;
-                const float v = inv == 0.f ? 0.f : __uint_as_float(o[e + 2 * y + 1]) * inv;
-                finite = finite && fabsf(u) <= 3.402823466e38f && fabsf(v) <= 3.402823466e38f;
-                x[y] = pack2<T>(u, v);
+                v[y] = acc[e + y] * inv;
+                finite = finite && fabsf(v[y]) <= 3.402823466e38f;
               }
-              if (32 * q + e < p.head_dim)
-                *reinterpret_cast<uint4*>(out + 32 * q + e) = make_uint4(x[0], x[1], x[2], x[3]);
+              if (e < p.head_dim) *reinterpret_cast<float4*>(out + e) = make_float4(v[0], v[1], v[2], v[3]);
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (int q = 0; q < D / 32; ++q) {
+            uint32_t o[32];
+            if (n > 0) load_o<false>(o_addr + 32 * q, o);
+            if (live && ok) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 8) {
+                uint32_t x[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                  const float u = inv == 0.f ? 0.f : __uint_as_float(o[e + 2 * y]) * inv;
+                  const float v = inv == 0.f ? 0.f : __uint_as_float(o[e + 2 * y + 1]) * inv;
+                  finite = finite && fabsf(u) <= 3.402823466e38f && fabsf(v) <= 3.402823466e38f;
+                  x[y] = pack2<T>(u, v);
+                }
+                if (32 * q + e < p.head_dim)
+                  *reinterpret_cast<uint4*>(out + 32 * q + e) = make_uint4(x[0], x[1], x[2], x[3]);
+              }
             }
           }
         }
@@ -805,22 +1110,29 @@ __global__ void __launch_bounds__(kThreads, 1)
           slot_o[tid] = row_sum == 0.f ? -INFINITY : ref;  // a row that saw none of these keys takes no part
           slot_o[256 + tid] = row_sum;
         }
-#pragma unroll 1
-        for (int q = 0; q < D / 32; ++q) {
-          uint32_t o[32];
-          if (n > 0) {
-            tmem_ld32(o_addr + 32 * q, o);
-            tmem_wait_ld();
-            after_wait(o);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0u;
-          }
+        if constexpr (kF32) {
           if (live) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              *reinterpret_cast<uint4*>(slot_o + 512 + ((8 * q + e) * 256 + tid) * 4) =
-                  make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            for (int e = 0; e < D / 4; ++e)
+              *reinterpret_cast<float4*>(slot_o + 512 + (e * 256 + tid) * 4) =
+                  make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
+          }
+        } else {
+#pragma unroll 1
+          for (int q = 0; q < D / 32; ++q) {
+            uint32_t o[32];
+            if (n > 0) {
+              load_o<false>(o_addr + 32 * q, o);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = 0u;
+            }
+            if (live) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                *reinterpret_cast<uint4*>(slot_o + 512 + ((8 * q + e) * 256 + tid) * 4) =
+                    make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            }
           }
         }
       }
@@ -830,7 +1142,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   tc_fence_before();
-  cta_barrier();
+  cta_barrier<kThreads>();
   if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
@@ -883,7 +1195,11 @@ __global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant
 #pragma unroll
       for (int e = 0; e < 4; ++e) finite = finite && fabsf(v[e]) <= 3.402823466e38f;
       const int d = 4 * (warp + 8 * k);
-      if (d < p.head_dim) *reinterpret_cast<uint2*>(out + d) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+      if (d >= p.head_dim) continue;
+      if constexpr (is_f32<T>)
+        *reinterpret_cast<float4*>(out + d) = make_float4(v[0], v[1], v[2], v[3]);
+      else
+        *reinterpret_cast<uint2*>(out + d) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
     }
     if (!finite) redo_s[lane] = 1;
   }
@@ -901,10 +1217,11 @@ int launch(const AttnParams& p, int64_t max_new, int sms, void* work, cudaStream
   TcParams tp;
   tp.a = p;
   tp.tokens = kTileRows / p.group;
-  const int type = std::is_same_v<T, __nv_bfloat16> ? EFG_BF16 : EFG_F16;
+  const int type = is_f32<T> ? EFG_F32 : std::is_same_v<T, __nv_bfloat16> ? EFG_BF16 : EFG_F16;
   const int64_t kv_rows = p.kv_len ? p.n_pages * p.page_size : p.n_rows;
   tp.box_rows = p.kv_len ? static_cast<int>(std::min<int64_t>(p.page_size, kTileKeys)) : kTileKeys;
   CUtensorMap mq, mk, mv;
+  // (F32 queries do not come by TMA: their map is made all the same, it checks the rows)
   if (!encode_heads_map(&mq, type, p.q, p.head_dim, p.heads, p.n_rows, p.q_stride, p.group, tp.tokens) ||
       !encode_heads_map(&mk, type, p.k, p.head_dim, p.kv_heads, kv_rows, p.k_stride, 1, tp.box_rows) ||
       !encode_heads_map(&mv, type, p.v, p.head_dim, p.kv_heads, kv_rows, p.v_stride, 1, tp.box_rows))
@@ -916,14 +1233,14 @@ int launch(const AttnParams& p, int64_t max_new, int sms, void* work, cudaStream
   tp.tiles = static_cast<int>(tiles);
   tp.tiles_per_seq = fixed <= bound ? static_cast<int>(per_seq) : 0;
   const auto fn = attn_tc_kernel<T, D>;
-  if (int st = ensure_smem_attr(reinterpret_cast<const void*>(fn), smem_bytes<D>())) return st;
+  if (int st = ensure_smem_attr(reinterpret_cast<const void*>(fn), smem_bytes<T, D>)) return st;
   cudaLaunchConfig_t cf{};
   tp.joins = static_cast<TcJoin*>(work);
   tp.slots = work ? reinterpret_cast<float*>(tp.joins + sms) : nullptr;
   // a CTA per run, or per item; those that run take over the others
   cf.gridDim = dim3(static_cast<unsigned>(work ? sms : tiles * p.kv_heads));
-  cf.blockDim = dim3(kThreads);
-  cf.dynamicSmemBytes = smem_bytes<D>();
+  cf.blockDim = dim3(threads<T>);
+  cf.dynamicSmemBytes = smem_bytes<T, D>;
   cf.stream = s;
   EFG_TRY_CUDA(cudaLaunchKernelEx(&cf, fn, tp, mq, mk, mv), "attention launch");
   if (!work) return EFG_OK;
@@ -942,7 +1259,7 @@ int launch(const AttnParams& p, int64_t max_new, int sms, void* work, cudaStream
 }  // namespace
 
 bool attn_tc_takes(int type, const AttnParams& p) {
-  if (type == EFG_F32 || !(p.scale > 0.f) || p.group > kTileRows || reinterpret_cast<uintptr_t>(p.out) % 16) return false;
+  if ((type == EFG_F32 && p.head_dim > 64) || !(p.scale > 0.f) || p.group > kTileRows || reinterpret_cast<uintptr_t>(p.out) % 16) return false;
   if (p.q_stride == 0 || p.k_stride == 0 || p.v_stride == 0) return false;
   if (p.kv_len) {  // whole boxes of a page, whole 8-row groups of the swizzle
     if (p.n_pages == 0 || p.page_size < 8 || (p.page_size & (p.page_size - 1))) return false;
@@ -964,6 +1281,7 @@ size_t attn_tc_workspace(const AttnParams& p, int sms) {
 
 int launch_attn_tc(int type, const AttnParams& p, int sms, void* work, cudaStream_t s) {
   const int64_t max_new = p.kv_len ? std::min(p.max_new, p.n_rows) : p.n_rows;
+  if (type == EFG_F32) return launch<float, 64>(p, max_new, sms, work, s);
   if (type == EFG_F16)
     return p.head_dim <= 64 ? launch<__half, 64>(p, max_new, sms, work, s) : launch<__half, 128>(p, max_new, sms, work, s);
   return p.head_dim <= 64 ? launch<__nv_bfloat16, 64>(p, max_new, sms, work, s)
