@@ -334,7 +334,10 @@ __device__ __forceinline__ int weight_of(const AttnParams& p, int64_t seq, int p
   return sum;
 }
 
-template <typename T, int D>
+// kRuns: the work is cut into runs (tp.joins and tp.slots are set); otherwise whole items are handed out. Apart,
+// because the code of one costs the other: one 8192-token prompt takes 512 us with both in one kernel, 490
+// without the runs.
+template <typename T, int D, bool kRuns>
 __global__ void __launch_bounds__(threads<T>, 1)
     attn_tc_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ CUtensorMap map_q,
                    const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
@@ -390,8 +393,8 @@ __global__ void __launch_bounds__(threads<T>, 1)
     fence_barrier_init();
   }
   if (warp == 9) tmem_alloc(&tmem_slot, 512);
-  if (tp.tiles_per_seq == 0 && blockIdx.x == 0) check_offsets(p);
-  if (tp.joins) {
+  if (!kRuns && tp.tiles_per_seq == 0 && blockIdx.x == 0) check_offsets(p);
+  if constexpr (kRuns) {
     // This CTA's run of the line of all items' key tiles: every thread adds up a block of sequences, the one
     // whose block holds the beginning finds the sequence.
     const int n_seqs = static_cast<int>(p.n_seqs), per = (n_seqs + kThreads - 1) / kThreads;
@@ -700,7 +703,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
       };
       Item w;
       w.stop = 0;
-      if (tp.joins) {
+      if constexpr (kRuns) {
         const int line = run_s[2], n_runs = run_s[3];
         if (line > 0 && static_cast<int>(blockIdx.x) < n_runs) {
           const Runs runs(line, n_runs);
@@ -1053,7 +1056,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
       const int row0 = w.c.begin + w.token0 + i * tp.tokens;
       const bool live = token < a.tok[i];
 
-      if (w.slot < 0) {
+      if (!kRuns || w.slot < 0) {
         const float inv = sees > 0 && row_sum != 0.f ? 1.f / row_sum : 0.f;
         const int64_t row = row0 + token;
         const int head = w.kvh * p.group + r - token * p.group;
@@ -1232,7 +1235,7 @@ int launch(const AttnParams& p, int64_t max_new, int sms, void* work, cudaStream
   if (tiles * p.kv_heads > 0x3FFFFFFFll) return fail(EFG_EINVAL, "attention: too many rows");
   tp.tiles = static_cast<int>(tiles);
   tp.tiles_per_seq = fixed <= bound ? static_cast<int>(per_seq) : 0;
-  const auto fn = attn_tc_kernel<T, D>;
+  const auto fn = work ? attn_tc_kernel<T, D, true> : attn_tc_kernel<T, D, false>;
   if (int st = ensure_smem_attr(reinterpret_cast<const void*>(fn), smem_bytes<T, D>)) return st;
   cudaLaunchConfig_t cf{};
   tp.joins = static_cast<TcJoin*>(work);
