@@ -351,9 +351,9 @@ def _kinds():
     return _KINDS
 
 
-def _look(what: str, ints, floats) -> tuple[int, int]:
+def _look(what: str, ints, *groups) -> tuple:
     """Every tensor lies on the current CUDA device, where the call is queued; `ints` are contiguous
-    int32, `floats` of one plain type. Returns (its EFG code, the current stream)."""
+    int32, each group of one plain type. Returns (the current stream, the EFG code of each group)."""
     import torch
 
     kinds = _KINDS or _kinds()
@@ -363,20 +363,21 @@ def _look(what: str, ints, floats) -> tuple[int, int]:
             raise EdgeForgeError(1, f"{what}: tensors on different devices")
         if kinds.get(t.dtype) != -1 or not t.is_contiguous():
             raise EdgeForgeError(1, f"{what}: lengths, offsets, slots and pages are contiguous int32 tensors")
-    kind = None
-    for t in floats:
-        if t.get_device() != dev:
-            raise EdgeForgeError(1, f"{what}: tensors on different devices")
-        if t.dtype is not kind:
-            if kind is not None:
+    found = []
+    for group in groups:
+        kind = group[0].dtype
+        for t in group:
+            if t.get_device() != dev:
+                raise EdgeForgeError(1, f"{what}: tensors on different devices")
+            if t.dtype is not kind:
                 raise EdgeForgeError(1, f"{what}: tensors of different types, {kind} and {t.dtype}")
-            kind = t.dtype
-    code = kinds.get(kind, -1) if floats else 0
-    if code < 0:
-        raise EdgeForgeError(1, f"{what}: expected float32, float16 or bfloat16, got {kind}")
+        code = kinds.get(kind, -1)
+        if code < 0:
+            raise EdgeForgeError(1, f"{what}: expected float32, float16 or bfloat16, got {kind}")
+        found.append(code)
     if dev < 0 or dev != torch._C._cuda_getDevice():
         raise EdgeForgeError(1, f"{what}: expected tensors on the current CUDA device, got {ints[0].device}")
-    return code, torch._C._cuda_getCurrentRawStream(dev)
+    return torch._C._cuda_getCurrentRawStream(dev), *found
 
 
 def _rows3(what: str, t) -> tuple[int, int, int, int]:
@@ -394,7 +395,7 @@ def page_plan(block_table, slots, positions, cu, kv_len, taken, cached, new, fre
     """One serving step's block tables and slot map on the GPU (efg_page_plan). In: cached and new
     token counts per sequence [n], the free list. In and out: block_table [n][max_pages]. Out:
     slots and positions [rows], cu [n + 1], kv_len [n], taken [1]; all int32 CUDA tensors."""
-    _, stream = _look("page_plan", (block_table, slots, positions, cu, kv_len, taken, cached, new, free), ())
+    stream, = _look("page_plan", (block_table, slots, positions, cu, kv_len, taken, cached, new, free))
     n, rows = new.numel(), slots.numel()
     if block_table.dim() != 2 or block_table.shape[0] != n:
         raise EdgeForgeError(1, f"page_plan: expected a block table [{n}][max_pages], got {list(block_table.shape)}")
@@ -429,9 +430,10 @@ def page_store(q_out, k_cache, v_cache, q, k, v, slots, positions, cos=None, sin
         if q_out.shape != q.shape or q.shape[0] != n_rows or q.shape[2] != dim:
             raise EdgeForgeError(1, f"page_store: q {list(q.shape)} and q_out {list(q_out.shape)} for k {list(k.shape)}")
         rows, outs = (k, v, q), (k_cache, v_cache, q_out)
-    ints = (slots, positions)
-    kind, stream = _look("page_store", ints, rows)
-    cache_kind, _ = _look("page_store", ints, outs)
+    if cos is None:
+        stream, kind, cache_kind = _look("page_store", (slots, positions), rows, outs)
+    else:
+        stream, kind, cache_kind, table_kind = _look("page_store", (slots, positions), rows, outs, (cos, sin))
     if v.shape != k.shape or k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
         raise EdgeForgeError(1, f"page_store: caches {list(k_cache.shape)} and {list(v_cache.shape)} for rows "
                                 f"{list(k.shape)} and {list(v.shape)}")
@@ -442,7 +444,7 @@ def page_store(q_out, k_cache, v_cache, q, k, v, slots, positions, cos=None, sin
         raise EdgeForgeError(1, "page_store: one slot and one position per row")
     if cos is not None:
         max_pos = cos.shape[0]
-        if _look("page_store", ints, (cos, sin))[0] != 0 or tuple(cos.shape) != (max_pos, dim // 2) or sin.shape != cos.shape:
+        if table_kind != 0 or tuple(cos.shape) != (max_pos, dim // 2) or sin.shape != cos.shape:
             raise EdgeForgeError(1, f"page_store: cos and sin are float32 [max_pos][{dim // 2}]")
         outs += (cos, sin)
     for t in outs:
@@ -461,7 +463,7 @@ def attn_prompt(out, q, k, v, cu, scale: float | None = None) -> None:
     """Causal attention over packed prompts (efg_attn_prompt): out and q [rows][heads][dim], k and
     v [rows][kv_heads][dim], cu int32 [n + 1] the first row of each prompt; scale 1 / sqrt(dim) by
     default. q, k and v may be strided rows (views of one projection's output)."""
-    kind, stream = _look("attn_prompt", (cu,), (out, q, k, v))
+    stream, kind = _look("attn_prompt", (cu,), (out, q, k, v))
     n_rows, heads, dim, q_stride = _rows3("attn_prompt: q", q)
     k_rows, kv_heads, k_dim, k_stride = _rows3("attn_prompt: k", k)
     v_stride = _rows3("attn_prompt: v", v)[3]
@@ -486,7 +488,7 @@ def attn_paged(out, q, k_cache, v_cache, block_table, cu, kv_len, max_new: int, 
     [rows][heads][dim], caches [pages][page_size][kv_heads][dim], block_table [n][max_pages], cu
     [n + 1] and kv_len [n] as page_plan writes them; max_new: no chunk is longer (1 for decode).
     The workspace that long sequences need comes from torch's allocator, for this call."""
-    kind, stream = _look("attn_paged", (block_table, cu, kv_len), (out, q, k_cache, v_cache))
+    stream, kind = _look("attn_paged", (block_table, cu, kv_len), (out, q, k_cache, v_cache))
     n_rows, heads, dim, q_stride = _rows3("attn_paged: q", q)
     n = kv_len.numel()
     if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or out.shape != q.shape:

@@ -25,13 +25,19 @@ struct SeqNeed {
   bool valid;    // lengths are non-negative and the block table is wide enough
 };
 
+EFG_HD int64_t pages_for(uint32_t positions, uint32_t page_size) {
+  const uint32_t whole = positions / page_size;
+  return static_cast<int64_t>(whole) + (positions != whole * page_size);
+}
+
 EFG_HD SeqNeed seq_need(int32_t cached, int32_t fresh, int64_t page_size, int64_t max_pages) {
   SeqNeed n;
   n.rows = fresh > 0 ? fresh : 0;
   const int64_t end = static_cast<int64_t>(cached) + fresh;
   n.valid = cached >= 0 && fresh >= 0 && end <= max_pages * page_size;
-  n.have = n.valid ? (cached + page_size - 1) / page_size : 0;
-  n.need = n.valid ? (end + page_size - 1) / page_size - n.have : 0;
+  // lengths fit 32 unsigned bits here, and a 32-bit division is a fraction of a 64-bit one
+  n.have = n.valid ? pages_for(static_cast<uint32_t>(cached), static_cast<uint32_t>(page_size)) : 0;
+  n.need = n.valid ? pages_for(static_cast<uint32_t>(end), static_cast<uint32_t>(page_size)) - n.have : 0;
   return n;
 }
 
