@@ -156,15 +156,24 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
   if (tid < kKeys) slot_s[(tile_begin + kStages - 1) & 1][tid] = slot_of(tile_begin + kStages - 1);
 
   // ---- queries as A fragments (F32: the four dims 16 kk + 4 t .. + 3 of both rows)
+  // (64 wide F32 rows: from shared memory, a tile at a time; the registers are for sums)
+  constexpr bool kQueryInSmem = kF32 && D == 128 && MT == 4;
+  const uint32_t q_smem = base + kStages * 2 * kTile;
   uint32_t qa[kF32 ? 1 : KK][4];
-  float4 qf[kF32 ? KK : 1][2];
+  float4 qf[kF32 && !kQueryInSmem ? KK : 1][2];
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) {
     if constexpr (kF32) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int d = 16 * kk + 4 * t;
-        qf[kk][i] = qrow[i] && d < p.head_dim ? *reinterpret_cast<const float4*>(qrow[i] + d) : make_float4(0, 0, 0, 0);
+        const float4 v = qrow[i] && d < p.head_dim ? *reinterpret_cast<const float4*>(qrow[i] + d) : make_float4(0, 0, 0, 0);
+        if constexpr (kQueryInSmem) {
+          const int r = wrow + g + 8 * i;
+          *reinterpret_cast<float4*>(smem + (q_smem - base) + r * kRowBytes + key_chunk<T>(r, 4 * kk + t) * 16) = v;
+        } else {
+          qf[kk][i] = v;
+        }
       }
     } else {
 #pragma unroll
@@ -208,10 +217,13 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
         uint32_t qh[2][4], ql[2][4];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          split_tf32(qf[kk][i].x, qh[i][0], ql[i][0]);
-          split_tf32(qf[kk][i].y, qh[i][1], ql[i][1]);
-          split_tf32(qf[kk][i].z, qh[i][2], ql[i][2]);
-          split_tf32(qf[kk][i].w, qh[i][3], ql[i][3]);
+          const int r = wrow + g + 8 * i;  // (this lane's own stores, or registers)
+          const float4 q =
+              kQueryInSmem ? lds128(q_smem + r * kRowBytes + key_chunk<T>(r, 4 * kk + t) * 16) : qf[kQueryInSmem ? 0 : kk][i];
+          split_tf32(q.x, qh[i][0], ql[i][0]);
+          split_tf32(q.y, qh[i][1], ql[i][1]);
+          split_tf32(q.z, qh[i][2], ql[i][2]);
+          split_tf32(q.w, qh[i][3], ql[i][3]);
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -437,7 +449,8 @@ template <typename T, int D, int MT>
 int launch(const AttnParams& p, int64_t tiles, int tiles_per_seq, int splits, cudaStream_t s) {
   const auto fn = attn_mma_kernel<T, D, MT>;
   const void* key = reinterpret_cast<const void*>(fn);
-  const size_t smem = static_cast<size_t>(stages<T, D>()) * stage_bytes<T, D>();
+  const size_t smem = static_cast<size_t>(stages<T, D>()) * stage_bytes<T, D>() +
+                      (sizeof(T) == 4 && D == 128 && MT == 4 ? 64 * D * sizeof(T) : 0);
   if (int st = ensure_smem_attr(key, smem)) return st;
   if (splits > 8)
     if (int st = ensure_wide_cluster(key)) return st;
