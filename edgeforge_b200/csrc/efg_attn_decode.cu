@@ -360,13 +360,15 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
         fence_proxy_async();  // before the copy that fills this stage again
         __syncwarp();
       }
-      float s[NT][4], s2[kF32 ? NT : 1][4];  // (F32: the small products apart)
+      // F32: the small products apart, and the large ones of 32 dims at a time, added to the score by an FP32
+      // addition: the matrix instructions cut off where those round, at every step of a chain.
+      float s[NT][4], s2[kF32 ? NT : 1][4], far[kF32 ? NT : 1][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           s[n][i] = 0.f;
-          if constexpr (kF32) s2[n][i] = 0.f;
+          if constexpr (kF32) s2[n][i] = far[n][i] = 0.f;
         }
       // ---- scores
 #pragma unroll
@@ -404,6 +406,13 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
                 mma_tf32(s[n], ah, kh[2 * h], kh[2 * h + 1]);
               }
             }
+            if (kk % 2 == 1 && kk + 1 < KK) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                far[n][e] += s[n][e];
+                s[n][e] = 0.f;
+              }
+            }
           }
         } else {
 #pragma unroll
@@ -420,12 +429,12 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) s[n][e] = (s[n][e] + (s[n][e + 2] + s2[n][e])) + s2[n][e + 2];
+          for (int e = 0; e < 2; ++e) s[n][e] = (far[n][e] + s[n][e]) + ((far[n][e + 2] + s[n][e + 2] + s2[n][e]) + s2[n][e + 2]);
       } else if constexpr (kF32) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
+          for (int e = 0; e < 4; ++e) s[n][e] = (far[n][e] + s[n][e]) + s2[n][e];
       }
       // ---- softmax (base 2)
       const bool edge = j0 + kWarpKeys > w.see_first;

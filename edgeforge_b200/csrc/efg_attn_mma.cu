@@ -202,13 +202,17 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
 
     const uint32_t ks = base + static_cast<uint32_t>(buf) * (2 * kTile), vs = ks + kTile;
     const int key0 = MT == 1 ? warp * 16 : 0;
-    float s[NT][4], s2[kF32 ? NT : 1][4];  // (F32: the small products apart)
+    // F32: the small products apart; under small tiles the large ones of 32 dims at a time, added to the score by an
+    // FP32 addition: the matrix instructions cut off where those round, at every step of a chain.
+    constexpr bool kSteps = kF32 && MT == 1;
+    float s[NT][4], s2[kF32 ? NT : 1][4], far[kSteps ? NT : 1][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         s[n][i] = 0.f;
         if constexpr (kF32) s2[n][i] = 0.f;
+        if constexpr (kSteps) far[n][i] = 0.f;
       }
     // ---- scores
 #pragma unroll
@@ -242,6 +246,13 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
             mma_tf32(s2[n], al, kh[2 * h], kh[2 * h + 1]);
             mma_tf32(s[n], ah, kh[2 * h], kh[2 * h + 1]);
           }
+          if (kSteps && kk % 2 == 1 && kk + 1 < KK) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              far[kSteps ? n : 0][e] += s[n][e];
+              s[n][e] = 0.f;
+            }
+          }
         }
       } else {
 #pragma unroll
@@ -258,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
+        for (int e = 0; e < 4; ++e) s[n][e] = (kSteps ? far[kSteps ? n : 0][e] + s[n][e] : s[n][e]) + s2[n][e];
     }
     // ---- softmax of this tile (base 2), rows g and g + 8
     float back[2];
