@@ -1,10 +1,11 @@
-// efg_attn_mma.cu - attention of small row tiles (decode steps, short chunks, every FP32 call) on
-// the warp-level tensor cores, with the key axis split over warps and over a cluster.
+// efg_attn_mma.cu - attention on the warp-level tensor cores, with the key axis split over warps and over a
+// cluster: calls of few rows that the decode kernel does not take, chunks of up to 64 rows per key head, FP32
+// heads above 64, scales of zero and below, wide groups, odd pages.
 //
 // Rows of one key head are packed: row i * group + h of a sequence is query head h of the group
 // at its i-th new token, so a decode step's group of heads shares one pass over the keys. A CTA
-// owns 16 rows (its four warps take a quarter of every 64-key tile) or 64 rows (16 per warp), and
-// a share of the tiles; keys and values arrive through a ring of cp.async stages. Softmax is the
+// owns 16 rows (its four warps take a quarter of every 64-key tile) or 64 rows, or 128 (16 per
+// warp), and a share of the tiles; keys and values arrive through a ring of cp.async stages. Softmax is the
 // running maximum and sum in FP32; partial results (maximum, sum, weighted values) meet in shared
 // memory, first across warps, then across the cluster, in rank order: no atomics, no workspace,
 // no second launch, the same bits on every call.
@@ -13,6 +14,11 @@
 // the unrounded weights). F32: every operand is split x = hi + lo into two 11-bit TF32 parts and
 // a product is hi hi + hi lo + lo hi (m16n8k8): what is left out is below 2^-21 of |x y|, so the
 // result keeps FP32 accuracy at a sixth of the 16-bit rate, still above the CUDA cores' FP32.
+//
+// What bounds it: in F32 the warp-level tensor cores and the splits beside them (2048 tokens, 32 query and 4 key
+// heads of 128, FP32: 695 us, 49 TFLOP/s of the formula's products, 148 TFLOP/s of TF32 ones); of few rows the
+// latency of a tile (two loads and two products in sequence). At head size 128 the F32 sums of 64 rows and more take
+// the registers, so the queries wait in shared memory (1225 -> 1046 us) and eight warps share a tile (-> 695).
 #include <algorithm>
 #include <type_traits>
 
@@ -30,18 +36,22 @@ namespace efg {
 namespace {
 
 constexpr int kKeys = 64;      // keys of a tile
-constexpr int kThreads = 128;  // four warps
 constexpr int kMaxCluster = 16;
+// Four warps, or one for every 16 rows of a larger tile.
+constexpr int threads_of(int MT) { return MT > 4 ? 32 * MT : 128; }
 
 template <typename T, int D>
 constexpr int stage_bytes() {
   return 2 * kKeys * D * static_cast<int>(sizeof(T));
 }
 // Bytes in flight per SM decide a decode step: about 96 KB in the stages of the CTAs that fit.
-template <typename T, int D>
+template <typename T, int D, int MT>
 constexpr int stages() {
-  return stage_bytes<T, D>() <= 16384 ? 4 : 3;
+  return stage_bytes<T, D>() <= 16384 ? 4 : MT > 4 ? 2 : 3;
 }
+// Wide F32 queries of large tiles wait in shared memory: the registers are for sums.
+template <typename T, int D, int MT>
+constexpr bool query_in_smem = sizeof(T) == 4 && D == 128 && MT > 1;
 
 // 16 bytes to shared memory, or zeros.
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
@@ -67,19 +77,20 @@ __device__ __forceinline__ int value_chunk(int r, int c) {
 }
 
 template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2)
+__global__ void __launch_bounds__(threads_of(MT), (sizeof(T) == 4 && D == 128) ? 1 : 2)
     attn_mma_kernel(const AttnParams p, const int tiles_per_seq) {
   constexpr bool kF32 = sizeof(T) == 4;
   constexpr int kRows = 16 * MT, kRowBytes = D * static_cast<int>(sizeof(T)), kChunks = kRowBytes / 16;
-  constexpr int kStages = stages<T, D>(), kTile = kKeys * kRowBytes;
+  constexpr int kThreads = threads_of(MT), kWarps = kThreads / 32;
+  constexpr int kStages = stages<T, D, MT>(), kTile = kKeys * kRowBytes;
   constexpr int NT = MT == 1 ? 2 : 8;  // 8-key column groups of a warp's scores
   constexpr int KK = D / 16;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int32_t slot_s[2][kKeys];
-  __shared__ int64_t scan_s[kThreads / 32 + 2];
-  __shared__ float top_s[4][16], sum_s[4][16];  // per warp, then (row order) per CTA
-  __shared__ float part_top[64], part_sum[64];
-  __shared__ int redo_s[64];
+  __shared__ int64_t scan_s[kWarps + 2];
+  __shared__ float top_s[kWarps][16], sum_s[kWarps][16];  // per warp, then (row order) per CTA
+  __shared__ float part_top[16 * kWarps], part_sum[16 * kWarps];
+  __shared__ int redo_s[16 * kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   cg::cluster_group cluster = cg::this_cluster();
   const int splits = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
@@ -97,8 +108,9 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
   Chunk c;
   if (!chunk_of_seq(p, rt.seq, c)) return;
   const int64_t m = c.end - c.begin;
-  const int64_t row0 = rt.index * kRows;  // packed rows of this tile: row0 ..
-  if (row0 >= m * p.group) return;
+  const int64_t tiles_here = (m * p.group + kRows - 1) / kRows;
+  if (rt.index >= tiles_here) return;
+  const int64_t row0 = (tiles_here - 1 - rt.index) * kRows;  // packed rows of this tile: row0 .., the last tile first
   const int64_t rows_here = min(static_cast<int64_t>(kRows), m * p.group - row0);
   const int first_token = static_cast<int>(row0 / p.group), last_token = static_cast<int>((row0 + rows_here - 1) / p.group);
   const int see_first = seen_by(c, c.begin + first_token), see_all = seen_by(c, c.begin + last_token);
@@ -156,8 +168,7 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
   if (tid < kKeys) slot_s[(tile_begin + kStages - 1) & 1][tid] = slot_of(tile_begin + kStages - 1);
 
   // ---- queries as A fragments (F32: the four dims 16 kk + 4 t .. + 3 of both rows)
-  // (64 wide F32 rows: from shared memory, a tile at a time; the registers are for sums)
-  constexpr bool kQueryInSmem = kF32 && D == 128 && MT == 4;
+  constexpr bool kQueryInSmem = query_in_smem<T, D, MT>;
   const uint32_t q_smem = base + kStages * 2 * kTile;
   uint32_t qa[kF32 ? 1 : KK][4];
   float4 qf[kF32 && !kQueryInSmem ? KK : 1][2];
@@ -409,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
     part_top[tid] = top_s[tid >> 4][tid & 15];
     part_sum[tid] = sum_s[tid >> 4][tid & 15];
   }
-  if (tid < 64) redo_s[tid] = 0;
+  if (tid < kRows) redo_s[tid] = 0;
   if (splits > 1)
     cluster.sync();
   else
@@ -445,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && D == 128) ? 1 : 2
   }
   if (see_first < see_all) {  // a row may not be reached by what lies at positions it does not see
     __syncthreads();
-    for (int r = r_lo + warp; r < r_hi; r += kThreads / 32) {
+    for (int r = r_lo + warp; r < r_hi; r += kWarps) {
       if (!redo_s[r]) continue;
       const int64_t token = (row0 + r) / p.group;
       const int head = kvh * p.group + static_cast<int>(row0 + r - token * p.group);
@@ -460,15 +471,15 @@ template <typename T, int D, int MT>
 int launch(const AttnParams& p, int64_t tiles, int tiles_per_seq, int splits, cudaStream_t s) {
   const auto fn = attn_mma_kernel<T, D, MT>;
   const void* key = reinterpret_cast<const void*>(fn);
-  const size_t smem = static_cast<size_t>(stages<T, D>()) * stage_bytes<T, D>() +
-                      (sizeof(T) == 4 && D == 128 && MT == 4 ? 64 * D * sizeof(T) : 0);
+  const size_t smem = static_cast<size_t>(stages<T, D, MT>()) * stage_bytes<T, D>() +
+                      (query_in_smem<T, D, MT> ? 16 * MT * D * sizeof(T) : 0);
   if (int st = ensure_smem_attr(key, smem)) return st;
   if (splits > 8)
     if (int st = ensure_wide_cluster(key)) return st;
   if (tiles * splits > 0x7FFFFFFFll) return fail(EFG_EINVAL, "attention: too many rows");
   cudaLaunchConfig_t cf{};
   cf.gridDim = dim3(static_cast<unsigned>(tiles * splits), static_cast<unsigned>(p.kv_heads));
-  cf.blockDim = dim3(kThreads);
+  cf.blockDim = dim3(threads_of(MT));
   cf.dynamicSmemBytes = smem;
   cf.stream = s;
   cudaLaunchAttribute attr[1];
@@ -482,16 +493,26 @@ int launch(const AttnParams& p, int64_t tiles, int tiles_per_seq, int splits, cu
 
 template <typename T, int D>
 int dispatch(const AttnParams& p, int64_t max_rows, int64_t max_keys, int sms, cudaStream_t s) {
-  const int rows = max_rows <= 16 ? 16 : 64;
+  const bool wide = sizeof(T) == 4 && D == 128;
   // Tiles of one sequence at fixed places when that launches no more of them than an upper bound
   // over the whole batch (a decode step: exactly one per sequence), else found by a scan.
-  const int64_t fixed = p.n_seqs * ((max_rows + rows - 1) / rows), bound = p.n_rows * p.group / rows + p.n_seqs;
-  const int64_t tiles = std::min(fixed, bound);
-  const int per_seq = fixed <= bound ? static_cast<int>((max_rows + rows - 1) / rows) : 0;
-  // Split the keys until there are about four CTAs per SM, but leave each two tiles of keys.
+  auto fixed = [&](int rows) { return p.n_seqs * ((max_rows + rows - 1) / rows); };
+  auto bound = [&](int rows) { return p.n_rows * p.group / rows + p.n_seqs; };
+  auto tiles_of = [&](int rows) { return std::min(fixed(rows), bound(rows)); };
+  // 16 or 64 rows. Wide FP32 heads leave room for one CTA per SM, four warps: 128 rows on eight warps where 64-row
+  // tiles would not all run at once (2048 tokens: 692 against 1046 us; 3 prompts of up to 214 tokens, 8 key heads,
+  // 64-row tiles on 100 SMs: 58 against 48).
+  const int rows = max_rows <= 16 ? 16 : wide && max_rows > 64 && tiles_of(64) * p.kv_heads > sms ? 128 : 64;
+  const int64_t tiles = tiles_of(rows);
+  const int per_seq = fixed(rows) <= bound(rows) ? static_cast<int>((max_rows + rows - 1) / rows) : 0;
+  // Split the keys until there are about four CTAs per SM (one, where no more fit: 4 chunks of up to 169 FP32 tokens,
+  // 4 key heads of 128: 48 against 89 us), but leave each two tiles of keys.
+  const int64_t enough = (wide && rows > 16 ? 1 : 4) * sms;
   int splits = 1;
-  while (splits < kMaxCluster && tiles * p.kv_heads * splits * 2 <= 4 * sms && max_keys >= kKeys * 4 * splits) splits *= 2;
+  while (splits < kMaxCluster && tiles * p.kv_heads * splits * 2 <= enough && max_keys >= kKeys * 4 * splits) splits *= 2;
   if (rows == 16) return launch<T, D, 1>(p, tiles, per_seq, splits, s);
+  if constexpr (sizeof(T) == 4 && D == 128)
+    if (rows == 128) return launch<T, D, 8>(p, tiles, per_seq, splits, s);
   return launch<T, D, 4>(p, tiles, per_seq, splits, s);
 }
 
