@@ -43,17 +43,23 @@ int launch_rows(const AttnParams& p, cudaStream_t s) {
   return EFG_OK;
 }
 
+int check_workspace(size_t need, const void* work, size_t bytes) {
+  if (need > bytes || (need && !work))
+    return fail(EFG_EINVAL, "attention: a workspace of %zu bytes is needed, got %zu", need, bytes);
+  if (need && reinterpret_cast<uintptr_t>(work) % 16)
+    return fail(EFG_EINVAL, "attention: the workspace is not 16-byte aligned");
+  return EFG_OK;
+}
+
 int launch_attn(int type, const AttnParams& p, int sms, void* work, size_t work_bytes, cudaStream_t s) {
   if (attn_decode_takes(type, p)) {
     const size_t need = attn_decode_workspace(type, p, sms);
-    if (need > work_bytes || (need && !work))
-      return fail(EFG_EINVAL, "attention: a workspace of %zu bytes is needed, got %zu", need, work_bytes);
+    if (int st = check_workspace(need, work, work_bytes)) return st;
     return launch_attn_decode(type, p, sms, work, s);
   }
   if (attn_tc_takes(type, p)) {
     const size_t need = attn_tc_workspace(p, sms);
-    if (need > work_bytes || (need && !work))
-      return fail(EFG_EINVAL, "attention: a workspace of %zu bytes is needed, got %zu", need, work_bytes);
+    if (int st = check_workspace(need, work, work_bytes)) return st;
     return launch_attn_tc(type, p, sms, need ? work : nullptr, s);
   }
   if (attn_mma_takes(type, p)) return launch_attn_mma(type, p, sms, s);

@@ -209,6 +209,13 @@ __device__ __forceinline__ float finite_max(float m, const float4& v) {
 __device__ __forceinline__ int exponent_of(float m) { return max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -100); }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 constexpr int kTop = 14;  // split operands are scaled so that their largest value is below 2^(kTop + 1)
+// Scaled by the largest value of a tile, a part is held within 2^-25 of the scaled unit, so a value that is far larger
+// than the rest of its tile (also at a position that a row does not see, or that it gives next to no weight) takes
+// digits from the rest: of a score up to 2^-31 scale 2^(eq + ek), of a weighted sum 2^-36 2^ev for every key (eq, ek,
+// ev: exponents of the query and of the largest key and value). Rows where that passes 2^-15 of a score, or 2^-23 of
+// the largest of their sums, are computed again in FP32 (attend_row).
+constexpr float kScoreRange = 65536.f;
+constexpr int kSumRange = 13;
 
 // Whether `ok` holds for all 128 converter threads; a barrier among them.
 __device__ __forceinline__ bool all_converters(bool ok) {
@@ -866,11 +873,13 @@ __global__ void __launch_bounds__(threads<T>, 1)
         mbar_arrive(&q_full);
       }
       tiles += count > 0;
+      bool coarse = false;  // F32: a row that is computed again
       if constexpr (kF32) {
         // O of one key tile at a time is added up here, in registers: the tensor cores' accumulators cut off instead
         // of rounding, which over a long row would shrink it (by 5e-6 at 8192 keys). S is read by halves
         // to leave room for that.
         float unit = 0.f;  // of O of the key tile before
+        int high_k = -126, high_v = -126;
         const auto take = [&](float back) {
 #pragma unroll
           for (int q = 0; q < D / 32; ++q) {
@@ -911,6 +920,8 @@ __global__ void __launch_bounds__(threads<T>, 1)
           }
           const int ki = ring_at + 2 * j, vi = ki + 1;
           ok = wait_own(&exp_full[ki & 7], (ki >> 3) & 1, p.err) && wait_own(&exp_full[vi & 7], (vi >> 3) & 1, p.err);
+          high_k = max(high_k, exp_s[ki & 7]);
+          high_v = max(high_v, exp_s[vi & 7]);
           const float factor = scale2 * power_of_two(max(-120, min(120, exp_q + exp_s[ki & 7] - 2 * kTop)));
           const float high = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * factor;
           if (j == 0) {
@@ -950,6 +961,11 @@ __global__ void __launch_bounds__(threads<T>, 1)
           tc_fence_after();
           take(1.f);
         }
+        float most = 0.f;
+#pragma unroll
+        for (int e = 0; e < D; ++e) most = fmaxf(most, fabsf(acc[e]));
+        coarse = p.scale * power_of_two(max(-126, min(127, exp_q + high_k))) > kScoreRange ||
+                 (most > 0.f && most < power_of_two(max(-126, high_v - kSumRange)));
       } else {
         for (int j = 0; j < n; ++j, ++step) {
           ok = wait_own(&s_full[i], step & 1, p.err);
@@ -1098,19 +1114,22 @@ __global__ void __launch_bounds__(threads<T>, 1)
           }
         }
         // a row may not be reached by what lies at positions it does not see
-        uint32_t redo = __ballot_sync(0xFFFFFFFFu, live && ok && !finite && sees < see_all);
+        const uint32_t again = __ballot_sync(0xFFFFFFFFu, live && ok && coarse && sees > 0);
+        uint32_t redo = again | __ballot_sync(0xFFFFFFFFu, live && ok && !finite && sees < see_all);
         while (redo) {
           const int l = __ffs(redo) - 1;
           redo &= redo - 1;
           const int64_t row_l = __shfl_sync(0xFFFFFFFFu, row, l);
           const int head_l = __shfl_sync(0xFFFFFFFFu, head, l);
-          if (reached_from_behind<T>(p, w.c, row_l, w.kvh, see_all)) attend_row<T>(p, w.c, row_l, head_l);
+          if ((again >> l & 1) || reached_from_behind<T>(p, w.c, row_l, w.kvh, see_all))
+            attend_row<T>(p, w.c, row_l, head_l);
         }
       } else {
         // a piece: row `tid` of the slot; 16-byte pieces of the rows lie side by side, so that a warp's stores do
         float* slot_o = tp.slots + (static_cast<int64_t>(blockIdx.x) * 2 + w.slot) * (256 * (D + 2));
         if (live) {
-          slot_o[tid] = row_sum == 0.f ? -INFINITY : ref;  // a row that saw none of these keys takes no part
+          // a row that saw none of these keys takes no part; infinity: to be computed again
+          slot_o[tid] = row_sum == 0.f ? -INFINITY : coarse ? INFINITY : ref;
           slot_o[256 + tid] = row_sum;
         }
         if constexpr (kF32) {
@@ -1204,13 +1223,17 @@ __global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant
       else
         *reinterpret_cast<uint2*>(out + d) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
     }
-    if (!finite) redo_s[lane] = 1;
+    if (mx == INFINITY)
+      redo_s[lane] = 2;
+    else if (!finite)
+      redo_s[lane] = 1;
   }
   __syncthreads();
   const int see_all = keys_of(j.c, min(j.c.end - j.c.begin, j.token0 + 2 * tp.tokens));
   for (int x = warp; x < 32; x += 8) {
     const int rx = __shfl_sync(0xFFFFFFFFu, row, x), hx = __shfl_sync(0xFFFFFFFFu, head, x);
-    if (redo_s[x] && seen_by(j.c, rx) < see_all && reached_from_behind<T>(p, j.c, rx, j.kvh, see_all))
+    if (redo_s[x] == 2 ||
+        (redo_s[x] && seen_by(j.c, rx) < see_all && reached_from_behind<T>(p, j.c, rx, j.kvh, see_all)))
       attend_row<T>(p, j.c, rx, hx);
   }
 }

@@ -352,3 +352,165 @@ def test_bad_pages_lengths_and_chunks_are_recorded(cuda, kind, m):
     if m > 1:
         again(max_new=m - 1)
     again(cu=_i(torch, [0, m, 5 * m, 3 * m]))
+
+
+@pytest.mark.parametrize("big", [1e4, 1e8, 1e30])
+@pytest.mark.parametrize("paged", [False, True])
+def test_f32_outliers_take_no_digits_from_other_rows(cuda, big, paged):
+    """Huge finite keys and values at positions that a row does not see, and a huge value that every row gives
+    next to no weight."""
+    import torch
+
+    n, dim, at = 400, 64, 300
+    g = torch.Generator(device="cuda").manual_seed(12)
+    q = 1 + 0.1 * torch.randn(n, 4, dim, generator=g, device="cuda")
+    k, v = (torch.randn(n, 2, dim, generator=g, device="cuda") for _ in range(2))
+    k[at:], v[at:] = k[at:] * big, v[at:] * big  # the rows before do not see these
+    k[5], v[5] = -2.0, v[5] * min(big, 1e6)       # seen by all rows: a weight of about 2^-24 exp(..)
+    out = torch.full_like(q, 7.0)
+    if paged:
+        ps = 16
+        table = torch.randperm(n // ps, generator=g, device="cuda").int()[None]
+        kc, vc = (torch.empty(n // ps, ps, 2, dim, device="cuda") for _ in range(2))
+        kc[table[0].long()], vc[table[0].long()] = k.view(-1, ps, 2, dim), v.view(-1, ps, 2, dim)
+        efg.attn_paged(out, q, kc, vc, table, _i(torch, [0, n]), _i(torch, [n]), n)
+    else:
+        efg.attn_prompt(out, q, k, v, _i(torch, [0, n]))
+    _held("f32", _d(out)[:at], *attend(_d(q)[:at], _d(k)[:at], _d(v)[:at], float(np.float32(dim**-0.5))))
+    assert efg.device_error() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_long_chunks_cut_along_the_keys(cuda, kind, dim):
+    """Few long chunks share the GPU: row tiles are cut along the keys and joined; NaN and infinities at a row's
+    later positions reach it neither through a piece nor through the join."""
+    import torch
+
+    chunks = [(150, 2900), (0, 40), (70, 4100), (1, 900), (130, 130), (20, 7)]
+    q, seqs, out, args = _paged(torch, kind, chunks, 4, 2, dim, 16, seed=13, pad=2)
+    _check_paged(kind, chunks, q, seqs, out)
+    again = torch.full_like(out, 7.0)
+    efg.attn_paged(again, *args, 150)
+    assert torch.equal(out, again)
+    _, kc, vc, table, _, _ = args
+    for bad in (float("nan"), float("inf")):
+        for j in range(2800, 2900):
+            kc[int(table[0, j // 16]), j % 16] = vc[int(table[0, j // 16]), j % 16] = bad
+        efg.attn_paged(again, *args, 150)
+        k, v = seqs[0]
+        want = attend(_d(q)[:50], _d(k)[:2800], _d(v)[:2800], float(np.float32(dim**-0.5)))
+        _held(kind, _d(again)[:50], *want)
+        assert not torch.isfinite(again[50:150]).any()
+        _check_paged(kind, chunks[1:], q[150:], seqs[1:], again[150:])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 0.4])
+def test_paged_with_other_scales(cuda, kind, scale):
+    import torch
+
+    for chunks in ([(1, 300), (1, 20)], [(40, 333), (3, 3)]):
+        q, seqs, out, args = _paged(torch, kind, chunks, 8, 2, 64, 16, seed=14)
+        efg.attn_paged(out, *args, max(m for m, _ in chunks), scale=scale)
+        Q, O, a = _d(q), _d(out), 0
+        for (m, n), (k, v) in zip(chunks, seqs):
+            _held(kind, O[a : a + m], *attend(Q[a : a + m], _d(k), _d(v), float(np.float32(scale))))
+            a += m
+    assert efg.device_error() == 0
+
+
+def _c_call(torch, args, max_new, work, work_bytes):
+    """efg_attn_paged through the C interface, with a workspace of the test's choice."""
+    from edgeforge_b200 import _lib
+
+    q, kc, vc, table, cu, kv_len = args
+    out = torch.full_like(q, 7.0)
+    kind = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[q.dtype]
+    block = _lib.ATTN_PAGED.pack(kind, q.shape[2] ** -0.5, out.data_ptr(), q.data_ptr(), q.shape[1] * q.shape[2],
+                                 kc.data_ptr(), vc.data_ptr(), kc.shape[0], kc.shape[1], table.data_ptr(),
+                                 table.shape[1], cu.data_ptr(), kv_len.data_ptr(), kv_len.numel(), q.shape[0], max_new,
+                                 q.shape[1], kc.shape[2], q.shape[2], work, work_bytes)
+    return _lib.load().efg_attn_paged(block, torch.cuda.current_stream().cuda_stream), out
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m", [1, 200])
+def test_workspace_is_asked_for_and_checked(cuda, kind, m):
+    import torch
+
+    from edgeforge_b200 import _lib
+
+    chunks = [(m, 5000), (1, 100)]
+    q, seqs, out, args = _paged(torch, kind, chunks, 4, 2, 64, 16, seed=15)
+    q, kc, vc, table, cu, kv_len = args
+    kinds = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    need = _lib.load().efg_attn_paged_workspace(_lib.ATTN_PAGED.pack(
+        kinds[q.dtype], 1.0, 0, 0, 0, 0, 0, 0, 16, 0, table.shape[1], 0, 0, 2, q.shape[0], m, 4, 2, 64, 0, 0))
+    assert need > 0
+    work = torch.empty(need + 16, dtype=torch.uint8, device="cuda")
+    for ptr, size in ((0, 0), (0, need), (work.data_ptr(), need - 1), (work.data_ptr() + 8, need)):
+        status, o = _c_call(torch, args, m, ptr, size)
+        torch.cuda.synchronize()
+        assert status == 1 and (o == 7.0).all()  # EFG_EINVAL, nothing queued
+    work[need:] = 77
+    status, o = _c_call(torch, args, m, work.data_ptr(), need)
+    torch.cuda.synchronize()
+    assert status == 0 and torch.equal(o, out) and (work[need:] == 77).all()
+    _check_paged(kind, chunks, q, seqs, o)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_two_calls_at_once_and_a_graph_of_them(cuda, kind):
+    """Decode steps and chunks on two streams, and both captured in one graph, as the calls one by one."""
+    import torch
+
+    calls = []
+    for chunks, seed in (([(1, 9000), (1, 70)], 16), ([(180, 3000), (2, 50)], 17), ([(1, 400)] * 40, 18)):
+        q, _, out, args = _paged(torch, kind, chunks, 8, 2, 64, 16, seed=seed)
+        calls.append((args, max(m for m, _ in chunks), out))
+    streams = [torch.cuda.Stream() for _ in calls]
+    outs = [torch.full_like(o, 7.0) for _, _, o in calls]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for st, (args, m, _), o in zip(streams, calls, outs):
+            with torch.cuda.stream(st):
+                efg.attn_paged(o, *args, m)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o, (_, _, want) in zip(outs, calls))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        for st, (args, m, _), o in zip(streams, calls, outs):
+            st.wait_stream(main)
+            with torch.cuda.stream(st):
+                efg.attn_paged(o, *args, m)
+            main.wait_stream(st)
+    for _ in range(3):
+        for o in outs:
+            o.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o, (_, _, want) in zip(outs, calls))
+    assert efg.device_error() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m,dim,ps", [(1, 128, 128), (20, 128, 128), (100, 128, 128), (5, 128, 160)])
+def test_cache_of_more_than_2_to_the_31_elements(cuda, kind, m, dim, ps):
+    """Rows stored to and read from pages whose elements lie past 2^31 of the pool (one pool for keys and values)."""
+    import torch
+
+    dt = getattr(torch, TYPES[kind])
+    kv, n = 2, 300
+    pages = 2**31 // (ps * kv * dim) + 8
+    pool = torch.empty(pages, ps, kv, dim, dtype=dt, device="cuda")
+    table = _i(torch, [[pages - 1, 0, pages - 2]])
+    g = torch.Generator(device="cuda").manual_seed(19)
+    k, q = (torch.randn(x, h, dim, generator=g, device="cuda").to(dt) for x, h in ((n, kv), (m, 4)))
+    slots = _i(torch, [int(table[0, j // ps]) * ps + j % ps for j in range(n)])
+    efg.page_store(None, pool, pool, None, k, k, slots, slots.clone())
+    out = torch.full_like(q, 7.0)
+    efg.attn_paged(out, q, pool, pool, table, _i(torch, [0, m]), _i(torch, [n]), m)
+    _held(kind, _d(out), *attend(_d(q), _d(k), _d(k), float(np.float32(dim**-0.5))))
+    assert efg.device_error() == 0

@@ -43,7 +43,8 @@ def _setting(r, n, longest, context, ps, spare=2):
 
 @pytest.mark.parametrize("n,longest,context,ps,pad", [(1, 1, 0, 16, 0), (8, 1, 500, 16, 0), (3, 200, 40, 16, 9),
                                                       (511, 3, 70, 1, 1), (512, 40, 7, 32, 0), (513, 5, 90, 64, 600),
-                                                      (1500, 300, 300, 16, 5), (2, 5000, 3, 128, 0), (5, 0, 33, 16, 4)])
+                                                      (1500, 300, 300, 16, 5), (2, 5000, 3, 128, 0), (5, 0, 33, 16, 4), (2047, 2, 20, 16, 0),
+                                                      (2048, 3, 40, 8, 3), (2049, 9, 9, 16, 0), (5000, 4, 100, 32, 1)])
 def test_plan(cuda, n, longest, context, ps, pad):
     import torch
 
