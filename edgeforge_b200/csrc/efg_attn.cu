@@ -81,6 +81,12 @@ int check_attn(const char* who, int type, size_t n_seqs, size_t n_rows, size_t h
   return EFG_OK;
 }
 
+// Whether `out` (n_out bytes) and an input of n_rows rows overlap.
+bool overlap(const void* out, size_t n_out, const void* in, size_t n_rows, size_t stride, size_t row, size_t es) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(out), b = reinterpret_cast<uintptr_t>(in);
+  return in && n_rows && a < b + ((n_rows - 1) * stride + row) * es && b < a + n_out;
+}
+
 }  // namespace
 }  // namespace efg
 
@@ -98,6 +104,11 @@ int efg_attn_prompt(const efg_attn_prompt_args* args, void* stream) {
     return fail(EFG_EINVAL, "attn_prompt: a row stride is shorter than a row");
   if (n_rows == 0 || n_seqs == 0) return EFG_OK;
   if (!d_out || !d_q || !d_k || !d_v || !d_cu) return fail(EFG_EINVAL, "attn_prompt: null pointer");
+  const size_t es = type == EFG_F32 ? 4 : 2, n_out = n_rows * heads * head_dim * es, row = kv_heads * head_dim;
+  if (efg::overlap(d_out, n_out, d_q, n_rows, q_stride, heads * head_dim, es) ||
+      efg::overlap(d_out, n_out, d_k, n_rows, k_stride, row, es) ||
+      efg::overlap(d_out, n_out, d_v, n_rows, v_stride, row, es))
+    return fail(EFG_EINVAL, "attn_prompt: out overlaps an input");
   efg::DeviceInfo* dev = efg::current_device();
   if (!dev) return EFG_ECUDA;
   efg::AttnParams p{};
@@ -157,6 +168,11 @@ int efg_attn_paged(const efg_attn_paged_args* args, void* stream) {
   if (!d_out || !d_q || !d_cu || !d_kv_len || (n_pages && (!d_k_cache || !d_v_cache)) ||
       (max_pages && !d_block_table))
     return fail(EFG_EINVAL, "attn_paged: null pointer");
+  const size_t es = type == EFG_F32 ? 4 : 2, n_out = n_rows * heads * head_dim * es, row = kv_heads * head_dim;
+  if (efg::overlap(d_out, n_out, d_q, n_rows, q_stride, heads * head_dim, es) ||
+      efg::overlap(d_out, n_out, d_k_cache, n_pages * page_size, row, row, es) ||
+      efg::overlap(d_out, n_out, d_v_cache, n_pages * page_size, row, row, es))
+    return fail(EFG_EINVAL, "attn_paged: out overlaps an input");
   efg::DeviceInfo* dev = efg::current_device();
   if (!dev) return EFG_ECUDA;
   efg::AttnParams p{};

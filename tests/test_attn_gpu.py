@@ -514,3 +514,52 @@ def test_cache_of_more_than_2_to_the_31_elements(cuda, kind, m, dim, ps):
     efg.attn_paged(out, q, pool, pool, table, _i(torch, [0, m]), _i(torch, [n]), m)
     _held(kind, _d(out), *attend(_d(q), _d(k), _d(k), float(np.float32(dim**-0.5))))
     assert efg.device_error() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m,dim", [(1, 64), (100, 64), (1, 128), (30, 128), (100, 20)])
+def test_without_pages_and_without_positions(cuda, kind, m, dim):
+    """An empty pool and a table without columns: rows that see nothing are zeros; a length there is an error."""
+    import torch
+
+    dt = getattr(torch, TYPES[kind])
+    q = torch.randn(2 * m, 4, dim, device="cuda").to(dt)
+    cache = torch.empty(0, 16, 2, dim, dtype=dt, device="cuda")
+    for wide in (0, 2):
+        table = torch.full((2, wide), -1, dtype=torch.int32, device="cuda")
+        out = torch.full_like(q, 7.0)
+        efg.attn_paged(out, q, cache, cache, table, _i(torch, [0, m, 2 * m]), _i(torch, [0, 0]), m)
+        assert (out == 0).all() and efg.device_error() == 0
+        efg.attn_paged(out, q, cache, cache, table, _i(torch, [0, m, 2 * m]), _i(torch, [0, 5]), m)
+        torch.cuda.synchronize()
+        assert (out[:m] == 0).all() and efg.device_error() == 1
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m,heads,kv", [(1, 64, 8), (30, 64, 64), (50, 64, 8)])
+def test_queries_of_more_than_2_to_the_31_elements(cuda, kind, m, heads, kv):
+    """The last sequences' rows lie past 2^31 elements of q and out; the ones before see nothing."""
+    import torch
+
+    dt = getattr(torch, TYPES[kind])
+    dim, ps, n = 128, 16, 70
+    before = 2**31 // (heads * dim) // m + 2  # sequences of m rows and no position
+    rows = (before + 2) * m
+    q = torch.zeros(rows, heads, dim, dtype=dt, device="cuda")
+    out = torch.full_like(q, 7.0)
+    g = torch.Generator(device="cuda").manual_seed(20)
+    q[-2 * m :] = torch.randn(2 * m, heads, dim, generator=g, device="cuda").to(dt)
+    k, v = (torch.randn(10, ps, kv, dim, generator=g, device="cuda").to(dt) for _ in range(2))
+    table = torch.zeros(before + 2, 5, dtype=torch.int32, device="cuda")
+    table[-2:] = _i(torch, [[3, 1, 4, 0, 9], [2, 6, 5, 8, 7]])
+    kv_len = torch.zeros(before + 2, dtype=torch.int32, device="cuda")
+    kv_len[-2:] = n
+    cu = torch.arange(before + 3, dtype=torch.int32, device="cuda") * m
+    efg.attn_paged(out, q, k, v, table, cu, kv_len, m)
+    assert efg.device_error() == 0
+    for s in (0, 1):
+        at = table[before + s].long()
+        a = (before + s) * m
+        want = attend(_d(q[a : a + m]), _d(k[at].flatten(0, 1)[:n]), _d(v[at].flatten(0, 1)[:n]), float(np.float32(dim**-0.5)))
+        _held(kind, _d(out[a : a + m]), *want)
+    assert float(out[: before * m].abs().max()) == 0

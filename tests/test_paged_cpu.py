@@ -147,6 +147,11 @@ def test_c_refusals(efg_lib):
     said(prompt(scale=float("inf")), "not finite")
     said(prompt(cu=None), "null pointer")
     said(prompt(n_rows=2**31), "out of range")
+    Q, K, V = 2**20, 2**21, 2**22
+    said(prompt(), "out overlaps an input")
+    said(prompt(out=Q - 5 * 512 * 2 + 2, q=Q, k=K, v=V), "out overlaps an input")
+    said(prompt(out=K + (4 * 128 + 127) * 2, q=Q, k=K, v=V), "out overlaps an input")
+    said(prompt(out=V, q=Q, k=K, v=V), "out overlaps an input")
     assert prompt(n_rows=0) == 0 and prompt(n_seqs=0) == 0
 
     paged = call(lib.efg_attn_paged, ATTN_PAGED, type=2, scale=0.125, out=P, q=P, q_stride=512, k_cache=P, v_cache=P,
@@ -159,6 +164,9 @@ def test_c_refusals(efg_lib):
     said(paged(block_table=None), "null pointer")
     said(paged(v_cache=None), "null pointer")
     said(paged(heads=9), "do not divide")
+    said(paged(), "out overlaps an input")
+    said(paged(out=K + (16 * 16 * 128 - 1) * 2, q=Q, k_cache=K, v_cache=V), "out overlaps an input")
+    said(paged(out=V - 2, q=Q, k_cache=K, v_cache=V), "out overlaps an input")
     assert paged(n_rows=0) == 0 and paged(max_new=0) == 0
     assert lib.efg_attn_paged_workspace(None) == 0
 
