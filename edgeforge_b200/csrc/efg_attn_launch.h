@@ -9,7 +9,7 @@ namespace efg {
 
 struct AttnParams;
 
-// Warp-level tensor cores (efg_attn_mma.cu): head sizes up to 128 in whole 16-byte pieces, rows
+// Warp-level tensor cores (efg_attn_mma.cu): head sizes to 128 in whole 16-byte pieces, rows
 // and bases 16-byte aligned.
 bool attn_mma_takes(int type, const AttnParams& p);
 int launch_attn_mma(int type, const AttnParams& p, int sms, cudaStream_t s);
@@ -20,7 +20,8 @@ bool attn_decode_takes(int type, const AttnParams& p);
 size_t attn_decode_workspace(int type, const AttnParams& p, int sms);
 int launch_attn_decode(int type, const AttnParams& p, int sms, void* work, cudaStream_t s);
 
-// 5th-generation tensor cores (efg_attn_tc.cu): 16-bit types and more than 64 rows per key head.
+// 5th-generation tensor cores (efg_attn_tc.cu): more than 16 rows per key head, over pages more than 64; F32 head
+// sizes to 64.
 bool attn_tc_takes(int type, const AttnParams& p);
 // With a workspace of attn_tc_workspace bytes the work is cut evenly along the keys; without one (or where
 // that is 0) row tiles stay whole.

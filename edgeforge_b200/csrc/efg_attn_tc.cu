@@ -1,5 +1,5 @@
-// efg_attn_tc.cu - attention of large row tiles (prompts, chunks) in 16-bit types on the 5th-generation
-// tensor cores.
+// efg_attn_tc.cu - attention of large row tiles (prompts, chunks) on the 5th-generation tensor cores: 16-bit types
+// to head size 128, F32 to 64.
 //
 // One CTA per SM owns two 128-row tiles of one key head, each of floor(128 / group) tokens times the
 // group's query heads (row = token * group + head), so a group shares its keys and the two tiles share
@@ -15,8 +15,8 @@
 // What bounds it: at head size 128 the two products of a 128 x 128 tile take 1024 tensor-core cycles and
 // its 16384 exponentials 1024 cycles of the special function units, so neither may wait for the other;
 // at 64 the exponentials (and the instructions around them) are the bound. Measured: one 8192-token
-// prompt, 32 query and 8 key heads of 128, BF16: 476 us, 1155 TFLOP/s, 0.70 of the measured GEMM rate;
-// the same with heads of 64 in groups of 8: 383 us, 718 TFLOP/s. Measured and not kept: a part of the
+// prompt, 32 query and 8 key heads of 128, BF16: 490 us, 1120 TFLOP/s, 0.68 of the measured GEMM rate, the tensor
+// pipe and the exponentials' pipe busy for 54 % each. Measured and not kept: a part of the
 // exponentials as a degree-4 polynomial on the FMA pipes (no gain at any share), turns at the
 // exponentials for the two warps of a scheduler (491 against 430 us at 64: one warp alone does not fill
 // the special function units), sums and packing one quarter behind the exponentials (540 against 486).
@@ -28,6 +28,12 @@
 // the softmax asks for it. At 128 P overwrites S, and the other row tile's work fills the wait. With a workspace
 // (paged chunks) the work is one line of key tiles cut into equal runs, and a second launch joins the
 // rows of items that were cut, in order.
+//
+// F32 (16 warps; registers 2 x 128 x 200 and 2 x 128 x 56 of 512 x 128): TMA brings FP32 tiles, four converter warps
+// (12-15) turn each into two F16 tiles hi + lo, scaled by a power of two for the tile, and S = Qh Kh + Qh Kl + Ql Kh,
+// O = Ph [Vh | Vl] + Pl Vh in the same instructions, with P split as well. O of each key tile begins at zero and is
+// added up in the softmax threads' registers, in FP32. 2048 tokens, 32 query and 4 key heads of 64: 121 us (in TF32
+// parts on the warp-level tensor cores: 436); error of a row 4.4e-7.
 #include <algorithm>
 
 #include <cuda_runtime.h>

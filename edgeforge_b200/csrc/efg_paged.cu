@@ -60,7 +60,7 @@ __device__ __forceinline__ Pair64 block_prefix(Pair64 v, Pair64* warp_sums, Pair
 // table's entry (fresh pages start at multiples of page_size). Bound by latency: the bytes (8 per row,
 // 12 per sequence, 8 per page) are a few MB at most, and a second launch for the prefix sums would
 // cost more than repeating them per CTA does. Measured: 4.2 us for 8 single tokens; 2048 sequences with
-// 297763 new tokens 13.0 us with one sequence per thread and 64-bit divisions, 8.4 us (a call from Python, 7.3 us on the device) as it is.
+// 297763 new tokens 13.0 us with one sequence per thread and 64-bit divisions, 7.3 us as it is.
 constexpr int kPerThread = 4, kChunk = kPlanThreads * kPerThread;
 
 __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanParams p) {
@@ -203,7 +203,8 @@ struct alignas(sizeof(T) * V) Vec {
 // One CTA column per row, one thread per pair of V-wide pieces at dims i and i + head_dim / 2 of
 // one head (the two halves that a half-split rotation mixes, src/kernels.cpp:133-147); value
 // heads take the same shape without the rotation. The rotation is the decoder's: products and
-// sums rounded one by one in FP32, then once to the cache's type.
+// sums rounded one by one in FP32, then once to the cache's type. Bound by HBM: 178 MB (prompts up to 4096 FP32
+// tokens, 32 query and 2 x 8 heads of 128, to BF16 pages) in 30.6 us, 5.8 TB/s; of few rows by latency.
 template <typename Tin, typename Tout, int V>
 __global__ void __launch_bounds__(256) page_store_kernel(const StoreParams p) {
   pdl_wait();
