@@ -262,7 +262,8 @@ __device__ __noinline__ bool reached_from_behind(const AttnParams& p, const Chun
     const int64_t vr = key_row(p, c, j);
     if (vr < 0) continue;
     const T* v = static_cast<const T*>(p.v) + vr * p.v_stride + static_cast<int64_t>(kvh) * p.head_dim;
-    for (int d = lane; d < p.head_dim; d += 32) bad = bad || !(fabsf(attn_widen(v[d])) <= 3.402823466e38f);
+    // (from 2^127 on the upper part of a split FP32 value may round to infinity)
+    for (int d = lane; d < p.head_dim; d += 32) bad = bad || !(fabsf(attn_widen(v[d])) < 1.701411835e38f);
   }
   return __any_sync(0xFFFFFFFFu, bad);
 }

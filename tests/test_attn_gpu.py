@@ -563,3 +563,30 @@ def test_queries_of_more_than_2_to_the_31_elements(cuda, kind, m, heads, kv):
         want = attend(_d(q[a : a + m]), _d(k[at].flatten(0, 1)[:n]), _d(v[at].flatten(0, 1)[:n]), float(np.float32(dim**-0.5)))
         _held(kind, _d(out[a : a + m]), *want)
     assert float(out[: before * m].abs().max()) == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("m,dim", [(3, 64), (3, 128), (8, 80), (20, 64), (40, 128), (100, 64), (100, 128), (70, 20)])
+def test_the_largest_values_at_later_positions(cuda, kind, sign, m, dim):
+    """Later positions hold the type's largest or lowest value, in a prompt and over pages."""
+    import torch
+
+    dt = getattr(torch, TYPES[kind])
+    g = torch.Generator(device="cuda").manual_seed(21)
+    n, heads, kv, ps, see = 160, 4, 2, 16, 2  # the last m - see positions hold it
+    q, k, v = (torch.randn(x, h, dim, generator=g, device="cuda").to(dt) for x, h in ((m, heads), (n, kv), (n, kv)))
+    far = n - m + see
+    k[far:] = v[far:] = sign * torch.finfo(dt).max
+    scale = float(np.float32(dim**-0.5))
+    table = torch.randperm(n // ps, generator=g, device="cuda").int()[None]
+    kc, vc = (torch.empty(n // ps, ps, kv, dim, dtype=dt, device="cuda") for _ in range(2))
+    kc[table[0].long()], vc[table[0].long()] = k.view(-1, ps, kv, dim), v.view(-1, ps, kv, dim)
+    out = torch.full_like(q, 7.0)
+    efg.attn_paged(out, q, kc, vc, table, _i(torch, [0, m]), _i(torch, [n]), m)
+    want = attend(_d(q)[:see], _d(k)[:far], _d(v)[:far], scale)
+    _held(kind, _d(out)[:see], *want)
+    efg.attn_prompt(out, q, k[n - m :], v[n - m :], _i(torch, [0, m]))
+    want = attend(_d(q)[:see], _d(k)[n - m : far], _d(v)[n - m : far], scale)
+    _held(kind, _d(out)[:see], *want)
+    assert efg.device_error() == 0
