@@ -81,12 +81,6 @@ int check_attn(const char* who, int type, size_t n_seqs, size_t n_rows, size_t h
   return EFG_OK;
 }
 
-// Whether `out` (n_out bytes) and an input of n_rows rows overlap.
-bool overlap(const void* out, size_t n_out, const void* in, size_t n_rows, size_t stride, size_t row, size_t es) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(out), b = reinterpret_cast<uintptr_t>(in);
-  return in && n_rows && a < b + ((n_rows - 1) * stride + row) * es && b < a + n_out;
-}
-
 }  // namespace
 }  // namespace efg
 

@@ -344,6 +344,21 @@ int efg_page_store(const efg_page_store_args* args, void* stream) {
     return fail(EFG_EINVAL, "page_store: null pointer");
   if ((d_q && q_stride < heads * head_dim) || k_stride < kv_heads * head_dim || v_stride < kv_heads * head_dim)
     return fail(EFG_EINVAL, "page_store: a row stride is shorter than a row");
+  const size_t es = type == EFG_F32 ? 4 : 2, co = cache_type == EFG_F32 ? 4 : 2;
+  const size_t q_row = heads * head_dim, kv_row = kv_heads * head_dim;
+  const bool in_place = d_q == d_q_out && type == cache_type && q_stride == q_row;
+  auto meets = [&](const void* out, size_t n_out, bool own_q) {
+    return (!own_q && efg::overlap(out, n_out, d_q, n_rows, q_stride, q_row, es)) ||
+           efg::overlap(out, n_out, d_k, n_rows, k_stride, kv_row, es) ||
+           efg::overlap(out, n_out, d_v, n_rows, v_stride, kv_row, es);
+  };
+  const size_t cache = n_slots * kv_row * co;
+  if (meets(d_q_out, n_rows * q_row * co, in_place) || meets(d_k_cache, cache, false) || meets(d_v_cache, cache, false))
+    return fail(EFG_EINVAL, "page_store: an output overlaps an input");
+  if (efg::overlap(d_k_cache, cache, d_v_cache, n_slots, kv_row, kv_row, co) ||
+      efg::overlap(d_q_out, n_rows * q_row * co, d_k_cache, n_slots, kv_row, kv_row, co) ||
+      efg::overlap(d_q_out, n_rows * q_row * co, d_v_cache, n_slots, kv_row, kv_row, co))
+    return fail(EFG_EINVAL, "page_store: outputs overlap");
   efg::DeviceInfo* dev = efg::current_device();
   if (!dev) return EFG_ECUDA;
   efg::StoreParams p{};
@@ -366,7 +381,6 @@ int efg_page_store(const efg_page_store_args* args, void* stream) {
   p.kv_heads = static_cast<int>(kv_heads);
   p.head_dim = static_cast<int>(head_dim);
   p.err = dev->d_err;
-  const size_t es = type == EFG_F32 ? 4 : 2, co = cache_type == EFG_F32 ? 4 : 2;
   const bool wide = head_dim % 8 == 0 && q_stride % 4 == 0 && k_stride % 4 == 0 && v_stride % 4 == 0 &&
                     efg::aligned(d_q, 4 * es) && efg::aligned(d_k, 4 * es) && efg::aligned(d_v, 4 * es) &&
                     efg::aligned(d_q_out, 4 * co) && efg::aligned(d_k_cache, 4 * co) &&

@@ -329,7 +329,8 @@ int efg_page_plan(const efg_page_plan_args* args, void* stream);
 /* For every row r: q_out[r] = RoPE(q[r]) at d_positions[r], the cache's slot d_slots[r] gets
  * RoPE(k[r]) and v[r]. d_cos and d_sin are [max_pos][head_dim / 2] tables (the rotation of
  * src/kernels.cpp:133-147, halves of a head paired); both NULL: no rotation. d_q and d_q_out
- * both NULL: keys and values only. q_out may be q itself (same type, rows back to back).
+ * both NULL: keys and values only. q_out may be q itself (same type, rows back to back);
+ * otherwise no output overlaps an input or another output (EFG_EINVAL).
  * cache_type (of q_out and of the caches) is `type`, or EFG_F16 / EFG_BF16 for EFG_F32 rows: the
  * rotation is in FP32 and rounds once, to nearest even. A row with position -1 is left out, one
  * with slot -1 has its query rotated and stores nothing. The slots of a call must be distinct.

@@ -498,21 +498,21 @@ def test_two_calls_at_once_and_a_graph_of_them(cuda, kind):
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("m,dim,ps", [(1, 128, 128), (20, 128, 128), (100, 128, 128), (5, 128, 160)])
 def test_cache_of_more_than_2_to_the_31_elements(cuda, kind, m, dim, ps):
-    """Rows stored to and read from pages whose elements lie past 2^31 of the pool (one pool for keys and values)."""
+    """Rows stored to and read from pages whose elements lie past 2^31 of the pool."""
     import torch
 
     dt = getattr(torch, TYPES[kind])
     kv, n = 2, 300
     pages = 2**31 // (ps * kv * dim) + 8
-    pool = torch.empty(pages, ps, kv, dim, dtype=dt, device="cuda")
+    kc, vc = (torch.empty(pages, ps, kv, dim, dtype=dt, device="cuda") for _ in range(2))
     table = _i(torch, [[pages - 1, 0, pages - 2]])
     g = torch.Generator(device="cuda").manual_seed(19)
-    k, q = (torch.randn(x, h, dim, generator=g, device="cuda").to(dt) for x, h in ((n, kv), (m, 4)))
+    k, v, q = (torch.randn(x, h, dim, generator=g, device="cuda").to(dt) for x, h in ((n, kv), (n, kv), (m, 4)))
     slots = _i(torch, [int(table[0, j // ps]) * ps + j % ps for j in range(n)])
-    efg.page_store(None, pool, pool, None, k, k, slots, slots.clone())
+    efg.page_store(None, kc, vc, None, k, v, slots, slots.clone())
     out = torch.full_like(q, 7.0)
-    efg.attn_paged(out, q, pool, pool, table, _i(torch, [0, m]), _i(torch, [n]), m)
-    _held(kind, _d(out), *attend(_d(q), _d(k), _d(k), float(np.float32(dim**-0.5))))
+    efg.attn_paged(out, q, kc, vc, table, _i(torch, [0, m]), _i(torch, [n]), m)
+    _held(kind, _d(out), *attend(_d(q), _d(k), _d(v), float(np.float32(dim**-0.5))))
     assert efg.device_error() == 0
 
 

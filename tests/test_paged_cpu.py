@@ -133,6 +133,15 @@ def test_c_refusals(efg_lib):
     said(store(sin=None), "come together")
     said(store(k_stride=127), "shorter than a row")
     said(store(slots=None), "null pointer")
+    A = {"q_out": 2**16, "k_cache": 2**18, "v_cache": 2**19, "q": 2**20, "k": 2**21, "v": 2**22}
+    said(store(), "an output overlaps an input")
+    said(store(**{**A, "q_out": 2**20 + 2}), "an output overlaps an input")  # not q itself
+    said(store(**{**A, "q_out": 2**20, "q_stride": 513}), "an output overlaps an input")  # rows apart
+    said(store(**{**A, "type": 0, "q_out": 2**20}), "an output overlaps an input")  # another type
+    said(store(**{**A, "k_cache": 2**21 + (2 * 128 + 127) * 2}), "an output overlaps an input")
+    said(store(**{**A, "v_cache": 2**22 - 64 * 128 * 2 + 2}), "an output overlaps an input")
+    said(store(**{**A, "v_cache": 2**18}), "outputs overlap")
+    said(store(**{**A, "q_out": 2**18 + 64 * 128 * 2 - 2}), "outputs overlap")
     assert store(n_rows=0) == 0  # nothing to do
 
     prompt = call(lib.efg_attn_prompt, ATTN_PROMPT, type=2, scale=0.125, out=P, q=P, q_stride=512, k=P, k_stride=128, v=P,
