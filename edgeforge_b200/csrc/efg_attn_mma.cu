@@ -97,6 +97,8 @@ __global__ void __launch_bounds__(threads_of(MT), (sizeof(T) == 4 && D == 128) ?
   const int kvh = blockIdx.y;
   const int64_t tile_id = blockIdx.x / splits;
 
+  pdl_wait();
+  pdl_launch_dependents();
   if (tiles_per_seq == 0 && blockIdx.x == 0 && kvh == 0) check_offsets(p);
   RowTile rt;
   if (tiles_per_seq > 0) {
@@ -482,11 +484,13 @@ int launch(const AttnParams& p, int64_t tiles, int tiles_per_seq, int splits, cu
   cf.blockDim = dim3(threads_of(MT));
   cf.dynamicSmemBytes = smem;
   cf.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {static_cast<unsigned>(splits), 1, 1};
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cf.attrs = attr;
-  cf.numAttrs = 1;
+  cf.numAttrs = 2;
   EFG_TRY_CUDA(cudaLaunchKernelEx(&cf, fn, p, tiles_per_seq), "attention launch");
   return EFG_OK;
 }

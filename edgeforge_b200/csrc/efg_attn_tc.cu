@@ -406,6 +406,9 @@ __global__ void __launch_bounds__(threads<T>, 1)
     fence_barrier_init();
   }
   if (warp == 9) tmem_alloc(&tmem_slot, 512);
+  // (the next launch may not begin early: its CTAs would take SMs from items that are still to be handed out, 120
+  // against 127 us for 2048 FP32 tokens call after call)
+  pdl_wait();
   if (!kRuns && tp.tiles_per_seq == 0 && blockIdx.x == 0) check_offsets(p);
   if constexpr (kRuns) {
     // This CTA's run of the line of all items' key tiles: every thread adds up a block of sequences, the one
@@ -1274,16 +1277,16 @@ int launch(const AttnParams& p, int64_t max_new, int sms, void* work, cudaStream
   cf.blockDim = dim3(threads<T>);
   cf.dynamicSmemBytes = smem_bytes<T, D>;
   cf.stream = s;
-  EFG_TRY_CUDA(cudaLaunchKernelEx(&cf, fn, tp, mq, mk, mv), "attention launch");
-  if (!work) return EFG_OK;
-  cf.gridDim = dim3(static_cast<unsigned>(sms), 8);
-  cf.blockDim = dim3(256);
-  cf.dynamicSmemBytes = 0;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cf.attrs = attr;
   cf.numAttrs = 1;
+  EFG_TRY_CUDA(cudaLaunchKernelEx(&cf, fn, tp, mq, mk, mv), "attention launch");
+  if (!work) return EFG_OK;
+  cf.gridDim = dim3(static_cast<unsigned>(sms), 8);
+  cf.blockDim = dim3(256);
+  cf.dynamicSmemBytes = 0;
   EFG_TRY_CUDA(cudaLaunchKernelEx(&cf, attn_tc_join_kernel<T, D>, tp), "attention launch");
   return EFG_OK;
 }

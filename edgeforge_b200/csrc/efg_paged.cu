@@ -298,6 +298,15 @@ int efg_page_plan(const efg_page_plan_args* args, void* stream) {
     return fail(EFG_EINVAL, "page_plan: %zu pages of %zu slots pass the 2^31 slots of a cache", n_pages, page_size);
   if (n_rows > 0x7FFFFFFFull || n_seqs > (1ull << 24) || n_free > 0x7FFFFFFFull || max_pages > 0x7FFFFFFFull)
     return fail(EFG_EINVAL, "page_plan: a size is out of range");
+  const struct {
+    const void* at;
+    size_t n;
+  } parts[] = {{d_block_table, n_seqs * max_pages}, {d_slots, n_rows}, {d_positions, n_rows}, {d_cu, n_seqs + 1},
+               {d_kv_len, n_seqs}, {d_taken, 1}, {d_cached, n_seqs}, {d_new, n_seqs}, {d_free, n_free}};
+  for (int i = 0; i < 6; ++i)  // the outputs, against everything behind them
+    for (int j = i + 1; j < 9; ++j)
+      if (efg::overlap(parts[i].at, parts[i].n * 4, parts[j].at, parts[j].n ? 1 : 0, 0, parts[j].n, 4))
+        return fail(EFG_EINVAL, "page_plan: an output overlaps an input or another output");
   efg::DeviceInfo* dev = efg::current_device();
   if (!dev) return EFG_ECUDA;
   efg::PlanParams p{};

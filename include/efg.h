@@ -312,7 +312,8 @@ int efg_lm_head_argmax_sharded(int qtype, float* d_logits_shard, int32_t* d_toke
  * needs a page (EFG_ENOMEM for efg_device_error); one with negative lengths or more positions
  * than max_pages hold is not served either (EFG_EINVAL). The rows of a sequence that is not
  * served get slot and position -1 and its kv_len is 0. More new tokens than n_rows: the rows
- * behind n_rows are dropped and d_cu stops at n_rows (EFG_EINVAL). */
+ * behind n_rows are dropped and d_cu stops at n_rows (EFG_EINVAL). No output may overlap an input
+ * or another output (EFG_EINVAL; kv_len is not cached updated in place). */
 typedef struct {
   int32_t* d_block_table; /* [n_seqs][max_pages], in and out */
   size_t max_pages;

@@ -119,6 +119,12 @@ def test_c_refusals(efg_lib):
     said(plan(page_size=0), "page size 0")
     said(plan(n_pages=2**30), "2^31 slots")
     said(plan(n_rows=2**31), "out of range")
+    A = {n: 2**16 * (i + 1) for i, n in enumerate(("block_table", "slots", "positions", "cu", "kv_len", "taken", "cached", "new", "free"))}
+    said(plan(**{**A, "kv_len": A["cached"]}), "overlaps")
+    said(plan(**{**A, "kv_len": A["new"] + 4}), "overlaps")
+    said(plan(**{**A, "positions": A["slots"] + 28}), "overlaps")
+    said(plan(**{**A, "taken": A["cu"] + 8}), "overlaps")
+    said(plan(**{**A, "block_table": A["free"] + 28}), "overlaps")
 
     store = call(lib.efg_page_store, PAGE_STORE, type=2, cache_type=2, q_out=P, k_cache=P, v_cache=P, n_slots=64, q=P,
                  q_stride=512, k=P, k_stride=128, v=P, v_stride=128, slots=P, positions=P, n_rows=3, cos=P, sin=P,
