@@ -211,8 +211,9 @@ __device__ __forceinline__ float finite_max(float m, const float4& v) {
   for (int i = 0; i < 4; ++i) m = a[i] <= 3.402823466e38f ? fmaxf(m, a[i]) : m;
   return m;
 }
-// Exponent of the largest magnitude (held at -100 and above), and 2^e.
-__device__ __forceinline__ int exponent_of(float m) { return max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -100); }
+// Exponent of the largest magnitude (held at kLeast and above, also for zeros), and 2^e.
+constexpr int kLeast = -100;
+__device__ __forceinline__ int exponent_of(float m) { return max(static_cast<int>(__float_as_uint(m) >> 23) - 127, kLeast); }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 constexpr int kTop = 14;  // split operands are scaled so that their largest value is below 2^(kTop + 1)
 // Scaled by the largest value of a tile, a part is held within 2^-25 of the scaled unit, so a value that is far larger
@@ -970,11 +971,13 @@ __global__ void __launch_bounds__(threads<T>, 1)
           tc_fence_after();
           take(1.f);
         }
-        float most = 0.f;
+        float most = 0.f, ta, tb;
 #pragma unroll
         for (int e = 0; e < D; ++e) most = fmaxf(most, fabsf(acc[e]));
+        unpair(add2(total[0], total[1]), ta, tb);
+        // (sums of zero too: both parts of a value far below its tile's largest are zero; tiles of zeros have none)
         coarse = p.scale * power_of_two(max(-126, min(127, exp_q + high_k))) > kScoreRange ||
-                 (most > 0.f && most < power_of_two(max(-126, high_v - kSumRange)));
+                 (ta + tb > 0.f && high_v > kLeast && most < power_of_two(max(-126, high_v - kSumRange)));
       } else {
         for (int j = 0; j < n; ++j, ++step) {
           ok = wait_own(&s_full[i], step & 1, p.err);

@@ -1,0 +1,71 @@
+"""FP32 attention over wide ranges of values, element by element against float64 (attn_reference.py states the error
+that is allowed and why; no term is added to it here)."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import edgeforge_b200 as efg
+from attn_reference import attend, tolerance
+
+pytestmark = pytest.mark.gpu
+MAX = float(np.finfo(np.float32).max)
+
+
+def _i(torch, a):
+    return torch.tensor(a, dtype=torch.int32, device="cuda")
+
+
+def _d(t):
+    return t.double().cpu().numpy()
+
+
+def _held(got, *expected):
+    want, tol = expected[0], tolerance("f32", *expected)
+    off = np.abs(got - want)
+    assert np.isfinite(got).all()
+    assert (off <= tol).all(), (float((off / np.maximum(tol, 1e-300)).max()), float(off.max()))
+
+
+def _call(torch, q, k, v, ps=16):
+    """The chunk q after all but its own of the positions of k and v: as a prompt where it has them all, over shuffled
+    pages otherwise."""
+    m, n, dim = q.shape[0], k.shape[0], q.shape[2]
+    out = torch.full_like(q, 7.0)
+    if m == n:
+        efg.attn_prompt(out, q, k, v, _i(torch, [0, m]))
+    else:
+        pages = -(-n // ps)
+        table = torch.randperm(pages, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").int()[None]
+        kc, vc = (torch.full((pages, ps, k.shape[1], dim), float("nan"), device="cuda") for _ in range(2))
+        at = torch.arange(n, device="cuda")
+        slots = table[0].long()[at // ps] * ps + at % ps
+        kc.view(-1, k.shape[1], dim)[slots], vc.view(-1, k.shape[1], dim)[slots] = k, v
+        efg.attn_paged(out, q, kc, vc, table, _i(torch, [0, m]), _i(torch, [n]), m)
+    torch.cuda.synchronize()
+    assert efg.device_error() == 0
+    return _d(out)
+
+
+def _inputs(torch, m, n, dim, seed, heads=4, kv=2):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = 1 + 0.1 * torch.randn(m, heads, dim, generator=g, device="cuda")
+    k, v = (torch.randn(n, kv, dim, generator=g, device="cuda") for _ in range(2))
+    return q, k, v
+
+
+@pytest.mark.parametrize("what", ["values", "keys", "both"])
+@pytest.mark.parametrize("big", [1e8, 1e13, 1e30, MAX])
+@pytest.mark.parametrize("m,n,see,dim", [(64, 64, 40, 64), (400, 400, 300, 64), (100, 100, 3, 20), (100, 1500, 40, 64),
+                                         (100, 4000, 70, 64), (20, 20, 9, 64), (64, 64, 40, 128), (4, 300, 2, 64)])
+def test_huge_later_positions(cuda, what, big, m, n, see, dim):
+    """Huge finite keys or values from the position behind row see - 1 on: the rows before see none of them, whether
+    they fill a key tile, lie in the first one or are all that one piece of the keys holds."""
+    import torch
+
+    q, k, v = _inputs(torch, m, n, dim, 31)
+    far = n - m + see
+    for t in {"values": (v,), "keys": (k,), "both": (k, v)}[what]:
+        t[far:] = (t[far:].sign() if big == MAX else t[far:]) * big
+    out = _call(torch, q, k, v)
+    _held(out[:see], *attend(_d(q)[:see], _d(k)[:far], _d(v)[:far], float(np.float32(dim**-0.5))))
