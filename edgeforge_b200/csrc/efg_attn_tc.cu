@@ -30,10 +30,11 @@
 // rows of items that were cut, in order.
 //
 // F32 (16 warps; registers 2 x 128 x 200 and 2 x 128 x 56 of 512 x 128): TMA brings FP32 tiles, four converter warps
-// (12-15) turn each into two F16 tiles hi + lo, scaled by a power of two for the tile, and S = Qh Kh + Qh Kl + Ql Kh,
-// O = Ph [Vh | Vl] + Pl Vh in the same instructions, with P split as well. O of each key tile begins at zero and is
-// added up in the softmax threads' registers, in FP32. 2048 tokens, 32 query and 4 key heads of 64: 121 us (in TF32
-// parts on the warp-level tensor cores: 436); error of a row 4.4e-7.
+// (12-15) turn each into two F16 tiles hi + lo, scaled by a power of two (keys: one for the tile, values: one for each
+// dim), and S = Qh Kh + Qh Kl + Ql Kh, O = Ph [Vh | Vl] + Pl Vh in the same instructions, with P split as well. O of each
+// key tile begins at zero and is added up in the softmax threads' registers, in FP32. Bound by the converters: 2048
+// tokens, 32 query and 4 key heads of 64: 133 us (in TF32 parts on the warp-level tensor cores: 436; with one scale for
+// a tile's values, which takes the digits of small dims beside large ones: 121); error of a row 4.4e-7.
 #include <algorithm>
 
 #include <cuda_runtime.h>
@@ -146,6 +147,18 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// Largest and least of three magnitudes (NaN left out).
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float r;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float min3_abs(float a, float b, float c) {
+  float r;
+  asm("min.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // Ties the registers of a TMEM load to the point after its wait.
 __device__ __forceinline__ void after_wait(uint32_t* r) {
 #pragma unroll
@@ -170,7 +183,11 @@ __device__ __forceinline__ void weights32(const uint32_t* s, uint64_t scale, uin
   }
 }
 
-// The same for F32: each weight as the sum of two F16 values.
+// The lo parts of weights and values are held 2^11 times larger than they are: next to their hi part that is the
+// largest factor that F16 takes, and it keeps the digits of what lies up to 2^28 below the largest.
+constexpr float kLoUp = 2048.f;
+
+// The same for F32: each weight (below 2^3, raised by 2^12) as hi + 2^-11 lo in F16, within 2^-22 of itself or 2^-48 of 1.
 __device__ __forceinline__ void weights32_split(const uint32_t* s, uint64_t scale, uint64_t nref, uint64_t (&total)[2],
                                                 uint32_t (&hi)[16], uint32_t (&lo)[16]) {
 #pragma unroll
@@ -185,24 +202,29 @@ __device__ __forceinline__ void weights32_split(const uint32_t* s, uint64_t scal
     const __half2 h = __floats2half2_rn(a, b);
     const float2 back = __half22float2(h);
     hi[i] = *reinterpret_cast<const uint32_t*>(&h);
-    lo[i] = pack2<__half>(a - back.x, b - back.y);
+    const uint64_t rest = fma2(pair(back.x, back.y), pair(-1.f, -1.f), w);  // exact
+    unpair(fma2(rest, pair(kLoUp, kLoUp), 0), a, b);
+    lo[i] = pack2<__half>(a, b);
   }
 }
 
-// Eight FP32 values times a power of two, as F16 hi and lo parts: x = hi + lo within 2^-22 |x| (or 2^-25
-// of the scaled unit).
-__device__ __forceinline__ void split8(const float4& x, const float4& y, float scale, uint4& hi, uint4& lo) {
-  const float v[8] = {x.x * scale, x.y * scale, x.z * scale, x.w * scale, y.x * scale, y.y * scale, y.z * scale, y.w * scale};
-  uint32_t h[4], l[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __half2 t = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-    const float2 back = __half22float2(t);
-    h[i] = *reinterpret_cast<const uint32_t*>(&t);
-    l[i] = pack2<__half>(v[2 * i] - back.x, v[2 * i + 1] - back.y);
-  }
-  hi = make_uint4(h[0], h[1], h[2], h[3]);
-  lo = make_uint4(l[0], l[1], l[2], l[3]);
+// Four FP32 values, scaled by powers of two, as F16 parts hi + lo, or hi + lo / kLoUp: within 2^-22 of the value or
+// 2^-25 (2^-36) of the scaled unit.
+template <bool kUp>
+__device__ __forceinline__ void split4(const float4& x, const float4& scale, uint2& hi, uint2& lo) {
+  const auto split2 = [](uint64_t v, uint32_t& hi, uint32_t& lo) {
+    float a, b;
+    unpair(v, a, b);
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 back = __half22float2(h);
+    uint64_t rest = fma2(pair(back.x, back.y), pair(-1.f, -1.f), v);  // exact
+    if (kUp) rest = fma2(rest, pair(kLoUp, kLoUp), 0);
+    unpair(rest, a, b);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = pack2<__half>(a, b);
+  };
+  split2(fma2(pair(x.x, x.y), pair(scale.x, scale.y), 0), hi.x, lo.x);
+  split2(fma2(pair(x.z, x.w), pair(scale.z, scale.w), 0), hi.y, lo.y);
 }
 // Largest finite magnitude of a quad and what came before.
 __device__ __forceinline__ float finite_max(float m, const float4& v) {
@@ -211,18 +233,20 @@ __device__ __forceinline__ float finite_max(float m, const float4& v) {
   for (int i = 0; i < 4; ++i) m = a[i] <= 3.402823466e38f ? fmaxf(m, a[i]) : m;
   return m;
 }
-// Exponent of the largest magnitude (held at kLeast and above, also for zeros), and 2^e.
-constexpr int kLeast = -100;
-__device__ __forceinline__ int exponent_of(float m) { return max(static_cast<int>(__float_as_uint(m) >> 23) - 127, kLeast); }
+// Exponent of the largest magnitude (held at -100 and above), and 2^e.
+__device__ __forceinline__ int exponent_of(float m) { return max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -100); }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 constexpr int kTop = 14;  // split operands are scaled so that their largest value is below 2^(kTop + 1)
-// Scaled by the largest value of a tile, a part is held within 2^-25 of the scaled unit, so a value that is far larger
-// than the rest of its tile (also at a position that a row does not see, or that it gives next to no weight) takes
-// digits from the rest: of a score up to 2^-31 scale 2^(eq + ek), of a weighted sum 2^-36 2^ev for every key (eq, ek,
-// ev: exponents of the query and of the largest key and value). Rows where that passes 2^-15 of a score, or 2^-23 of
-// the largest of their sums, are computed again in FP32 (attend_row).
+// A value that is far larger than the rest of what shares its scale (also one at a position that a row does not see, or
+// that it gives next to no weight) takes digits from the rest.
+//   Keys: one scale for a tile. A score loses up to 2^-31 scale 2^(eq + ek) (eq, ek: exponents of the query and of the
+// largest key); rows where that passes 2^-15 are computed again in FP32 (attend_row).
+//   Values: a scale for every dim of a tile. A weighted sum loses up to 2^(ev - 50) of the sum of the weights, and
+// 2^(ev - 48) for every key that weighs less than 2^-26 (ev: exponent of the dim's largest value). Where every value of
+// the dim is zero or at least 2^(ev - 26), the first is below 2^-24 of sum w |v|, whatever the weights are. Where one is
+// not, rows with a sum below 2^(ev - 26) of the weights' are computed again: of normally distributed values a dim in
+// a thousand tiles, and then one row in ten thousand. (kTop + kRaise = 26: a dim's unit is that bound.)
 constexpr float kScoreRange = 65536.f;
-constexpr int kSumRange = 13;
 
 // Whether `ok` holds for all 128 converter threads; a barrier among them.
 __device__ __forceinline__ bool all_converters(bool ok) {
@@ -277,7 +301,7 @@ struct alignas(16) TcJoin {
   int32_t kvh, token0, first, parts;  // parts 0: nothing begins here that is cut
 };
 
-// 32 columns of O; F32: the products with V hi plus those with V lo, 64 columns on.
+// 32 columns of O; F32: the products of both hi parts plus, 64 columns on, those with a lo part.
 template <bool kF32>
 __device__ __forceinline__ void load_o(uint32_t addr, uint32_t (&o)[32]) {
   tmem_ld32(addr, o);
@@ -288,7 +312,7 @@ __device__ __forceinline__ void load_o(uint32_t addr, uint32_t (&o)[32]) {
     after_wait(o);
     after_wait(lo);
 #pragma unroll
-    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) + __uint_as_float(lo[e]));
+    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(fmaf(__uint_as_float(lo[e]), 1.f / kLoUp, __uint_as_float(o[e])));
   } else {
     tmem_wait_ld();
     after_wait(o);
@@ -368,10 +392,16 @@ __global__ void __launch_bounds__(threads<T>, 1)
   __shared__ uint64_t q_full, q_empty, kv_full[kStages], kv_empty[kStages], s_full[2], s_free[2], p_ready[2], pv_done[2],
       drained[2], item_full[2], item_empty[2], fetch, asked;
   __shared__ uint64_t stage_full[kStaging], stage_empty[kStaging], exp_full[8];
-  __shared__ int exp_s[8];  // exponents of the split tiles, by ring item
+  // exponents of the split key tiles, by ring item; units of the value tiles' dims (what 1 of O stands for), by value
+  // tile; by item with keys the biased exponent of the largest unit of every dim, 0 where its values are close enough;
+  // by dim the exponents of each warp's largest and least values, a byte each
+  __shared__ int exp_s[8];
+  __shared__ float4 unit_s[kF32 ? 3 : 1][16];
+  __shared__ uint4 wide_s[2][kF32 ? 4 : 1], dims_s[2][kF32 ? 16 : 1];
   __shared__ float max_s[2][4];
   __shared__ uint4 answer;
-  __shared__ int scan_s[kThreads / 32], run_s[5];
+  __shared__ int run_s[5];
+  int* scan_s = reinterpret_cast<int*>(unit_s);  // (before the roles begin)
   __shared__ Item items[2];
   __shared__ uint32_t tmem_slot;
   const AttnParams& p = tp.a;
@@ -647,53 +677,145 @@ __global__ void __launch_bounds__(threads<T>, 1)
       mbar_drain(&drained[mine], 0, p.err);
     } else if (kF32 && warp >= 12) {
       // -------------------------------------------------------------- converters
-      // An FP32 tile (128 rows of 64 dims, two swizzled panels) becomes the hi and lo panels of an operand tile,
-      // scaled by a power of two after its largest magnitude; a thread per row. Rows behind the last
-      // position become zeros, whatever lies there.
-      const int r = tid - 384;
+      // An FP32 tile (128 rows of 64 dims, two swizzled panels) becomes the hi and lo panels of an operand tile. Keys: a
+      // thread per row, scaled by a power of two after the tile's largest magnitude. Values: 16 rows of four dims a
+      // thread, scaled after the largest of each dim. Rows behind the last position become zeros, whatever lies there.
+      const int r_ = tid - 384;
       Item w;
       bool ok = true;
-      int at = 0;
+      int at = 0, tiles = 0, part = 0;
       while (ok && next_item(w)) {
         const Plan a = plan_of(w, tp.tokens);
+        uint32_t most = 0, least = 0xFFFFFFFFu;  // exponents of dims 4 quad .. so far (threads 0-15)
         for (int x = 0; x < 2 * w.count && ok; ++x, ++at) {
-          const int st = at % kStaging, op = at % kStages;
-          const bool valid = (w.first + (x >> 1)) * kTileKeys + r < a.see_all;
+          // (opaque, so that the addresses below are not kept in registers across tiles, which spills)
+          int r = r_;
+          asm volatile("" : "+r"(r));
+          const int quad = r & 15, row0 = (r >> 4) * 16;
+          const int st = at % kStaging, op = at % kStages, keys = a.see_all - (w.first + (x >> 1)) * kTileKeys;
           ok = wait_own(&stage_full[st], (at / kStaging) & 1, p.err);
           if (ok && at >= kStages) ok = wait_own(&kv_empty[op], ((at / kStages) - 1) & 1, p.err);
-          const uint8_t* src = stage + st * kTileBytes + r * 128;
-          auto chunk = [&](int c) {
-            return *reinterpret_cast<const float4*>(src + (c >> 3) * kPanel + (((c & 7) ^ (r & 7)) << 4));
+          uint8_t *src = stage + st * kTileBytes, *dst = ring + op * kTileBytes;
+          auto chunk = [&](int row, int c) {
+            return *reinterpret_cast<const float4*>(src + row * 128 + (c >> 3) * kPanel + (((c & 7) ^ (row & 7)) << 4));
           };
-          float m = 0.f;
-          if (valid) {
+          if (x & 1) {
+            if (keys < kTileKeys) {
+              if (ok && r >= keys) {
+#pragma unroll 1
+                for (int c = 0; c < 16; ++c)
+                  *reinterpret_cast<uint4*>(src + r * 128 + (c >> 3) * kPanel + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+              }
+              ok = all_converters(ok);
+              if (!ok) break;
+            }
+            float4 hi = make_float4(0, 0, 0, 0), lo = make_float4(INFINITY, INFINITY, INFINITY, INFINITY);
 #pragma unroll
-            for (int c = 0; c < 16; ++c) m = finite_max(m, chunk(c));
-          }
+            for (int k = 0; k < 16; k += 2) {
+              const float4 v = chunk(row0 + k, quad), u = chunk(row0 + k + 1, quad);
+              hi = make_float4(max3_abs(hi.x, v.x, u.x), max3_abs(hi.y, v.y, u.y), max3_abs(hi.z, v.z, u.z), max3_abs(hi.w, v.w, u.w));
+              lo = make_float4(min3_abs(lo.x, v.x, u.x), min3_abs(lo.y, v.y, u.y), min3_abs(lo.z, v.z, u.z), min3_abs(lo.w, v.w, u.w));
+            }
+            if (lo.x == 0.f || lo.y == 0.f || lo.z == 0.f || lo.w == 0.f) {  // the least but zero
+              lo = make_float4(INFINITY, INFINITY, INFINITY, INFINITY);
+              const auto some = [](float l, float v) { return v != 0.f ? min3_abs(l, v, v) : l; };
+              if (hi.x != 0.f || hi.y != 0.f || hi.z != 0.f || hi.w != 0.f) {
+#pragma unroll 1
+                for (int k = 0; k < 16; ++k) {
+                  const float4 v = chunk(row0 + k, quad);
+                  lo = make_float4(some(lo.x, v.x), some(lo.y, v.y), some(lo.z, v.z), some(lo.w, v.w));
+                }
+              }
+            }
+            // biased exponents, 0 for zeros alone; of a dim of zeros the least is 255
+            const auto exponent = [](float v) { return max(__float_as_uint(v) >> 23, min(__float_as_uint(v), 1u)); };
+            uint32_t high = exponent(hi.x) | exponent(hi.y) << 8 | exponent(hi.z) << 16 | exponent(hi.w) << 24;
+            uint32_t low = exponent(lo.x) | exponent(lo.y) << 8 | exponent(lo.z) << 16 | exponent(lo.w) << 24;
+            high = __vmaxu4(high, __shfl_xor_sync(0xFFFFFFFFu, high, 16));
+            low = __vminu4(low, __shfl_xor_sync(0xFFFFFFFFu, low, 16));
+            if (lane < 16) {
+              reinterpret_cast<uint32_t*>(&dims_s[0][quad])[warp - 12] = high;
+              reinterpret_cast<uint32_t*>(&dims_s[1][quad])[warp - 12] = low;
+            }
+            ok = all_converters(ok);  // also orders dims_s
+            if (!ok) break;
+            const uint4 h = dims_s[0][quad];
+            high = __vmaxu4(__vmaxu4(h.x, h.y), __vmaxu4(h.z, h.w));
+            // (a dim with an infinity makes NaN of its sums: its scale only has to be a number)
+            const auto of = [](uint32_t high, int y) { return max(-100, min(127, static_cast<int>(high >> (8 * y) & 255u) - 127)); };
+            const float4 scale = make_float4(power_of_two(kTop - of(high, 0)), power_of_two(kTop - of(high, 1)),
+                                             power_of_two(kTop - of(high, 2)), power_of_two(kTop - of(high, 3)));
+            if (r < 16) {
+              // (a unit times its scale is 2^-kRaise)
+              const auto unit = [](float s) { return __uint_as_float(((254u - kRaise) << 23) - __float_as_uint(s)); };
+              unit_s[part][quad] = make_float4(unit(scale.x), unit(scale.y), unit(scale.z), unit(scale.w));
+              const uint4 l = dims_s[1][quad];
+              most = __vmaxu4(most, high);
+              least = __vminu4(least, __vminu4(__vminu4(l.x, l.y), __vminu4(l.z, l.w)));
+              uint32_t wide = 0;
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-          if (lane == 0) max_s[at & 1][warp - 12] = m;
-          ok = all_converters(ok);  // also orders max_s
-          if (!ok) break;
-          const float* ms = max_s[at & 1];
-          const int e = exponent_of(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])));
-          const float scale = power_of_two(kTop - e);
-          uint8_t* dst = ring + op * kTileBytes + r * 128;
+              for (int y = 0; y < 4; ++y) {
+                const int bound = of(most, y) - kTop - kRaise + 127;  // the largest unit
+                if (static_cast<int>(least >> (8 * y) & 255u) < bound) wide |= static_cast<uint32_t>(bound) << (8 * y);
+              }
+              reinterpret_cast<uint32_t*>(wide_s[tiles & 1])[quad] = wide;
+            }
+            part = part == 2 ? 0 : part + 1;
+#pragma unroll 1
+            for (int k0 = 0; k0 < 16; k0 += 8) {
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-            if (valid) split8(chunk(2 * c), chunk(2 * c + 1), scale, hi, lo);
-            *reinterpret_cast<uint4*>(dst + ((c ^ (r & 7)) << 4)) = hi;
-            *reinterpret_cast<uint4*>(dst + kPanel + ((c ^ (r & 7)) << 4)) = lo;
+              for (int k = 0; k < 8; ++k) {
+                uint2 a, b;
+                split4<true>(chunk(row0 + k0 + k, quad), scale, a, b);
+                uint8_t* to = dst + (row0 + k0 + k) * 128 + (((quad >> 1) ^ k) << 4) + (quad & 1) * 8;
+                *reinterpret_cast<uint2*>(to) = a;
+                *reinterpret_cast<uint2*>(to + kPanel) = b;
+              }
+            }
+            __syncwarp();  // unit_s and wide_s, before exp_full
+          } else {
+            const bool valid = r < keys;
+            float m = 0.f;
+            if (valid) {
+              float4 hi = make_float4(0, 0, 0, 0);
+#pragma unroll
+              for (int c = 0; c < 16; c += 2) {
+                const float4 v = chunk(r, c), u = chunk(r, c + 1);
+                hi = make_float4(max3_abs(hi.x, v.x, u.x), max3_abs(hi.y, v.y, u.y), max3_abs(hi.z, v.z, u.z), max3_abs(hi.w, v.w, u.w));
+              }
+              m = fmaxf(fmaxf(hi.x, hi.y), fmaxf(hi.z, hi.w));
+              if (!(m <= 3.402823466e38f)) {  // an infinity
+                m = 0.f;
+#pragma unroll 1
+                for (int c = 0; c < 16; ++c) m = finite_max(m, chunk(r, c));
+              }
+            }
+            const uint32_t bits = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m));
+            float* ms = max_s[(at >> 1) & 1];
+            if (lane == 0) ms[warp - 12] = __uint_as_float(bits);
+            ok = all_converters(ok);  // also orders max_s
+            if (!ok) break;
+            const int e = exponent_of(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])));
+            const float f = power_of_two(kTop - e);
+            const float4 scale = make_float4(f, f, f, f);
+            if (r == 0) exp_s[at & 7] = e;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              uint2 a[2] = {}, b[2] = {};
+              if (valid) {
+                split4<false>(chunk(r, 2 * c), scale, a[0], b[0]);
+                split4<false>(chunk(r, 2 * c + 1), scale, a[1], b[1]);
+              }
+              *reinterpret_cast<uint4*>(dst + r * 128 + ((c ^ (r & 7)) << 4)) = make_uint4(a[0].x, a[0].y, a[1].x, a[1].y);
+              *reinterpret_cast<uint4*>(dst + r * 128 + kPanel + ((c ^ (r & 7)) << 4)) = make_uint4(b[0].x, b[0].y, b[1].x, b[1].y);
+            }
           }
-          if (r == 0) {
-            exp_s[at & 7] = e;
-            mbar_arrive(&exp_full[at & 7]);
-          }
+          if (r == 0) mbar_arrive(&exp_full[at & 7]);
           fence_proxy_async();
           mbar_arrive(&kv_full[op]);
           mbar_arrive(&stage_empty[st]);
         }
+        tiles += w.count > 0;
       }
     } else if (warp == 10) {
       // -------------------------------------------------------------- scheduler
@@ -874,10 +996,13 @@ __global__ void __launch_bounds__(threads<T>, 1)
         uint8_t* dst = q_s + i * kTileBytes + r * 128;
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-          uint4 hi, lo;
-          split8(v[2 * c], v[2 * c + 1], power_of_two(kTop - exp_q), hi, lo);
-          *reinterpret_cast<uint4*>(dst + ((c ^ (r & 7)) << 4)) = hi;
-          *reinterpret_cast<uint4*>(dst + kPanel + ((c ^ (r & 7)) << 4)) = lo;
+          const float f = power_of_two(kTop - exp_q);
+          const float4 scale = make_float4(f, f, f, f);
+          uint2 hi[2], lo[2];
+          split4<false>(v[2 * c], scale, hi[0], lo[0]);
+          split4<false>(v[2 * c + 1], scale, hi[1], lo[1]);
+          *reinterpret_cast<uint4*>(dst + ((c ^ (r & 7)) << 4)) = make_uint4(hi[0].x, hi[0].y, hi[1].x, hi[1].y);
+          *reinterpret_cast<uint4*>(dst + kPanel + ((c ^ (r & 7)) << 4)) = make_uint4(lo[0].x, lo[0].y, lo[1].x, lo[1].y);
         }
         fence_proxy_async();
         mbar_arrive(&q_full);
@@ -888,15 +1013,22 @@ __global__ void __launch_bounds__(threads<T>, 1)
         // O of one key tile at a time is added up here, in registers: the tensor cores' accumulators cut off instead
         // of rounding, which over a long row would shrink it (by 5e-6 at 8192 keys). S is read by halves
         // to leave room for that.
-        float unit = 0.f;  // of O of the key tile before
-        int high_k = -126, high_v = -126;
-        const auto take = [&](float back) {
+        int high_k = -126;
+        const auto take = [&](int j, float back) {  // O of key tile j
+          const float4* units = unit_s[(ring_at / 2 + j) % 3];
 #pragma unroll
           for (int q = 0; q < D / 32; ++q) {
             uint32_t o[32];
             load_o<true>(o_addr + 32 * q, o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) acc[32 * q + e] = fmaf(__uint_as_float(o[e]), unit, acc[32 * q + e]) * back;
+            for (int e = 0; e < 32; e += 4) {
+              const float4 u = units[8 * q + e / 4];
+              float* a = acc + 32 * q + e;
+              a[0] = fmaf(__uint_as_float(o[e]), u.x, a[0]) * back;
+              a[1] = fmaf(__uint_as_float(o[e + 1]), u.y, a[1]) * back;
+              a[2] = fmaf(__uint_as_float(o[e + 2]), u.z, a[2]) * back;
+              a[3] = fmaf(__uint_as_float(o[e + 3]), u.w, a[3]) * back;
+            }
           }
         };
         for (int j = 0; j < n; ++j, ++step) {
@@ -928,10 +1060,9 @@ __global__ void __launch_bounds__(threads<T>, 1)
 #pragma unroll
               for (int q = 0; q < 4; ++q) mx[q] = max3(mx[q], __uint_as_float(s[k + q]), __uint_as_float(s[k + q + 4]));
           }
-          const int ki = ring_at + 2 * j, vi = ki + 1;
-          ok = wait_own(&exp_full[ki & 7], (ki >> 3) & 1, p.err) && wait_own(&exp_full[vi & 7], (vi >> 3) & 1, p.err);
+          const int ki = ring_at + 2 * j;
+          ok = wait_own(&exp_full[ki & 7], (ki >> 3) & 1, p.err);
           high_k = max(high_k, exp_s[ki & 7]);
-          high_v = max(high_v, exp_s[vi & 7]);
           const float factor = scale2 * power_of_two(max(-120, min(120, exp_q + exp_s[ki & 7] - 2 * kTop)));
           const float high = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * factor;
           if (j == 0) {
@@ -942,16 +1073,16 @@ __global__ void __launch_bounds__(threads<T>, 1)
             if (move) ref = high;
             total[0] = fma2(total[0], pair(back, back), 0);
             total[1] = fma2(total[1], pair(back, back), 0);
-            ok = ok && wait_own(&pv_done[i], (step - 1) & 1, p.err);
+            ok = ok && wait_own(&pv_done[i], (step - 1) & 1, p.err) &&
+                 wait_own(&exp_full[(ki - 1) & 7], ((ki - 1) >> 3) & 1, p.err);  // (its units; long there)
             if (!__all_sync(0xFFFFFFFFu, ok)) break;
             tc_fence_after();
-            take(back);
+            take(j - 1, back);
           }
-          unit = power_of_two(max(-126, exp_s[vi & 7] - kTop - kRaise));
           const uint64_t scale_pair = pair(factor, factor), nref = pair(-ref, -ref);
 #pragma unroll
-          for (int h = 1; h >= 0; --h) {  // the second half is still there
-            if (h == 0) load(0);
+          for (int h = 0; h < 2; ++h) {  // (P takes the place of the half of S that has been read)
+            load(h);
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
               uint32_t hi[16], lo[16];
@@ -966,18 +1097,34 @@ __global__ void __launch_bounds__(threads<T>, 1)
           mbar_arrive(&p_ready[i]);
         }
         if (n > 0) {
-          ok = ok && wait_own(&pv_done[i], (step - 1) & 1, p.err);
+          const int own = ring_at + 2 * n - 1, last = ring_at + 2 * count - 1;  // the item's last value tile: wide_s stands
+          ok = ok && wait_own(&pv_done[i], (step - 1) & 1, p.err) && wait_own(&exp_full[own & 7], (own >> 3) & 1, p.err);
           ok = __all_sync(0xFFFFFFFFu, ok);
           tc_fence_after();
-          take(1.f);
+          take(n - 1, 1.f);
+          ok = ok && wait_own(&exp_full[last & 7], (last >> 3) & 1, p.err);
+          ok = __all_sync(0xFFFFFFFFu, ok);
         }
-        float most = 0.f, ta, tb;
+        coarse = p.scale * power_of_two(max(-126, min(127, exp_q + high_k))) > kScoreRange;
+        if (n > 0 && sees > 0) {
+          const uint4* wide = wide_s[(tiles - 1) & 1];
+          const uint4 a = wide[0], b = wide[1], c = wide[2], d = wide[3];
+          if ((a.x | a.y | a.z | a.w | b.x | b.y | b.z | b.w | c.x | c.y | c.z | c.w | d.x | d.y | d.z | d.w) != 0) {
+            float ta, tb;
+            unpair(add2(total[0], total[1]), ta, tb);
+            const float sum = (ta + tb) * power_of_two(-kRaise);
+            const auto far = [&](uint32_t four, const float* acc) {
 #pragma unroll
-        for (int e = 0; e < D; ++e) most = fmaxf(most, fabsf(acc[e]));
-        unpair(add2(total[0], total[1]), ta, tb);
-        // (sums of zero too: both parts of a value far below its tile's largest are zero; tiles of zeros have none)
-        coarse = p.scale * power_of_two(max(-126, min(127, exp_q + high_k))) > kScoreRange ||
-                 (ta + tb > 0.f && high_v > kLeast && most < power_of_two(max(-126, high_v - kSumRange)));
+              for (int y = 0; y < 4; ++y)  // (a bound of 0 holds for none)
+                coarse = coarse || fabsf(acc[y]) < sum * __uint_as_float((four >> (8 * y) & 255u) << 23);
+            };
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint4 w = e == 0 ? a : e == 1 ? b : e == 2 ? c : d;
+              far(w.x, acc + 16 * e), far(w.y, acc + 16 * e + 4), far(w.z, acc + 16 * e + 8), far(w.w, acc + 16 * e + 12);
+            }
+          }
+        }
       } else {
         for (int j = 0; j < n; ++j, ++step) {
           ok = wait_own(&s_full[i], step & 1, p.err);

@@ -69,3 +69,64 @@ def test_huge_later_positions(cuda, what, big, m, n, see, dim):
         t[far:] = (t[far:].sign() if big == MAX else t[far:]) * big
     out = _call(torch, q, k, v)
     _held(out[:see], *attend(_d(q)[:see], _d(k)[:far], _d(v)[:far], float(np.float32(dim**-0.5))))
+
+
+def _check(torch, q, k, v):
+    _held(_call(torch, q, k, v), *attend(_d(q), _d(k), _d(v), float(np.float32(q.shape[2] ** -0.5))))
+
+
+SIZES = [(200, 200, 64), (64, 64, 64), (150, 1500, 64), (100, 100, 20), (20, 20, 64), (90, 90, 128), (4, 300, 64)]
+
+
+@pytest.mark.parametrize("big", [1e3, 1e6, 1e8, 1e10, 1e30])
+@pytest.mark.parametrize("m,n,dim", SIZES)
+def test_a_large_channel_of_values(cuda, big, m, n, dim):
+    """One dim of all values is far larger than the others: every element keeps FP32 accuracy, with the large dim also
+    of another size at later positions, and with one dim of zeros."""
+    import torch
+
+    q, k, v = _inputs(torch, m, n, dim, 32)
+    v[:, :, 3] *= big
+    _check(torch, q, k, v)
+    v[n - m // 2 :, :, 3] *= 1e4
+    v[:, 1, 7] = 0
+    _check(torch, q, k, v)
+
+
+@pytest.mark.parametrize("first,second", [(1e-12, 1.0), (1.0, 1e-12), (1.0, 1e9), (1e-30, 1e30)])
+@pytest.mark.parametrize("m,n,dim", SIZES)
+def test_values_of_two_sizes(cuda, first, second, m, n, dim):
+    """Positions of one size, then positions of another, in all dims and in every second one."""
+    import torch
+
+    for step in (1, 2):
+        q, k, v = _inputs(torch, m, n, dim, 33)
+        half = n - m // 2
+        v[:half, :, ::step] *= first
+        v[half:, :, ::step] *= second
+        _check(torch, q, k, v)
+
+
+@pytest.mark.parametrize("bits", [20, 26, 30, 40, 60, 100])
+@pytest.mark.parametrize("where", [5, 130])
+@pytest.mark.parametrize("m,n,dim", [(200, 200, 64), (150, 1500, 64), (100, 400, 32), (200, 200, 128), (4, 300, 64)])
+def test_a_huge_value_of_next_to_no_weight(cuda, bits, where, m, n, dim):
+    """A value of 2^bits whose weight is near 2^-bits: what it adds is as large as the rest, and its weight has to be
+    as exact as theirs."""
+    import torch
+
+    q, k, v = _inputs(torch, m, n, dim, 34)
+    k[where] = -bits * np.log(2) / dim**0.5
+    v[where] *= 2.0**bits
+    _check(torch, q, k, v)
+
+
+def test_a_value_far_below_the_others_of_its_dim(cuda):
+    """Rows that see nothing else than a key whose value is tiny in a few dims, also with zeros about."""
+    import torch
+
+    q, k, v = _inputs(torch, 150, 150, 64, 35)
+    for d, small in ((0, 1e-9), (1, 1e-15), (2, 1e-30), (3, 0.0)):
+        v[:30, :, d] *= small
+    v[60:90, :, 5] = 0
+    _check(torch, q, k, v)
