@@ -146,7 +146,8 @@ def set_weight_prefetch(enable: bool) -> bool:
 
 
 def device_error() -> int:
-    """Reads and clears the device error word (EFG_OK or EFG_ETIMEOUT / EFG_EINVAL)."""
+    """Reads and clears a device error word: what bounded waits recorded (EFG_ETIMEOUT, ...), else what
+    the paged calls' checks did (EFG_EINVAL, EFG_ENOMEM), else EFG_OK."""
     code = C.c_int(0)
     check(load().efg_device_error(C.byref(code)))
     return code.value

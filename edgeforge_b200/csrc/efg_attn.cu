@@ -122,6 +122,7 @@ int efg_attn_prompt(const efg_attn_prompt_args* args, void* stream) {
   p.head_dim = static_cast<int>(head_dim);
   p.scale = scale;
   p.err = dev->d_err;
+  p.checks = dev->d_checks;
   return efg::launch_attn(type, p, dev->sm_count, nullptr, 0, static_cast<cudaStream_t>(stream));
 }
 
@@ -192,6 +193,7 @@ int efg_attn_paged(const efg_attn_paged_args* args, void* stream) {
   p.head_dim = static_cast<int>(head_dim);
   p.scale = scale;
   p.err = dev->d_err;
+  p.checks = dev->d_checks;
   return efg::launch_attn(type, p, dev->sm_count, d_workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 

@@ -24,7 +24,7 @@ struct AttnParams {
   int page_shift;            // page_size = 1 << page_shift, or -1
   int heads, kv_heads, group, head_dim;
   float scale;
-  int* err;
+  int *err, *checks;         // for waits that give up, for offsets, lengths and pages that make no sense
 };
 
 __device__ __forceinline__ float attn_widen(float v) { return v; }
@@ -54,14 +54,14 @@ __device__ __forceinline__ bool chunk_of_seq(const AttnParams& p, int64_t s, Chu
   c.begin = p.cu[s];
   c.end = p.cu[s + 1];
   if (c.begin < 0 || c.end > p.n_rows || c.end < c.begin || (p.kv_len && c.end - c.begin > p.max_new)) {
-    record_error(p.err, EFG_EINVAL);
+    record_error(p.checks, EFG_EINVAL);
     return false;
   }
   c.kv_len = c.end - c.begin;
   if (p.kv_len) {
     c.kv_len = p.kv_len[s];
     if (c.kv_len < 0 || c.kv_len > p.max_pages * p.page_size) {
-      record_error(p.err, EFG_EINVAL);
+      record_error(p.checks, EFG_EINVAL);
       return false;
     }
   }
@@ -72,7 +72,7 @@ __device__ __forceinline__ bool chunk_of_seq(const AttnParams& p, int64_t s, Chu
 // bad one.
 __device__ __forceinline__ void check_offsets(const AttnParams& p) {
   for (int64_t s = threadIdx.x; s < p.n_seqs; s += blockDim.x)
-    if (p.cu[s] < 0 || p.cu[s + 1] < p.cu[s] || p.cu[s + 1] > p.n_rows) record_error(p.err, EFG_EINVAL);
+    if (p.cu[s] < 0 || p.cu[s + 1] < p.cu[s] || p.cu[s + 1] > p.n_rows) record_error(p.checks, EFG_EINVAL);
 }
 
 // Offset of the key (stride k_stride) of position j of the chunk's sequence, in rows of kv_heads *
@@ -84,7 +84,7 @@ __device__ __forceinline__ int64_t key_row(const AttnParams& p, const Chunk& c, 
   const uint32_t pi = p.page_shift >= 0 ? pos >> p.page_shift : pos / size;
   const int32_t page = p.table[static_cast<int64_t>(c.seq) * p.max_pages + pi];
   if (!page_ok(page, p.n_pages)) {
-    record_error(p.err, EFG_EINVAL);
+    record_error(p.checks, EFG_EINVAL);
     return -1;
   }
   return page * p.page_size + (pos - pi * size);
@@ -107,8 +107,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
-// Waits of a CTA for its own copies, MMAs and threads: an error that another CTA recorded (a bad page,
-// say) does not end them, only their own time limit.
+// Waits of a CTA for its own copies, MMAs and threads: an error that another CTA recorded does not end
+// them, only their own time limit.
 __device__ __forceinline__ bool wait_own(uint64_t* bar, uint32_t parity, int* err) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();

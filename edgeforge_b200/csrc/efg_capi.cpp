@@ -172,8 +172,12 @@ int efg_device_error(int* code) {
   DeviceInfo* dev = current_device();
   if (!dev) return EFG_ECUDA;
   EFG_TRY_CUDA(cudaDeviceSynchronize(), "device synchronize");
-  EFG_TRY_CUDA(cudaMemcpy(code, dev->d_err, sizeof(int), cudaMemcpyDeviceToHost), "read error word");
-  EFG_TRY_CUDA(cudaMemset(dev->d_err, 0, sizeof(int)), "clear error word");
+  for (int* word : {dev->d_err, dev->d_checks}) {
+    EFG_TRY_CUDA(cudaMemcpy(code, word, sizeof(int), cudaMemcpyDeviceToHost), "read error word");
+    if (*code == EFG_OK) continue;
+    EFG_TRY_CUDA(cudaMemset(word, 0, sizeof(int)), "clear error word");
+    break;
+  }
   return EFG_OK;
 }
 

@@ -96,12 +96,14 @@ DeviceInfo* current_device() {
   if (cuda_check(cudaDeviceGetAttribute(&smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev), "device attribute") !=
       EFG_OK)
     return nullptr;
+  constexpr size_t kErrorWordBytes = 256;  // two words, a line each
   int* err = nullptr;
-  if (cuda_check(cudaMalloc(&err, sizeof(int)), "error word allocation") != EFG_OK) return nullptr;
-  if (cuda_check(cudaMemset(err, 0, sizeof(int)), "error word init") != EFG_OK) return nullptr;
+  if (cuda_check(cudaMalloc(&err, kErrorWordBytes), "error word allocation") != EFG_OK) return nullptr;
+  if (cuda_check(cudaMemset(err, 0, kErrorWordBytes), "error word init") != EFG_OK) return nullptr;
   d.sm_count = sms;
   d.smem_optin = static_cast<size_t>(smem);
   d.d_err = err;
+  d.d_checks = err + kErrorWordBytes / sizeof(int) / 2;
   d.device = dev;
   return &d;
 }

@@ -1,5 +1,5 @@
 // efg_host.h - host-side helpers shared by the C-ABI implementation: the thread-local
-// error message, status helpers and per-device state (SM count, the device error word).
+// error message, status helpers and per-device state (SM count, the device error words).
 #pragma once
 
 #include <cstdarg>
@@ -25,7 +25,8 @@ struct DeviceInfo {
   int device = -1;
   int sm_count = 0;
   size_t smem_optin = 0;  // max dynamic shared memory per block (opt-in)
-  int* d_err = nullptr;   // device error word written by bounded waits
+  int* d_err = nullptr;   // device error word written by bounded waits: other kernels' waits end when it is set
+  int* d_checks = nullptr;  // what the paged calls' device-side checks found; no wait and no other call looks at it
 };
 
 // Thread-local default for MatvecArgs::pdl in the C-ABI calls (efg_set_weight_prefetch).
@@ -59,7 +60,7 @@ bool encode_u64_rows_map(CUtensorMap* m, const void* base, uint64_t rows, uint64
 bool encode_heads_map(CUtensorMap* m, int type, const void* base, uint64_t dim, uint64_t heads, uint64_t rows,
                       uint64_t row_stride, uint32_t box_heads, uint32_t box_rows);
 
-// State of the current device, created on first use (allocates the error word).
+// State of the current device, created on first use (allocates the error words).
 // Returns nullptr and records an error if the device cannot be queried.
 DeviceInfo* current_device();
 

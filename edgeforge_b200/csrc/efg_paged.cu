@@ -22,7 +22,7 @@ struct PlanParams {
   int32_t *slots, *positions, *cu, *kv_len, *taken;
   const int32_t *cached, *fresh, *free;
   int64_t max_pages, n_rows, n_seqs, n_free, n_pages, page_size, rows_per_cta;
-  int* err;
+  int* checks;
 };
 
 constexpr int kPlanThreads = 512;
@@ -105,11 +105,11 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanParam
       have_s[x] = static_cast<int32_t>(n[i].have);
       cached_s[x] = cached[i];
       if (lead && s < p.n_seqs) {
-        if (!served) record_error(p.err, n[i].valid ? EFG_ENOMEM : EFG_EINVAL);
+        if (!served) record_error(p.checks, n[i].valid ? EFG_ENOMEM : EFG_EINVAL);
         p.cu[s] = static_cast<int32_t>(min(at.rows, p.n_rows));
         p.kv_len[s] = served ? cached[i] + fresh[i] : 0;
         if (s == p.n_seqs - 1) {
-          if (at.rows + n[i].rows > p.n_rows) record_error(p.err, EFG_EINVAL);
+          if (at.rows + n[i].rows > p.n_rows) record_error(p.checks, EFG_EINVAL);
           p.cu[p.n_seqs] = static_cast<int32_t>(min(at.rows + n[i].rows, p.n_rows));
         }
       }
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanParam
           slot = static_cast<int32_t>(page * p.page_size + off);
           pos = static_cast<int32_t>(at_pos);
         } else {
-          record_error(p.err, EFG_EINVAL);
+          record_error(p.checks, EFG_EINVAL);
         }
         if (!old && off == 0) *entry = page;
       }
@@ -174,7 +174,7 @@ struct StoreParams {
   const float *cos, *sin;  // null: no rotation
   int64_t n_slots, max_pos;
   int heads, kv_heads, head_dim;
-  int* err;
+  int* checks;
 };
 
 __device__ __forceinline__ float widen(float v) { return v; }
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(256) page_store_kernel(const StoreParams p) {
   const bool is_q = head < qh, is_k = !is_q && head < qh + p.kv_heads;
   if (pos < 0 || (!is_q && slot < 0)) return;  // a padding row: everything of it stays as it was
   if (slot >= p.n_slots || pos >= p.max_pos) {
-    record_error(p.err, EFG_EINVAL);
+    record_error(p.checks, EFG_EINVAL);
     return;
   }
   const int kvh = head - qh - (is_k ? 0 : p.kv_heads);
@@ -325,7 +325,7 @@ int efg_page_plan(const efg_page_plan_args* args, void* stream) {
   p.n_free = static_cast<int64_t>(n_free);
   p.n_pages = static_cast<int64_t>(n_pages);
   p.page_size = static_cast<int64_t>(page_size);
-  p.err = dev->d_err;
+  p.checks = dev->d_checks;
   const size_t ctas = std::max<size_t>(1, std::min<size_t>(dev->sm_count, (n_rows + 511) / 512));
   p.rows_per_cta = static_cast<int64_t>((n_rows + ctas - 1) / ctas);
   return efg::launch_chained(efg::page_plan_kernel, dim3(static_cast<unsigned>(ctas)), efg::kPlanThreads, p,
@@ -389,7 +389,7 @@ int efg_page_store(const efg_page_store_args* args, void* stream) {
   p.heads = static_cast<int>(heads);
   p.kv_heads = static_cast<int>(kv_heads);
   p.head_dim = static_cast<int>(head_dim);
-  p.err = dev->d_err;
+  p.checks = dev->d_checks;
   const bool wide = head_dim % 8 == 0 && q_stride % 4 == 0 && k_stride % 4 == 0 && v_stride % 4 == 0 &&
                     efg::aligned(d_q, 4 * es) && efg::aligned(d_k, 4 * es) && efg::aligned(d_v, 4 * es) &&
                     efg::aligned(d_q_out, 4 * co) && efg::aligned(d_k_cache, 4 * co) &&

@@ -22,7 +22,8 @@
  *    A matrix is row-major [rows][cols] with rows packed back to back, exactly as
  *    stored in an .efq file (include/ef/qfile.h:1-21). cols must be a multiple of 32.
  *  - Device-side waits are bounded: a kernel that gives up records EFG_ETIMEOUT in a
- *    per-device error word, read (and cleared) with efg_device_error().
+ *    per-device error word, read (and cleared) with efg_device_error(). What the paged calls
+ *    find in lengths, pages and slots goes to a second word, read there too.
  */
 #ifndef EFG_H
 #define EFG_H
@@ -61,9 +62,11 @@ const char* efg_last_error(void);
 /* Name of a status code ("EFG_OK", "EFG_EINVAL", ...). */
 const char* efg_status_string(int status);
 
-/* Reads and clears the error word that device-side bounded waits (EFG_ETIMEOUT) and the
- * device-side checks of the paged calls (EFG_EINVAL, EFG_ENOMEM) write on the current device
- * (synchronises the device first). *code receives EFG_OK or the first such code. */
+/* Reads and clears one of the current device's two error words (synchronises the device first):
+ * the one that bounded waits and the decoder write (EFG_ETIMEOUT, ...), and when that is clear the
+ * one that the device-side checks of the paged calls write (EFG_EINVAL, EFG_ENOMEM). *code receives
+ * the first code that was written there, or EFG_OK when both words are clear. While the first word is
+ * set, kernels that wait give up early; the second one has no effect on any call. */
 int efg_device_error(int* code);
 
 /* Early weight streaming for the matvec calls made afterwards on this thread (default
