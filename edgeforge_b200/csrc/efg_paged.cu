@@ -359,7 +359,10 @@ int efg_page_store(const efg_page_store_args* args, void* stream) {
   auto meets = [&](const void* out, size_t n_out, bool own_q) {
     return (!own_q && efg::overlap(out, n_out, d_q, n_rows, q_stride, q_row, es)) ||
            efg::overlap(out, n_out, d_k, n_rows, k_stride, kv_row, es) ||
-           efg::overlap(out, n_out, d_v, n_rows, v_stride, kv_row, es);
+           efg::overlap(out, n_out, d_v, n_rows, v_stride, kv_row, es) ||
+           efg::overlap(out, n_out, d_slots, 1, 0, n_rows, 4) || efg::overlap(out, n_out, d_positions, 1, 0, n_rows, 4) ||
+           efg::overlap(out, n_out, d_cos, 1, 0, max_pos * (head_dim / 2), 4) ||
+           efg::overlap(out, n_out, d_sin, 1, 0, max_pos * (head_dim / 2), 4);
   };
   const size_t cache = n_slots * kv_row * co;
   if (meets(d_q_out, n_rows * q_row * co, in_place) || meets(d_k_cache, cache, false) || meets(d_v_cache, cache, false))
