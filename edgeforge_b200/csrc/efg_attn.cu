@@ -101,7 +101,7 @@ int efg_attn_prompt(const efg_attn_prompt_args* args, void* stream) {
   const size_t es = type == EFG_F32 ? 4 : 2, n_out = n_rows * heads * head_dim * es, row = kv_heads * head_dim;
   if (efg::overlap(d_out, n_out, d_q, n_rows, q_stride, heads * head_dim, es) ||
       efg::overlap(d_out, n_out, d_k, n_rows, k_stride, row, es) ||
-      efg::overlap(d_out, n_out, d_v, n_rows, v_stride, row, es))
+      efg::overlap(d_out, n_out, d_v, n_rows, v_stride, row, es) || efg::overlap(d_out, n_out, d_cu, 1, 0, n_seqs + 1, 4))
     return fail(EFG_EINVAL, "attn_prompt: out overlaps an input");
   efg::DeviceInfo* dev = efg::current_device();
   if (!dev) return EFG_ECUDA;
@@ -164,10 +164,16 @@ int efg_attn_paged(const efg_attn_paged_args* args, void* stream) {
       (max_pages && !d_block_table))
     return fail(EFG_EINVAL, "attn_paged: null pointer");
   const size_t es = type == EFG_F32 ? 4 : 2, n_out = n_rows * heads * head_dim * es, row = kv_heads * head_dim;
-  if (efg::overlap(d_out, n_out, d_q, n_rows, q_stride, heads * head_dim, es) ||
-      efg::overlap(d_out, n_out, d_k_cache, n_pages * page_size, row, row, es) ||
-      efg::overlap(d_out, n_out, d_v_cache, n_pages * page_size, row, row, es))
-    return fail(EFG_EINVAL, "attn_paged: out overlaps an input");
+  auto meets = [&](const void* to, size_t n) {
+    return efg::overlap(to, n, d_q, n_rows, q_stride, heads * head_dim, es) ||
+           efg::overlap(to, n, d_k_cache, n_pages * page_size, row, row, es) ||
+           efg::overlap(to, n, d_v_cache, n_pages * page_size, row, row, es) ||
+           efg::overlap(to, n, d_block_table, n_seqs, max_pages, max_pages, 4) ||
+           efg::overlap(to, n, d_cu, 1, 0, n_seqs + 1, 4) || efg::overlap(to, n, d_kv_len, 1, 0, n_seqs, 4);
+  };
+  if (meets(d_out, n_out)) return fail(EFG_EINVAL, "attn_paged: out overlaps an input");
+  if (meets(d_workspace, workspace_bytes) || efg::overlap(d_workspace, workspace_bytes, d_out, 1, 0, n_out, 1))
+    return fail(EFG_EINVAL, "attn_paged: the workspace overlaps out or an input");
   efg::DeviceInfo* dev = efg::current_device();
   if (!dev) return EFG_ECUDA;
   efg::AttnParams p{};

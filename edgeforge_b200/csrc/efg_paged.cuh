@@ -74,7 +74,7 @@ EFG_HD int64_t find_sequence(const int32_t* cu, int64_t n_seqs, int64_t row) {
 // Whether `out` (n_out bytes) and n_rows rows of `in` (`row` of `stride` elements of es bytes each) overlap.
 inline bool overlap(const void* out, size_t n_out, const void* in, size_t n_rows, size_t stride, size_t row, size_t es) {
   const uintptr_t a = reinterpret_cast<uintptr_t>(out), b = reinterpret_cast<uintptr_t>(in);
-  return out && in && n_out && n_rows && a < b + ((n_rows - 1) * stride + row) * es && b < a + n_out;
+  return out && in && n_out && n_rows && row && a < b + ((n_rows - 1) * stride + row) * es && b < a + n_out;
 }
 
 }  // namespace efg

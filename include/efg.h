@@ -386,7 +386,8 @@ int efg_attn_prompt(const efg_attn_prompt_args* args, void* stream);
  * last position is never used. Types as efg_attn_prompt, the caches of `type` too.
  * Long sequences with few new tokens are cut into parts that meet in d_workspace (16-byte aligned
  * device memory of at least efg_attn_paged_workspace bytes for the same sizes, contents of no
- * account before and after; NULL when that is 0). */
+ * account before and after; NULL when that is 0). out and the workspace overlap neither an input nor each
+ * other (EFG_EINVAL). */
 typedef struct {
   int type;
   float scale;

@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import pytest
 
-from edgeforge_b200._lib import PAGE_STORE
+from edgeforge_b200._lib import ATTN_PAGED, ATTN_PROMPT, PAGE_STORE
 
 FAR = 2**24  # no two arrays of these calls reach each other at this distance
 
@@ -50,3 +50,50 @@ def test_store(efg_lib, out, read):
     assert _refused(*args, **{read: f[out] - STORE_BYTES[read] + 4})
     assert not _refused(*args, **{read: f[out] + STORE_BYTES[out]})
     assert not _refused(*args, **{read: f[out] - STORE_BYTES[read]})
+
+
+@pytest.mark.parametrize("at,hits", [(0, True), (-5 * 512 * 2 + 2, True), (3 * 4, False), (8, True)])
+def test_prompt(efg_lib, at, hits):
+    lib = efg_lib.load()
+    f = dict(type=2, scale=0.125, q_stride=512, k_stride=128, v_stride=128, n_seqs=2, n_rows=5, heads=8, kv_heads=2,
+             head_dim=64, **_spread(("out", "q", "k", "v", "cu")))
+    args = lib, lib.efg_attn_prompt, ATTN_PROMPT, f
+    assert not _refused(*args)
+    assert _refused(*args, out=f["cu"] + at) == hits
+
+
+PAGED = ("out", "q", "k_cache", "v_cache", "block_table", "cu", "kv_len", "workspace")
+
+
+def _paged_fields():
+    return dict(type=2, scale=0.125, q_stride=512, n_pages=16, page_size=16, max_pages=16, n_seqs=3, n_rows=5, max_new=5,
+                heads=8, kv_heads=2, head_dim=64, workspace_bytes=2**20, **_spread(PAGED))
+
+
+@pytest.mark.parametrize("read,size", [("block_table", 3 * 16 * 4), ("cu", 16), ("kv_len", 12)])
+def test_paged(efg_lib, read, size):
+    lib = efg_lib.load()
+    f = _paged_fields()
+    args = lib, lib.efg_attn_paged, ATTN_PAGED, f
+    n_out = 5 * 512 * 2
+    assert not _refused(*args)
+    assert _refused(*args, out=f[read])
+    assert _refused(*args, out=f[read] + size - 2)
+    assert _refused(*args, out=f[read] - n_out + 2)
+    assert not _refused(*args, out=f[read] + size)
+    assert not _refused(*args, out=f[read] - n_out)
+
+
+@pytest.mark.parametrize("other,size", [("out", 5 * 512 * 2), ("q", 5 * 512 * 2), ("k_cache", 256 * 128 * 2),
+                                        ("v_cache", 256 * 128 * 2), ("block_table", 3 * 16 * 4), ("cu", 16), ("kv_len", 12)])
+def test_workspace(efg_lib, other, size):
+    lib = efg_lib.load()
+    f = _paged_fields()
+    args = lib, lib.efg_attn_paged, ATTN_PAGED, f
+    assert _refused(*args, workspace=f[other])
+    assert _refused(*args, workspace=f[other] - 2**20 + 4)
+    assert _refused(*args, **{other: f["workspace"] + 2**20 - 4})
+    assert not _refused(*args, **{other: f["workspace"] + 2**20})
+    assert not _refused(*args, workspace=f[other] - 2**20)
+    assert not _refused(*args, **{other: f["workspace"] - size})
+    assert not _refused(*args, workspace=0, workspace_bytes=0)
