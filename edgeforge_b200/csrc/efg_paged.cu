@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanParam
     }
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
-      n[i] = seq_need(cached[i], fresh[i], p.page_size, p.max_pages);
+      n[i] = seq_need_held(cached[i], fresh[i], p.page_size, p.max_pages);
       mine = mine + Pair64{n[i].rows, n[i].need};
     }
     Pair64 total;

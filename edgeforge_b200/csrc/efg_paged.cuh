@@ -41,6 +41,14 @@ EFG_HD SeqNeed seq_need(int32_t cached, int32_t fresh, int64_t page_size, int64_
   return n;
 }
 
+// The same for sequences whose lengths and positions other kernels hold in 32 signed bits (with room for a tile).
+constexpr int64_t kMaxPositions = 0x7FFFFF00;
+EFG_HD SeqNeed seq_need_held(int32_t cached, int32_t fresh, int64_t page_size, int64_t max_pages) {
+  SeqNeed n = seq_need(cached, fresh, page_size, max_pages);
+  if (static_cast<int64_t>(cached) + fresh > kMaxPositions) n = SeqNeed{n.rows, 0, 0, false};
+  return n;
+}
+
 // Fresh pages are handed out in sequence order. A sequence is served when its own pages end
 // inside the free list; once one is not, none after it that needs a page is (`first` counts
 // the needs of every sequence before it, served or not).

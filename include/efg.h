@@ -313,7 +313,7 @@ int efg_lm_head_argmax_sharded(int qtype, float* d_logits_shard, int32_t* d_toke
  * padding rows); d_kv_len[s] = cached + new; *d_taken = how many pages of d_free were taken.
  * A sequence whose pages do not fit in the free list is not served, nor is any after it that
  * needs a page (EFG_ENOMEM for efg_device_error); one with negative lengths or more positions
- * than max_pages hold is not served either (EFG_EINVAL). The rows of a sequence that is not
+ * than max_pages hold, or than 2^31 - 256, is not served either (EFG_EINVAL). The rows of a sequence that is not
  * served get slot and position -1 and its kv_len is 0. More new tokens than n_rows: the rows
  * behind n_rows are dropped and d_cu stops at n_rows (EFG_EINVAL). No output may overlap an input
  * or another output (EFG_EINVAL; kv_len is not cached updated in place). */
