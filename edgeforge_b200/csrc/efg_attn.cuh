@@ -190,34 +190,58 @@ __device__ bool find_tile(const AttnParams& p, int64_t want, int64_t mul, int64_
   return false;
 }
 
-// One warp computes one row of one query head: 32 keys at a time, a lane per key for the scores
-// (running maximum and sum of the softmax in FP32), then a lane per dim for the values. A key
-// behind the row's last visible one is never read, so what lies there (stale, infinite or NaN)
-// cannot reach the row. head_dim <= 256; lane l holds dims l, l + 32, .. of the query.
-template <typename T>
-__device__ __noinline__ void attend_row(const AttnParams& p, const Chunk& c, int64_t row, int head) {
-  const int lane = threadIdx.x & 31, D = p.head_dim, kvh = head / p.group;
+// One warp computes one row of one query head: 32 keys at a time, 8 lanes a key for the scores, running maximum and sum
+// of the softmax in FP32, then a lane per dim for the values. Bound by the latency of its loads, so they are
+// unconditional (of a place that is valid in any case) and several keys' are in flight. A key behind the row's last
+// visible one is never read, so what lies there (stale, infinite or NaN) cannot reach the row. head_dim <= 8 N; of a
+// key's lanes, lane l holds dims l, l + 8, .. of the query.
+template <typename T, int N>
+__device__ __forceinline__ void attend_row_of(const AttnParams& p, const Chunk& c, int64_t row, int head) {
+  // keys whose loads are in flight: groups of four, and values
+  constexpr int NV = (N + 3) / 4, kGroups = N <= 16 ? 2 : 1, kAhead = N <= 8 ? 8 : N <= 16 ? 4 : 2;
+  const int lane = threadIdx.x & 31, D = p.head_dim, kvh = head / p.group, part = lane & 7;
   const int32_t count = seen_by(c, static_cast<int32_t>(row));
+  const int64_t k_stride = p.k_stride, v_stride = p.v_stride;
   const T* q = static_cast<const T*>(p.q) + row * p.q_stride + static_cast<int64_t>(head) * D;
-  float qv[8];
+  const T* keys = static_cast<const T*>(p.k) + static_cast<int64_t>(kvh) * D;
+  const T* values = static_cast<const T*>(p.v) + static_cast<int64_t>(kvh) * D;
+  float qv[N];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) qv[i] = lane + 32 * i < D ? attn_widen(q[lane + 32 * i]) : 0.f;
+  for (int i = 0; i < N; ++i) qv[i] = part + 8 * i < D ? attn_widen(q[part + 8 * i]) : 0.f;
   const float to_base2 = p.scale * 1.4426950408889634f;
-  float acc[8] = {}, top = -INFINITY, sum = 0.f;
+  float acc[NV] = {}, top = -INFINITY, sum = 0.f;
   for (int32_t j0 = 0; j0 < count; j0 += 32) {
-    int64_t kr = -1;
-    float sc = -INFINITY, dot = 0.f;
+    int64_t kr = -1;  // of key j0 + lane
     if (j0 + lane < count) kr = key_row(p, c, j0 + lane);
-    const T* k = static_cast<const T*>(p.k) + max(kr, int64_t{0}) * p.k_stride + static_cast<int64_t>(kvh) * D;
+    const uint32_t good = __ballot_sync(0xFFFFFFFFu, kr >= 0);
+    if (good == 0) continue;
+    const int64_t some = __shfl_sync(0xFFFFFFFFu, kr, __ffs(good) - 1);
+    if (kr < 0) kr = some;
+    const int n = min(32, count - j0);
+    float dot = 0.f;
+#pragma unroll 1
+    for (int b = 0; 4 * b < n; b += kGroups) {  // groups b ..: keys 4 b ..
+      T x[kGroups][N];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int n = min(32, D - 32 * i);
-      for (int d = 0; d < n; ++d) {
-        const float x = __shfl_sync(0xFFFFFFFFu, qv[i], d);
-        if (kr >= 0) dot = fmaf(x, attn_widen(k[32 * i + d]), dot);
+      for (int y = 0; y < kGroups; ++y) {
+        const T* k = keys + __shfl_sync(0xFFFFFFFFu, kr, 4 * (b + y) + (lane >> 3)) * k_stride;
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[y][i] = k[min(part + 8 * i, D - 1)];
+      }
+#pragma unroll
+      for (int y = 0; y < kGroups; ++y) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (part + 8 * i < D) s = fmaf(qv[i], attn_widen(x[y][i]), s);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+        s = __shfl_sync(0xFFFFFFFFu, s, 8 * (lane & 3));
+        if (lane >> 2 == b + y) dot = s;
       }
     }
-    if (kr >= 0) sc = dot * to_base2;
+    const bool valid = good >> lane & 1;
+    const float sc = valid ? dot * to_base2 : -INFINITY;
     float m = sc;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -227,28 +251,45 @@ __device__ __noinline__ void attend_row(const AttnParams& p, const Chunk& c, int
     const float high = (m != m || top != top) ? NAN : fmaxf(top, m);
     // nothing visible so far (every score -inf): keep the sums at zero
     const float ref = high == -INFINITY ? 0.f : high;
-    const float w = kr >= 0 ? exp2f(sc - ref) : 0.f;
+    const float w = valid ? exp2f(sc - ref) : 0.f;
     const float back = exp2f(top - ref);
     sum = sum * back + warp_sum(w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] *= back;
+    for (int i = 0; i < NV; ++i) acc[i] *= back;
     top = high;
-    const int n = min(32, count - j0);
-    for (int t = 0; t < n; ++t) {
-      const int64_t vr = __shfl_sync(0xFFFFFFFFu, kr, t);
-      const float wt = __shfl_sync(0xFFFFFFFFu, w, t);
-      if (vr < 0) continue;
-      const T* v = static_cast<const T*>(p.v) + vr * p.v_stride + static_cast<int64_t>(kvh) * D;
+#pragma unroll 1
+    for (int t = 0; t < n; t += kAhead) {
+      T x[kAhead][NV];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (lane + 32 * i < D) acc[i] = fmaf(wt, attn_widen(v[lane + 32 * i]), acc[i]);
+      for (int y = 0; y < kAhead; ++y) {
+        const T* v = values + __shfl_sync(0xFFFFFFFFu, kr, t + y) * v_stride;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) x[y][i] = v[min(lane + 32 * i, D - 1)];
+      }
+#pragma unroll
+      for (int y = 0; y < kAhead; ++y) {
+        const float wt = __shfl_sync(0xFFFFFFFFu, w, t + y);
+        if (good >> (t + y) & 1) {
+#pragma unroll
+          for (int i = 0; i < NV; ++i) acc[i] = fmaf(wt, attn_widen(x[y][i]), acc[i]);
+        }
+      }
     }
   }
   T* out = static_cast<T*>(p.out) + (row * p.heads + head) * D;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing is zeros
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < NV; ++i)
     if (lane + 32 * i < D) out[lane + 32 * i] = attn_narrow<T>(acc[i] * inv);
+}
+template <typename T>
+__device__ __noinline__ void attend_row(const AttnParams& p, const Chunk& c, int64_t row, int head) {
+  if (p.head_dim <= 64)
+    attend_row_of<T, 8>(p, c, row, head);
+  else if (p.head_dim <= 128)
+    attend_row_of<T, 16>(p, c, row, head);
+  else
+    attend_row_of<T, 32>(p, c, row, head);
 }
 
 // Whether a non-finite value of the KV head lies at a position that the row does not see, but
