@@ -108,14 +108,16 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 // Waits of a CTA for its own copies, MMAs and threads: an error that another CTA recorded does not end
-// them, only their own time limit.
-__device__ __forceinline__ bool wait_own(uint64_t* bar, uint32_t parity, int* err) {
+// them, only their own time limit, and not before *until (shared memory): a warp that computes rows of a
+// long sequence alone (attend_row) may need longer, and moves that on.
+__device__ __forceinline__ bool wait_own(uint64_t* bar, uint32_t parity, int* err, const uint64_t* until) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
 #pragma unroll 1
   for (uint32_t i = 0;; ++i) {
     if (mbar_try_wait_sleep(bar, parity, 2000u)) return true;
-    if ((i & 15u) == 15u && globaltimer_ns() - t0 > kWaitTimeoutNs) {
+    if ((i & 15u) == 15u && globaltimer_ns() - t0 > kWaitTimeoutNs &&
+        globaltimer_ns() > *reinterpret_cast<const volatile uint64_t*>(until)) {
       record_error(err, EFG_ETIMEOUT);
       return false;
     }
@@ -190,27 +192,24 @@ __device__ bool find_tile(const AttnParams& p, int64_t want, int64_t mul, int64_
   return false;
 }
 
-// One warp computes one row of one query head: 32 keys at a time, 8 lanes a key for the scores, running maximum and sum
-// of the softmax in FP32, then a lane per dim for the values. Bound by the latency of its loads, so they are
-// unconditional (of a place that is valid in any case) and several keys' are in flight. A key behind the row's last
-// visible one is never read, so what lies there (stale, infinite or NaN) cannot reach the row. head_dim <= 8 N; of a
-// key's lanes, lane l holds dims l, l + 8, .. of the query.
+// One warp computes one row of one query head: 32 keys at a time, a lane per dim of keys and values, running maximum and
+// sum of the softmax in FP32. Bound by the latency of its loads, so they are unconditional (of a place that is valid in
+// any case) and kAhead keys' are in flight; more of them, or 8 lanes a key, would take registers that the kernels
+// that call this have none left of (64 FP32 rows of a decode step: 44.9 -> 56.6 us). A key behind the row's last visible
+// one is never read, so what lies there (stale, infinite or NaN) cannot reach the row. head_dim <= 32 N; lane l holds
+// dims l, l + 32, .. of the query.
 template <typename T, int N>
-__device__ __forceinline__ void attend_row_of(const AttnParams& p, const Chunk& c, int64_t row, int head) {
-  // keys whose loads are in flight: groups of four, and values
-  constexpr int NV = (N + 3) / 4, kGroups = N <= 16 ? 2 : 1, kAhead = N <= 8 ? 8 : N <= 16 ? 4 : 2;
-  const int lane = threadIdx.x & 31, D = p.head_dim, kvh = head / p.group, part = lane & 7;
+__device__ __forceinline__ void attend_row_of(const AttnParams& p, const Chunk& c, int64_t row, int head, uint64_t* until) {
+  constexpr int kAhead = N == 8 ? 2 : 16 / N;
+  const int lane = threadIdx.x & 31, D = p.head_dim, kvh = head / p.group;
   const int32_t count = seen_by(c, static_cast<int32_t>(row));
-  const int64_t k_stride = p.k_stride, v_stride = p.v_stride;
   const T* q = static_cast<const T*>(p.q) + row * p.q_stride + static_cast<int64_t>(head) * D;
-  const T* keys = static_cast<const T*>(p.k) + static_cast<int64_t>(kvh) * D;
-  const T* values = static_cast<const T*>(p.v) + static_cast<int64_t>(kvh) * D;
-  float qv[N];
+  float qv[N], acc[N] = {}, top = -INFINITY, sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) qv[i] = part + 8 * i < D ? attn_widen(q[part + 8 * i]) : 0.f;
+  for (int i = 0; i < N; ++i) qv[i] = lane + 32 * i < D ? attn_widen(q[lane + 32 * i]) : 0.f;
   const float to_base2 = p.scale * 1.4426950408889634f;
-  float acc[NV] = {}, top = -INFINITY, sum = 0.f;
   for (int32_t j0 = 0; j0 < count; j0 += 32) {
+    if (until && lane == 0) *reinterpret_cast<volatile uint64_t*>(until) = globaltimer_ns() + kWaitTimeoutNs;
     int64_t kr = -1;  // of key j0 + lane
     if (j0 + lane < count) kr = key_row(p, c, j0 + lane);
     const uint32_t good = __ballot_sync(0xFFFFFFFFu, kr >= 0);
@@ -218,26 +217,27 @@ __device__ __forceinline__ void attend_row_of(const AttnParams& p, const Chunk& 
     const int64_t some = __shfl_sync(0xFFFFFFFFu, kr, __ffs(good) - 1);
     if (kr < 0) kr = some;
     const int n = min(32, count - j0);
+    const auto load = [&](const void* base, int64_t stride, int t, T (&x)[kAhead][N]) {  // keys t .., this lane's dims
+#pragma unroll
+      for (int y = 0; y < kAhead; ++y) {
+        const T* at = static_cast<const T*>(base) + __shfl_sync(0xFFFFFFFFu, kr, t + y) * stride + static_cast<int64_t>(kvh) * D;
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[y][i] = at[min(lane + 32 * i, D - 1)];
+      }
+    };
     float dot = 0.f;
 #pragma unroll 1
-    for (int b = 0; 4 * b < n; b += kGroups) {  // groups b ..: keys 4 b ..
-      T x[kGroups][N];
+    for (int t = 0; t < n; t += kAhead) {
+      T x[kAhead][N];
+      load(p.k, p.k_stride, t, x);
 #pragma unroll
-      for (int y = 0; y < kGroups; ++y) {
-        const T* k = keys + __shfl_sync(0xFFFFFFFFu, kr, 4 * (b + y) + (lane >> 3)) * k_stride;
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[y][i] = k[min(part + 8 * i, D - 1)];
-      }
-#pragma unroll
-      for (int y = 0; y < kGroups; ++y) {
+      for (int y = 0; y < kAhead; ++y) {
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i)
-          if (part + 8 * i < D) s = fmaf(qv[i], attn_widen(x[y][i]), s);
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-        s = __shfl_sync(0xFFFFFFFFu, s, 8 * (lane & 3));
-        if (lane >> 2 == b + y) dot = s;
+          if (lane + 32 * i < D) s = fmaf(qv[i], attn_widen(x[y][i]), s);
+        s = warp_sum(s);
+        if (lane == t + y) dot = s;
       }
     }
     const bool valid = good >> lane & 1;
@@ -255,23 +255,18 @@ __device__ __forceinline__ void attend_row_of(const AttnParams& p, const Chunk& 
     const float back = exp2f(top - ref);
     sum = sum * back + warp_sum(w);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) acc[i] *= back;
+    for (int i = 0; i < N; ++i) acc[i] *= back;
     top = high;
 #pragma unroll 1
     for (int t = 0; t < n; t += kAhead) {
-      T x[kAhead][NV];
-#pragma unroll
-      for (int y = 0; y < kAhead; ++y) {
-        const T* v = values + __shfl_sync(0xFFFFFFFFu, kr, t + y) * v_stride;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) x[y][i] = v[min(lane + 32 * i, D - 1)];
-      }
+      T x[kAhead][N];
+      load(p.v, p.v_stride, t, x);
 #pragma unroll
       for (int y = 0; y < kAhead; ++y) {
         const float wt = __shfl_sync(0xFFFFFFFFu, w, t + y);
         if (good >> (t + y) & 1) {
 #pragma unroll
-          for (int i = 0; i < NV; ++i) acc[i] = fmaf(wt, attn_widen(x[y][i]), acc[i]);
+          for (int i = 0; i < N; ++i) acc[i] = fmaf(wt, attn_widen(x[y][i]), acc[i]);
         }
       }
     }
@@ -279,17 +274,18 @@ __device__ __forceinline__ void attend_row_of(const AttnParams& p, const Chunk& 
   T* out = static_cast<T*>(p.out) + (row * p.heads + head) * D;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing is zeros
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < N; ++i)
     if (lane + 32 * i < D) out[lane + 32 * i] = attn_narrow<T>(acc[i] * inv);
 }
+// The same for any head size; *until (null: none) is moved on for the waits of the CTA's other warps (wait_own).
 template <typename T>
-__device__ __noinline__ void attend_row(const AttnParams& p, const Chunk& c, int64_t row, int head) {
+__device__ __noinline__ void attend_row(const AttnParams& p, const Chunk& c, int64_t row, int head, uint64_t* until = nullptr) {
   if (p.head_dim <= 64)
-    attend_row_of<T, 8>(p, c, row, head);
+    attend_row_of<T, 2>(p, c, row, head, until);
   else if (p.head_dim <= 128)
-    attend_row_of<T, 16>(p, c, row, head);
+    attend_row_of<T, 4>(p, c, row, head, until);
   else
-    attend_row_of<T, 32>(p, c, row, head);
+    attend_row_of<T, 8>(p, c, row, head, until);
 }
 
 // Whether a non-finite value of the KV head lies at a position that the row does not see, but

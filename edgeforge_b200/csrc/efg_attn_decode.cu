@@ -99,12 +99,12 @@ __device__ __forceinline__ bool store_row(const AttnParams& p, const Rows& w, in
 // Rows marked in `redo` once more, alone, where something behind their last position reached them.
 // One warp.
 template <typename T>
-__device__ __forceinline__ void redo_rows(const AttnParams& p, const Rows& w, int kvh, const int* redo) {
+__device__ __forceinline__ void redo_rows(const AttnParams& p, const Rows& w, int kvh, const int* redo, uint64_t* until = nullptr) {
   for (int r = 0; r < w.rows; ++r) {
     const int token = r / p.group;
     if (redo[r] && seen_by(w.c, w.c.begin + token) < w.see_all &&
         reached_from_behind<T>(p, w.c, w.c.begin + token, kvh, w.see_all))
-      attend_row<T>(p, w.c, w.c.begin + token, kvh * p.group + r - token * p.group);
+      attend_row<T>(p, w.c, w.c.begin + token, kvh * p.group + r - token * p.group, until);
   }
 }
 
@@ -193,10 +193,12 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
   __shared__ float top_s[kConsumers][16], sum_s[kConsumers][16];
   __shared__ int scan_s[kThreads / 32], place_s[2];
   __shared__ int redo_s[16];
+  __shared__ uint64_t until_s;  // waits go on until then (wait_own)
   const AttnParams& p = dp.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const bool cut = dp.slots != nullptr;
   if (tid == 32 * kConsumers) {
+    until_s = 0;
     prefetch_map(&map_k);
     prefetch_map(&map_v);
     for (int i = 0; i < S::kStages; ++i) {
@@ -269,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
       for (int tile = walk.from; tile < walk.to; ++tile) {
         const int st = it % S::kStages;
         const int32_t next = row_of(tile + 1);
-        if (it >= S::kStages) ok = wait_own(&empty[st], ((it / S::kStages) - 1) & 1, p.err);
+        if (it >= S::kStages) ok = wait_own(&empty[st], ((it / S::kStages) - 1) & 1, p.err, &until_s);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&full[st], 2 * S::kTileBytes);
@@ -285,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
       }
     }
     if (!ok)  // the copies in flight land before the shared memory is given back
-      for (int i = max(0, it - S::kStages); i < it; ++i) wait_own(&full[i % S::kStages], (i / S::kStages) & 1, p.err);
+      for (int i = max(0, it - S::kStages); i < it; ++i) wait_own(&full[i % S::kStages], (i / S::kStages) & 1, p.err, &until_s);
     return;
   }
 
@@ -347,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
 
     for (int tile = walk.from; tile < walk.to; ++tile, ++it) {
       const int st = it % S::kStages;
-      if (ok) ok = wait_own(&full[st], (it / S::kStages) & 1, p.err);
+      if (ok) ok = wait_own(&full[st], (it / S::kStages) & 1, p.err, &until_s);
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) continue;  // a wait gave up (recorded): no more work, but every barrier below is met
       const uint32_t ks = base + static_cast<uint32_t>(st) * (2 * S::kTileBytes), vs = ks + S::kTileBytes;
@@ -601,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
     }
     if (uneven) {
       consumer_barrier();
-      if (warp == 0) redo_rows<T>(p, w, kvh, redo_s);
+      if (warp == 0) redo_rows<T>(p, w, kvh, redo_s, &until_s);
     }
     if (warp == 0) {
       if (!whole && walk.from == 0) {  // a key head that is cut begins here: its last piece is in another run

@@ -404,6 +404,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
   int* scan_s = reinterpret_cast<int*>(unit_s);  // (before the roles begin)
   __shared__ Item items[2];
   __shared__ uint32_t tmem_slot;
+  __shared__ uint64_t until_s;  // waits go on until then (wait_own)
   const AttnParams& p = tp.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t raw = smem_addr(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -434,6 +435,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
       mbar_init(&stage_empty[i], 128);
     }
     for (int i = 0; i < 8; ++i) mbar_init(&exp_full[i], 1);
+    until_s = 0;
     fence_barrier_init();
   }
   if (warp == 9) tmem_alloc(&tmem_slot, 512);
@@ -488,7 +490,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
   int turn = 0;
   auto next_item = [&](Item& w) {
     const int slot = turn & 1;
-    const bool ok = __all_sync(0xFFFFFFFFu, wait_own(&item_full[slot], (turn >> 1) & 1, p.err));
+    const bool ok = __all_sync(0xFFFFFFFFu, wait_own(&item_full[slot], (turn >> 1) & 1, p.err, &until_s));
     if (!ok) return false;
     w = items[slot];
     ++turn;
@@ -515,7 +517,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
           if (lane == 0) mbar_arrive(&fetch);
           continue;
         }
-        if (!kF32 && tiles > 0) ok = wait_own(&q_empty, (tiles - 1) & 1, p.err);
+        if (!kF32 && tiles > 0) ok = wait_own(&q_empty, (tiles - 1) & 1, p.err, &until_s);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;
         ++tiles;
@@ -541,7 +543,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
           if (j == max(0, w.count - 2) && lane == 0) mbar_arrive(&fetch);  // time to look for the next item
           for (int kv = 0; kv < 2 && ok; ++kv) {
             const int st = issued % kIn;
-            if (issued >= kIn) ok = wait_own(&in_empty[st], ((issued / kIn) - 1) & 1, p.err);
+            if (issued >= kIn) ok = wait_own(&in_empty[st], ((issued / kIn) - 1) & 1, p.err, &until_s);
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) break;
             if (lane == 0) mbar_arrive_expect_tx(&in_full[st], kTileBytes);
@@ -555,8 +557,8 @@ __global__ void __launch_bounds__(threads<T>, 1)
         }
       }
       // the copies in flight land before the shared memory is given back (all have, unless a wait gave up)
-      if (!kF32 && tiles > 0) wait_own(&q_full, (tiles - 1) & 1, p.err);
-      for (int i = max(0, issued - kIn); i < issued; ++i) wait_own(&in_full[i % kIn], (i / kIn) & 1, p.err);
+      if (!kF32 && tiles > 0) wait_own(&q_full, (tiles - 1) & 1, p.err, &until_s);
+      for (int i = max(0, issued - kIn); i < issued; ++i) wait_own(&in_full[i % kIn], (i / kIn) & 1, p.err, &until_s);
     } else if (warp == 9 || (kApart && warp == 11)) {
       // -------------------------------------------------------------- MMA
       // Where P lies apart, each row tile has a warp of its own (9 and 11): a softmax that is ready is never
@@ -611,7 +613,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
       };
       // The tile has landed. (A stage is given back only after that, also by a row tile that has no use for it:
       // the other one's use of the stage before is over then.)
-      auto landed = [&](int item) { return wait_own(&kv_full[item % kStages], (item / kStages) & 1, p.err); };
+      auto landed = [&](int item) { return wait_own(&kv_full[item % kStages], (item / kStages) & 1, p.err, &until_s); };
       Item w;
       bool ok = true;
       int ring_at = 0, tiles = 0;     // ring items and items with keys before this one
@@ -622,13 +624,13 @@ __global__ void __launch_bounds__(threads<T>, 1)
         int n[kMine];
 #pragma unroll
         for (int x = 0; x < kMine; ++x) n[x] = kApart && mine == 1 ? a.n[1] : a.n[x];
-        ok = wait_own(&q_full, tiles & 1, p.err) && landed(ring_at);
+        ok = wait_own(&q_full, tiles & 1, p.err, &until_s) && landed(ring_at);
         ++tiles;
 #pragma unroll
         for (int x = 0; x < kMine; ++x) {
           if (n[x] == 0) continue;
           // S of the item before has been read (where P lies in S, its value product precedes these MMAs)
-          if (kApart && step[x] > 0) ok = ok && wait_own(&s_free[mine + x], (step[x] - 1) & 1, p.err);
+          if (kApart && step[x] > 0) ok = ok && wait_own(&s_free[mine + x], (step[x] - 1) & 1, p.err, &until_s);
           if (!ok) continue;
           tc_fence_after();
           scores(mine + x, ring_at);
@@ -642,7 +644,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
           if (kApart && more) {
             ok = landed(ki);
             if (j + 1 < n[0]) {
-              ok = ok && wait_own(&s_free[mine], (step[0] + j) & 1, p.err);
+              ok = ok && wait_own(&s_free[mine], (step[0] + j) & 1, p.err, &until_s);
               if (!ok) break;
               tc_fence_after();
               scores(mine, ki);
@@ -655,7 +657,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
 #pragma unroll
           for (int x = 0; x < kMine; ++x) {
             if (j >= n[x]) continue;
-            ok = ok && wait_own(&p_ready[mine + x], (step[x] + j) & 1, p.err);
+            ok = ok && wait_own(&p_ready[mine + x], (step[x] + j) & 1, p.err, &until_s);
             if (!ok) continue;
             tc_fence_after();
             values(mine + x, vi, j > 0);
@@ -693,8 +695,8 @@ __global__ void __launch_bounds__(threads<T>, 1)
           asm volatile("" : "+r"(r));
           const int quad = r & 15, row0 = (r >> 4) * 16;
           const int st = at % kStaging, op = at % kStages, keys = a.see_all - (w.first + (x >> 1)) * kTileKeys;
-          ok = wait_own(&stage_full[st], (at / kStaging) & 1, p.err);
-          if (ok && at >= kStages) ok = wait_own(&kv_empty[op], ((at / kStages) - 1) & 1, p.err);
+          ok = wait_own(&stage_full[st], (at / kStaging) & 1, p.err, &until_s);
+          if (ok && at >= kStages) ok = wait_own(&kv_empty[op], ((at / kStages) - 1) & 1, p.err, &until_s);
           uint8_t *src = stage + st * kTileBytes, *dst = ring + op * kTileBytes;
           auto chunk = [&](int row, int c) {
             return *reinterpret_cast<const float4*>(src + row * 128 + (c >> 3) * kPanel + (((c & 7) ^ (row & 7)) << 4));
@@ -830,7 +832,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
       bool ok = true;
       auto send = [&](const Item& w) {
         const int slot = sent & 1;
-        if (sent >= 2) ok = wait_own(&item_empty[slot], ((sent >> 1) - 1) & 1, p.err);
+        if (sent >= 2) ok = wait_own(&item_empty[slot], ((sent >> 1) - 1) & 1, p.err, &until_s);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) return;
         if (lane == 0) {
@@ -889,7 +891,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
             ask_next_cta(&answer, &asked);
           }
           __syncwarp();
-          ok = __all_sync(0xFFFFFFFFu, wait_own(&asked, asks & 1, p.err));
+          ok = __all_sync(0xFFFFFFFFu, wait_own(&asked, asks & 1, p.err, &until_s));
           ++asks;
           if (!ok) return -1;
           const int x = next_cta(&answer);
@@ -934,7 +936,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
           w.count = tiles_of_pair(w.c, w.token0, pair_tokens);
           w.slot = -1;
           send(w);
-          if (ok) ok = __all_sync(0xFFFFFFFFu, wait_own(&fetch, (sent - 1) & 1, p.err));
+          if (ok) ok = __all_sync(0xFFFFFFFFu, wait_own(&fetch, (sent - 1) & 1, p.err, &until_s));
         }
       }
       if (ok) {
@@ -960,7 +962,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
     for (;; ++turn) {
       const int slot = turn & 1;
       // (read again where needed: the registers are for S)
-      ok = ok && __all_sync(0xFFFFFFFFu, wait_own(&item_full[slot], (turn >> 1) & 1, p.err));
+      ok = ok && __all_sync(0xFFFFFFFFu, wait_own(&item_full[slot], (turn >> 1) & 1, p.err, &until_s));
       if (!ok || items[slot].stop) break;
       int n, first, count, see_all, sees, see_first;
       {
@@ -980,7 +982,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
       float acc[kF32 ? D : 1] = {};  // F32: O of the key tiles before
       if (kF32 && count > 0) {
         // this row's query, scaled by a power of two, as the hi and lo rows of the Q operand
-        if (tiles > 0) ok = ok && wait_own(&q_empty, (tiles - 1) & 1, p.err);
+        if (tiles > 0) ok = ok && wait_own(&q_empty, (tiles - 1) & 1, p.err, &until_s);
         const int64_t row = items[slot].c.begin + items[slot].token0 + i * tp.tokens + token;
         const int head = items[slot].kvh * p.group + r - token * p.group;
         const bool live = token < plan_of(items[slot], tp.tokens).tok[i];
@@ -1032,7 +1034,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
           }
         };
         for (int j = 0; j < n; ++j, ++step) {
-          ok = ok && wait_own(&s_full[i], step & 1, p.err);
+          ok = ok && wait_own(&s_full[i], step & 1, p.err, &until_s);
           if (!__all_sync(0xFFFFFFFFu, ok)) break;
           tc_fence_after();
           const int key0 = (first + j) * kTileKeys;
@@ -1061,7 +1063,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
               for (int q = 0; q < 4; ++q) mx[q] = max3(mx[q], __uint_as_float(s[k + q]), __uint_as_float(s[k + q + 4]));
           }
           const int ki = ring_at + 2 * j;
-          ok = wait_own(&exp_full[ki & 7], (ki >> 3) & 1, p.err);
+          ok = wait_own(&exp_full[ki & 7], (ki >> 3) & 1, p.err, &until_s);
           high_k = max(high_k, exp_s[ki & 7]);
           const float factor = scale2 * power_of_two(max(-120, min(120, exp_q + exp_s[ki & 7] - 2 * kTop)));
           const float high = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * factor;
@@ -1073,8 +1075,8 @@ __global__ void __launch_bounds__(threads<T>, 1)
             if (move) ref = high;
             total[0] = fma2(total[0], pair(back, back), 0);
             total[1] = fma2(total[1], pair(back, back), 0);
-            ok = ok && wait_own(&pv_done[i], (step - 1) & 1, p.err) &&
-                 wait_own(&exp_full[(ki - 1) & 7], ((ki - 1) >> 3) & 1, p.err);  // (its units; long there)
+            ok = ok && wait_own(&pv_done[i], (step - 1) & 1, p.err, &until_s) &&
+                 wait_own(&exp_full[(ki - 1) & 7], ((ki - 1) >> 3) & 1, p.err, &until_s);  // (its units; long there)
             if (!__all_sync(0xFFFFFFFFu, ok)) break;
             tc_fence_after();
             take(j - 1, back);
@@ -1098,11 +1100,11 @@ __global__ void __launch_bounds__(threads<T>, 1)
         }
         if (n > 0) {
           const int own = ring_at + 2 * n - 1, last = ring_at + 2 * count - 1;  // the item's last value tile: wide_s stands
-          ok = ok && wait_own(&pv_done[i], (step - 1) & 1, p.err) && wait_own(&exp_full[own & 7], (own >> 3) & 1, p.err);
+          ok = ok && wait_own(&pv_done[i], (step - 1) & 1, p.err, &until_s) && wait_own(&exp_full[own & 7], (own >> 3) & 1, p.err, &until_s);
           ok = __all_sync(0xFFFFFFFFu, ok);
           tc_fence_after();
           take(n - 1, 1.f);
-          ok = ok && wait_own(&exp_full[last & 7], (last >> 3) & 1, p.err);
+          ok = ok && wait_own(&exp_full[last & 7], (last >> 3) & 1, p.err, &until_s);
           ok = __all_sync(0xFFFFFFFFu, ok);
         }
         coarse = p.scale * power_of_two(max(-126, min(127, exp_q + high_k))) > kScoreRange;
@@ -1127,7 +1129,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
         }
       } else {
         for (int j = 0; j < n; ++j, ++step) {
-          ok = wait_own(&s_full[i], step & 1, p.err);
+          ok = wait_own(&s_full[i], step & 1, p.err, &until_s);
           if (!__all_sync(0xFFFFFFFFu, ok)) break;
           tc_fence_after();
           uint32_t s[128];
@@ -1159,7 +1161,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
           const float high = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
           // P and O of the key tile before are free once its value product is done
           const auto before_done = [&] {
-            if (j > 0) ok = ok && wait_own(&pv_done[i], (step - 1) & 1, p.err);
+            if (j > 0) ok = ok && wait_own(&pv_done[i], (step - 1) & 1, p.err, &until_s);
             tc_fence_after();
           };
           if (j == 0) {
@@ -1202,7 +1204,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
             // values behind the last position: whatever lies there would meet weights of zero, and 0 times
             // infinity is NaN, so it becomes zero
             const int item = ring_at + 2 * j + 1, st = item % kStages;
-            ok = wait_own(&kv_full[st], (item / kStages) & 1, p.err);
+            ok = wait_own(&kv_full[st], (item / kStages) & 1, p.err, &until_s);
             if (ok && key0 + r >= see_all) {
 #pragma unroll
               for (int h = 0; h < kPanels; ++h) {
@@ -1223,7 +1225,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
       float ta, tb;
       unpair(add2(total[0], total[1]), ta, tb);
       const float row_sum = kF32 ? (ta + tb) * power_of_two(-kRaise) : ta + tb;
-      if (!kF32 && ok && n > 0) ok = wait_own(&pv_done[i], (step - 1) & 1, p.err);
+      if (!kF32 && ok && n > 0) ok = wait_own(&pv_done[i], (step - 1) & 1, p.err, &until_s);
       tc_fence_after();
       ok = __all_sync(0xFFFFFFFFu, ok);
       const Item w = items[slot];
@@ -1281,7 +1283,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
           const int64_t row_l = __shfl_sync(0xFFFFFFFFu, row, l);
           const int head_l = __shfl_sync(0xFFFFFFFFu, head, l);
           if ((again >> l & 1) || reached_from_behind<T>(p, w.c, row_l, w.kvh, see_all))
-            attend_row<T>(p, w.c, row_l, head_l);
+            attend_row<T>(p, w.c, row_l, head_l, &until_s);
         }
       } else {
         // a piece: row `tid` of the slot; 16-byte pieces of the rows lie side by side, so that a warp's stores do

@@ -130,3 +130,23 @@ def test_a_value_far_below_the_others_of_its_dim(cuda):
         v[:30, :, d] *= small
     v[60:90, :, 5] = 0
     _check(torch, q, k, v)
+
+
+def test_rows_that_take_longer_alone_than_a_wait_may(cuda):
+    """The last rows of a long prompt see a key far above the others and are computed alone, one after another (32 a
+    warp, about 3 s; a wait gives up after 2): the rest of the CTA waits for them, and every row is there."""
+    import torch
+
+    n, dim = 2**19, 64
+    g = torch.Generator(device="cuda").manual_seed(36)
+    q, k, v = (torch.randn(n, 1, dim, generator=g, device="cuda") for _ in range(3))
+    k[n - 130] = 1e8
+    out = torch.full_like(q, float("nan"))
+    efg.attn_prompt(out, q, k, v, _i(torch, [0, n]))
+    torch.cuda.synchronize()
+    assert efg.device_error() == 0
+    assert torch.isfinite(out).all()
+    scale = float(np.float32(dim**-0.5))
+    for r in (5, 1000, 300001, n - 300, n - 131, n - 130, n - 77, n - 1):
+        want = attend(_d(q[r : r + 1]), _d(k[: r + 1]), _d(v[: r + 1]), scale)
+        _held(_d(out[r : r + 1]), *want)
