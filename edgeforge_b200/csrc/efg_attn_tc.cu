@@ -29,12 +29,13 @@
 // (paged chunks) the work is one line of key tiles cut into equal runs, and a second launch joins the
 // rows of items that were cut, in order.
 //
-// F32 (16 warps; registers 2 x 128 x 200 and 2 x 128 x 56 of 512 x 128): TMA brings FP32 tiles, four converter warps
+// F32 (16 warps; registers 2 x 128 x 160 and 2 x 128 x 96 of 512 x 128): TMA brings FP32 tiles, four converter warps
 // (12-15) turn each into two F16 tiles hi + lo, scaled by a power of two (keys: one for the tile, values: one for each
 // dim), and S = Qh Kh + Qh Kl + Ql Kh, O = Ph [Vh | Vl] + Pl Vh in the same instructions, with P split as well. O of each
-// key tile begins at zero and is added up in the softmax threads' registers, in FP32. Bound by the converters: 2048
-// tokens, 32 query and 4 key heads of 64: 133 us (in TF32 parts on the warp-level tensor cores: 436; with one scale for
-// a tile's values, which takes the digits of small dims beside large ones: 121); error of a row 4.4e-7.
+// key tile begins at zero and is added up in the softmax threads' registers, in FP32. Bound by the converters and by
+// what spills to local memory (L1 is all shared memory here): S is read 32 columns at a time in loops that stay loops
+// (unrolled: 131 us). 2048 tokens, 32 query and 4 key heads of 64: 118 us (in TF32 parts on the warp-level tensor
+// cores: 436); error of a row 4.4e-7.
 #include <algorithm>
 
 #include <cuda_runtime.h>
@@ -312,7 +313,13 @@ __device__ __forceinline__ void load_o(uint32_t addr, uint32_t (&o)[32]) {
     after_wait(o);
     after_wait(lo);
 #pragma unroll
-    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(fmaf(__uint_as_float(lo[e]), 1.f / kLoUp, __uint_as_float(o[e])));
+    for (int e = 0; e < 32; e += 2) {
+      float a, b;
+      unpair(fma2(pair(__uint_as_float(lo[e]), __uint_as_float(lo[e + 1])), pair(1.f / kLoUp, 1.f / kLoUp),
+                  pair(__uint_as_float(o[e]), __uint_as_float(o[e + 1]))), a, b);
+      o[e] = __float_as_uint(a);
+      o[e + 1] = __float_as_uint(b);
+    }
   } else {
     tmem_wait_ld();
     after_wait(o);
@@ -500,7 +507,10 @@ __global__ void __launch_bounds__(threads<T>, 1)
   };
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if constexpr (kF32)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    else
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 8) {
       // -------------------------------------------------------------- TMA
       const int boxes = kTileKeys / tp.box_rows, b = lane % boxes, panel = lane / boxes;
@@ -599,15 +609,15 @@ __global__ void __launch_bounds__(threads<T>, 1)
       auto values = [&](int i, int item, uint32_t add) {
         const uint64_t dv = desc_values(ring_addr + (item % kStages) * kTileBytes);
         const uint32_t o = kColO + kWideO * i, pp = kColP + kStepP * i;
-        // F32: P hi times [V hi | V lo], then P lo times V hi onto the columns of the small products; of each half of
-        // the keys P hi lies in 32 columns and P lo in the next 32
-        const auto col = [&](int ks) { return pp + (kF32 ? (ks / 4) * 64 + (ks % 4) * 8 : 8 * ks); };
+        // F32: P hi times [V hi | V lo], then P lo times V hi onto the columns of the small products; of every 32
+        // keys P hi lies in 16 columns and P lo in the next 16
+        const auto col = [&](int ks) { return pp + (kF32 ? (ks / 2) * 32 + (ks % 2) * 8 : 8 * ks); };
         mma_ts(one, o, pp, dv, id_o, kF32 ? 0u : add);
 #pragma unroll
         for (int ks = 1; ks < kTileKeys / 16; ++ks) mma_ts(one, o, col(ks), dv + ks * (2048 >> 4), id_o, 1u);
         if constexpr (kF32) {
 #pragma unroll
-          for (int ks = 0; ks < kTileKeys / 16; ++ks) mma_ts(one, o + 64, col(ks) + 32, dv + ks * (2048 >> 4), id_half, 1u);
+          for (int ks = 0; ks < kTileKeys / 16; ++ks) mma_ts(one, o + 64, col(ks) + 16, dv + ks * (2048 >> 4), id_half, 1u);
         }
         commit_if(one, &pv_done[i]);
       };
@@ -702,21 +712,23 @@ __global__ void __launch_bounds__(threads<T>, 1)
             return *reinterpret_cast<const float4*>(src + row * 128 + (c >> 3) * kPanel + (((c & 7) ^ (row & 7)) << 4));
           };
           if (x & 1) {
-            if (keys < kTileKeys) {
-              if (ok && r >= keys) {
+            if (ok && r >= keys) {  // (in order by the barrier before these rows are read)
 #pragma unroll 1
-                for (int c = 0; c < 16; ++c)
-                  *reinterpret_cast<uint4*>(src + r * 128 + (c >> 3) * kPanel + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
-              }
-              ok = all_converters(ok);
-              if (!ok) break;
+              for (int c = 0; c < 16; ++c)
+                *reinterpret_cast<uint4*>(src + r * 128 + (c >> 3) * kPanel + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
             }
             float4 hi = make_float4(0, 0, 0, 0), lo = make_float4(INFINITY, INFINITY, INFINITY, INFINITY);
-#pragma unroll
-            for (int k = 0; k < 16; k += 2) {
-              const float4 v = chunk(row0 + k, quad), u = chunk(row0 + k + 1, quad);
+            const auto range = [&](const float4& v, const float4& u) {
               hi = make_float4(max3_abs(hi.x, v.x, u.x), max3_abs(hi.y, v.y, u.y), max3_abs(hi.z, v.z, u.z), max3_abs(hi.w, v.w, u.w));
               lo = make_float4(min3_abs(lo.x, v.x, u.x), min3_abs(lo.y, v.y, u.y), min3_abs(lo.z, v.z, u.z), min3_abs(lo.w, v.w, u.w));
+            };
+            if (keys >= kTileKeys) {
+#pragma unroll
+              for (int k = 0; k < 16; k += 2) range(chunk(row0 + k, quad), chunk(row0 + k + 1, quad));
+            } else {  // the last valid row in place of those behind it
+#pragma unroll 2
+              for (int k = 0; k < 16; k += 2)
+                range(chunk(min(row0 + k, keys - 1), quad), chunk(min(row0 + k + 1, keys - 1), quad));
             }
             if (lo.x == 0.f || lo.y == 0.f || lo.z == 0.f || lo.w == 0.f) {  // the least but zero
               lo = make_float4(INFINITY, INFINITY, INFINITY, INFINITY);
@@ -724,7 +736,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
               if (hi.x != 0.f || hi.y != 0.f || hi.z != 0.f || hi.w != 0.f) {
 #pragma unroll 1
                 for (int k = 0; k < 16; ++k) {
-                  const float4 v = chunk(row0 + k, quad);
+                  const float4 v = chunk(min(row0 + k, keys - 1), quad);
                   lo = make_float4(some(lo.x, v.x), some(lo.y, v.y), some(lo.z, v.z), some(lo.w, v.w));
                 }
               }
@@ -947,7 +959,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
   } else {
     // ---------------------------------------------------------------- softmax
     if constexpr (kF32)
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
     else
       asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int i = warp >> 2, r = tid & 127;
@@ -979,7 +991,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
       uint64_t total[2] = {0, 0};  // pairs of FP32 zeros
       float ref = 0.f;
       int exp_q = 0;                // F32: exponent of this row's query
-      float acc[kF32 ? D : 1] = {};  // F32: O of the key tiles before
+      uint64_t acc[kF32 ? D / 2 : 1] = {};  // F32: O of the key tiles before, pairs
       if (kF32 && count > 0) {
         // this row's query, scaled by a power of two, as the hi and lo rows of the Q operand
         if (tiles > 0) ok = ok && wait_own(&q_empty, (tiles - 1) & 1, p.err, &until_s);
@@ -1013,11 +1025,12 @@ __global__ void __launch_bounds__(threads<T>, 1)
       bool coarse = false;  // F32: a row that is computed again
       if constexpr (kF32) {
         // O of one key tile at a time is added up here, in registers: the tensor cores' accumulators cut off instead
-        // of rounding, which over a long row would shrink it (by 5e-6 at 8192 keys). S is read by halves
+        // of rounding, which over a long row would shrink it (by 5e-6 at 8192 keys). S is read 32 columns at a time
         // to leave room for that.
         int high_k = -126;
         const auto take = [&](int j, float back) {  // O of key tile j
           const float4* units = unit_s[(ring_at / 2 + j) % 3];
+          const uint64_t backs = pair(back, back);
 #pragma unroll
           for (int q = 0; q < D / 32; ++q) {
             uint32_t o[32];
@@ -1025,11 +1038,9 @@ __global__ void __launch_bounds__(threads<T>, 1)
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
               const float4 u = units[8 * q + e / 4];
-              float* a = acc + 32 * q + e;
-              a[0] = fmaf(__uint_as_float(o[e]), u.x, a[0]) * back;
-              a[1] = fmaf(__uint_as_float(o[e + 1]), u.y, a[1]) * back;
-              a[2] = fmaf(__uint_as_float(o[e + 2]), u.z, a[2]) * back;
-              a[3] = fmaf(__uint_as_float(o[e + 3]), u.w, a[3]) * back;
+              uint64_t* a = acc + 16 * q + e / 2;
+              a[0] = fma2(fma2(pair(__uint_as_float(o[e]), __uint_as_float(o[e + 1])), pair(u.x, u.y), a[0]), backs, 0);
+              a[1] = fma2(fma2(pair(__uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])), pair(u.z, u.w), a[1]), backs, 0);
             }
           }
         };
@@ -1040,27 +1051,25 @@ __global__ void __launch_bounds__(threads<T>, 1)
           const int key0 = (first + j) * kTileKeys;
           const bool edge = key0 + kTileKeys > see_first;
           const int limit = sees - key0;
-          uint32_t s[64];
-          const auto load = [&](int h) {
-            tmem_ld32(s_addr + 64 * h, s);
-            tmem_ld32(s_addr + 64 * h + 32, s + 32);
+          uint32_t s[32];
+          const auto load = [&](int q) {  // columns 32 q ..
+            tmem_ld32(s_addr + 32 * q, s);
             tmem_wait_ld();
             after_wait(s);
-            after_wait(s + 32);
             if (edge) {
 #pragma unroll
-              for (int k = 0; k < 64; ++k)
-                if (k + 64 * h >= limit) s[k] = 0xFF800000u;  // -inf
+              for (int k = 0; k < 32; ++k)
+                if (k + 32 * q >= limit) s[k] = 0xFF800000u;  // -inf
             }
           };
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q) {
+            load(q);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            load(h);
+            for (int k = 0; k < 32; k += 8)
 #pragma unroll
-            for (int k = 0; k < 64; k += 8)
-#pragma unroll
-              for (int q = 0; q < 4; ++q) mx[q] = max3(mx[q], __uint_as_float(s[k + q]), __uint_as_float(s[k + q + 4]));
+              for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(s[k + e]), __uint_as_float(s[k + e + 4]));
           }
           const int ki = ring_at + 2 * j;
           ok = wait_own(&exp_full[ki & 7], (ki >> 3) & 1, p.err, &until_s);
@@ -1082,16 +1091,13 @@ __global__ void __launch_bounds__(threads<T>, 1)
             take(j - 1, back);
           }
           const uint64_t scale_pair = pair(factor, factor), nref = pair(-ref, -ref);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {  // (P takes the place of the half of S that has been read)
-            load(h);
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              uint32_t hi[16], lo[16];
-              weights32_split(s + 32 * q, scale_pair, nref, total, hi, lo);
-              tmem_st16(p_addr + 64 * h + 16 * q, hi);
-              tmem_st16(p_addr + 64 * h + 32 + 16 * q, lo);
-            }
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q) {  // (P takes the place of the columns of S that have been read)
+            load(q);
+            uint32_t hi[16], lo[16];
+            weights32_split(s, scale_pair, nref, total, hi, lo);
+            tmem_st16(p_addr + 32 * q, hi);
+            tmem_st16(p_addr + 32 * q + 16, lo);
           }
           if (!__all_sync(0xFFFFFFFFu, ok)) break;
           tmem_wait_st();
@@ -1115,15 +1121,18 @@ __global__ void __launch_bounds__(threads<T>, 1)
             float ta, tb;
             unpair(add2(total[0], total[1]), ta, tb);
             const float sum = (ta + tb) * power_of_two(-kRaise);
-            const auto far = [&](uint32_t four, const float* acc) {
+            const auto far = [&](uint32_t four, const uint64_t* acc) {
+              float x[4];
+              unpair(acc[0], x[0], x[1]);
+              unpair(acc[1], x[2], x[3]);
 #pragma unroll
               for (int y = 0; y < 4; ++y)  // (a bound of 0 holds for none)
-                coarse = coarse || fabsf(acc[y]) < sum * __uint_as_float((four >> (8 * y) & 255u) << 23);
+                coarse = coarse || fabsf(x[y]) < sum * __uint_as_float((four >> (8 * y) & 255u) << 23);
             };
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const uint4 w = e == 0 ? a : e == 1 ? b : e == 2 ? c : d;
-              far(w.x, acc + 16 * e), far(w.y, acc + 16 * e + 4), far(w.z, acc + 16 * e + 8), far(w.w, acc + 16 * e + 12);
+              far(w.x, acc + 8 * e), far(w.y, acc + 8 * e + 2), far(w.z, acc + 8 * e + 4), far(w.w, acc + 8 * e + 6);
             }
           }
         }
@@ -1244,11 +1253,10 @@ __global__ void __launch_bounds__(threads<T>, 1)
 #pragma unroll
             for (int e = 0; e < D; e += 4) {
               float v[4];
+              unpair(fma2(acc[e / 2], pair(inv, inv), 0), v[0], v[1]);
+              unpair(fma2(acc[e / 2 + 1], pair(inv, inv), 0), v[2], v[3]);
 #pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                v[y] = acc[e + y] * inv;
-                finite = finite && fabsf(v[y]) <= 3.402823466e38f;
-              }
+              for (int y = 0; y < 4; ++y) finite = finite && fabsf(v[y]) <= 3.402823466e38f;
               if (e < p.head_dim) *reinterpret_cast<float4*>(out + e) = make_float4(v[0], v[1], v[2], v[3]);
             }
           }
@@ -1296,9 +1304,12 @@ __global__ void __launch_bounds__(threads<T>, 1)
         if constexpr (kF32) {
           if (live) {
 #pragma unroll
-            for (int e = 0; e < D / 4; ++e)
-              *reinterpret_cast<float4*>(slot_o + 512 + (e * 256 + tid) * 4) =
-                  make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
+            for (int e = 0; e < D / 4; ++e) {
+              float x[4];
+              unpair(acc[2 * e], x[0], x[1]);
+              unpair(acc[2 * e + 1], x[2], x[3]);
+              *reinterpret_cast<float4*>(slot_o + 512 + (e * 256 + tid) * 4) = make_float4(x[0], x[1], x[2], x[3]);
+            }
           }
         } else {
 #pragma unroll 1
