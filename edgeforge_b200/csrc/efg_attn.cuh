@@ -116,8 +116,9 @@ __device__ __forceinline__ bool wait_own(uint64_t* bar, uint32_t parity, int* er
 #pragma unroll 1
   for (uint32_t i = 0;; ++i) {
     if (mbar_try_wait_sleep(bar, parity, 2000u)) return true;
-    if ((i & 15u) == 15u && globaltimer_ns() - t0 > kWaitTimeoutNs &&
-        globaltimer_ns() > *reinterpret_cast<const volatile uint64_t*>(until)) {
+    if ((i & 15u) != 15u) continue;
+    const uint64_t now = globaltimer_ns();
+    if (now - t0 > kWaitTimeoutNs && now > *reinterpret_cast<const volatile uint64_t*>(until)) {
       record_error(err, EFG_ETIMEOUT);
       return false;
     }

@@ -21,7 +21,7 @@ struct PlanParams {
   int32_t* table;
   int32_t *slots, *positions, *cu, *kv_len, *taken;
   const int32_t *cached, *fresh, *free;
-  int64_t max_pages, n_rows, n_seqs, n_free, n_pages, page_size, rows_per_cta;
+  int64_t max_pages, n_rows, n_seqs, n_free, n_pages, page_size, most, rows_per_cta;  // most: positions of a sequence
   int* checks;
 };
 
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanParam
     }
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
-      n[i] = seq_need_held(cached[i], fresh[i], p.page_size, p.max_pages);
+      n[i] = seq_need_upto(cached[i], fresh[i], p.page_size, p.most);
       mine = mine + Pair64{n[i].rows, n[i].need};
     }
     Pair64 total;
@@ -325,6 +325,7 @@ int efg_page_plan(const efg_page_plan_args* args, void* stream) {
   p.n_free = static_cast<int64_t>(n_free);
   p.n_pages = static_cast<int64_t>(n_pages);
   p.page_size = static_cast<int64_t>(page_size);
+  p.most = efg::most_positions(p.max_pages, p.page_size);
   p.checks = dev->d_checks;
   const size_t ctas = std::max<size_t>(1, std::min<size_t>(dev->sm_count, (n_rows + 511) / 512));
   p.rows_per_cta = static_cast<int64_t>((n_rows + ctas - 1) / ctas);

@@ -30,23 +30,30 @@ EFG_HD int64_t pages_for(uint32_t positions, uint32_t page_size) {
   return static_cast<int64_t>(whole) + (positions != whole * page_size);
 }
 
-EFG_HD SeqNeed seq_need(int32_t cached, int32_t fresh, int64_t page_size, int64_t max_pages) {
+// `most`: positions that a sequence may have.
+EFG_HD SeqNeed seq_need_upto(int32_t cached, int32_t fresh, int64_t page_size, int64_t most) {
   SeqNeed n;
   n.rows = fresh > 0 ? fresh : 0;
   const int64_t end = static_cast<int64_t>(cached) + fresh;
-  n.valid = cached >= 0 && fresh >= 0 && end <= max_pages * page_size;
+  n.valid = cached >= 0 && fresh >= 0 && end <= most;
   // lengths fit 32 unsigned bits here, and a 32-bit division is a fraction of a 64-bit one
   n.have = n.valid ? pages_for(static_cast<uint32_t>(cached), static_cast<uint32_t>(page_size)) : 0;
   n.need = n.valid ? pages_for(static_cast<uint32_t>(end), static_cast<uint32_t>(page_size)) - n.have : 0;
   return n;
 }
 
-// The same for sequences whose lengths and positions other kernels hold in 32 signed bits (with room for a tile).
+EFG_HD SeqNeed seq_need(int32_t cached, int32_t fresh, int64_t page_size, int64_t max_pages) {
+  return seq_need_upto(cached, fresh, page_size, max_pages * page_size);
+}
+
+// Lengths and positions are held in 32 signed bits by the kernels that read them (with room for a tile).
 constexpr int64_t kMaxPositions = 0x7FFFFF00;
+EFG_HD int64_t most_positions(int64_t max_pages, int64_t page_size) {
+  const int64_t held = max_pages * page_size;
+  return held < kMaxPositions ? held : kMaxPositions;
+}
 EFG_HD SeqNeed seq_need_held(int32_t cached, int32_t fresh, int64_t page_size, int64_t max_pages) {
-  SeqNeed n = seq_need(cached, fresh, page_size, max_pages);
-  if (static_cast<int64_t>(cached) + fresh > kMaxPositions) n = SeqNeed{n.rows, 0, 0, false};
-  return n;
+  return seq_need_upto(cached, fresh, page_size, most_positions(max_pages, page_size));
 }
 
 // Fresh pages are handed out in sequence order. A sequence is served when its own pages end
