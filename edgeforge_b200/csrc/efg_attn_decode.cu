@@ -198,7 +198,6 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const bool cut = dp.slots != nullptr;
   if (tid == 32 * kConsumers) {
-    until_s = 0;
     prefetch_map(&map_k);
     prefetch_map(&map_v);
     for (int i = 0; i < S::kStages; ++i) {
@@ -209,6 +208,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
   }
   pdl_wait();
   pdl_launch_dependents();
+  if (tid == 0) move_on(&until_s);
 
   // ---- this CTA's run of the line: every thread adds up a block of sequences, then the one whose block
   // holds the run's beginning finds the sequence
@@ -271,6 +271,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kF32 && !kStack ? 2 : S
       for (int tile = walk.from; tile < walk.to; ++tile) {
         const int st = it % S::kStages;
         const int32_t next = row_of(tile + 1);
+        if (lane == 0) move_on(&until_s);
         if (it >= S::kStages) ok = wait_own(&empty[st], ((it / S::kStages) - 1) & 1, p.err, &until_s);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;

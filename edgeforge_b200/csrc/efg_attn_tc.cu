@@ -442,13 +442,13 @@ __global__ void __launch_bounds__(threads<T>, 1)
       mbar_init(&stage_empty[i], 128);
     }
     for (int i = 0; i < 8; ++i) mbar_init(&exp_full[i], 1);
-    until_s = 0;
     fence_barrier_init();
   }
   if (warp == 9) tmem_alloc(&tmem_slot, 512);
   // (the next launch may not begin early: its CTAs would take SMs from items that are still to be handed out, 120
   // against 127 us for 2048 FP32 tokens call after call)
   pdl_wait();
+  if (tid == 0) move_on(&until_s);
   if (!kRuns && tp.tiles_per_seq == 0 && blockIdx.x == 0) check_offsets(p);
   if constexpr (kRuns) {
     // This CTA's run of the line of all items' key tiles: every thread adds up a block of sequences, the one
@@ -550,6 +550,7 @@ __global__ void __launch_bounds__(threads<T>, 1)
         int32_t row = row_of(w.first);
         for (int j = 0; j < w.count && ok; ++j) {
           const int32_t next = row_of(w.first + j + 1);
+          if (lane == 0) move_on(&until_s);
           if (j == max(0, w.count - 2) && lane == 0) mbar_arrive(&fetch);  // time to look for the next item
           for (int kv = 0; kv < 2 && ok; ++kv) {
             const int st = issued % kIn;
