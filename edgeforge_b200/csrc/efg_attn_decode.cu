@@ -1,6 +1,6 @@
 // efg_attn_decode.cu - attention of at most 16 rows per key head (a decode step's head group, a few
 // drafted tokens): bound by reading the keys and values once. Measured: one BF16 row over 131072 positions,
-// 8 key heads of 128, 88 us, 6.1 TB/s; 64 FP32 rows over up to 4000 positions, 4 key heads of 64, 45 us, 4.1 TB/s,
+// 8 key heads of 128, 88-91 us, 5.9-6.1 TB/s; 64 FP32 rows over up to 4000 positions, 4 key heads of 64, 45 us, 4.1 TB/s,
 // where the TF32 splits take 42 % of the issue slots.
 //
 // The key tiles (64 positions) of all sequences and key heads form one line (each key head weighs its
@@ -36,8 +36,10 @@ namespace efg {
 namespace {
 
 constexpr int kConsumers = 4, kThreads = 32 * (kConsumers + 1);
-constexpr int kHeadCost = 2;   // what the begin and end of a key head cost, in key tiles
-constexpr int kMinRun = 3;     // weight of a run, at least
+// What the begin and end of a key head cost, in key tiles: 200 BF16 rows over 50 to 4000 positions, 8 key heads of
+// 128, 270 us (with a cost of 1: 302, of 4: 274). The weight of a run, at least: 16 rows over 8000 positions 94 us (of 1:
+// 93, of 6: 98), 512 rows over 300 positions 145 (147, 153).
+constexpr int kHeadCost = 2, kMinRun = 3;
 constexpr int kMaxCtas = 1024;
 
 template <typename T, int D>

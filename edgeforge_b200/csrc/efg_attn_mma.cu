@@ -44,7 +44,7 @@ template <typename T, int D>
 constexpr int stage_bytes() {
   return 2 * kKeys * D * static_cast<int>(sizeof(T));
 }
-// Bytes in flight per SM decide a decode step: about 96 KB in the stages of the CTAs that fit.
+// Calls of few rows wait for their loads: about 96 KB are in flight in the stages of the CTAs that fit on an SM.
 template <typename T, int D, int MT>
 constexpr int stages() {
   return stage_bytes<T, D>() <= 16384 ? 4 : MT > 4 ? 2 : 3;

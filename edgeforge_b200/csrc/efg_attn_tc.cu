@@ -15,8 +15,11 @@
 // What bounds it: at head size 128 the two products of a 128 x 128 tile take 1024 tensor-core cycles and
 // its 16384 exponentials 1024 cycles of the special function units, so neither may wait for the other;
 // at 64 the exponentials (and the instructions around them) are the bound. Measured: one 8192-token
-// prompt, 32 query and 8 key heads of 128, BF16: 490 us, 1120 TFLOP/s, 0.68 of the measured GEMM rate, the tensor
-// pipe and the exponentials' pipe busy for 54 % each. Measured and not kept: a part of the
+// prompt, 32 query and 8 key heads of 128, BF16: 550-565 us, 970-1000 TFLOP/s, in a run of seconds, where the clock
+// drops at the power cap; 480 us, 1145 TFLOP/s, in one of milliseconds, the tensor pipe and the exponentials' pipe busy
+// for 54 % each. P is rounded to the inputs' type, because A and B of an MMA have one type: a second
+// product for what that leaves out would take half of the tensor cores' time again. Error of that prompt's rows against
+// 64 bits 2.2e-3, of FP32 weights 1.7e-3 (the output's own rounding). Measured and not kept: a part of the
 // exponentials as a degree-4 polynomial on the FMA pipes (no gain at any share), turns at the
 // exponentials for the two warps of a scheduler (491 against 430 us at 64: one warp alone does not fill
 // the special function units), sums and packing one quarter behind the exponentials (540 against 486).
@@ -246,7 +249,8 @@ constexpr int kTop = 14;  // split operands are scaled so that their largest val
 // 2^(ev - 48) for every key that weighs less than 2^-26 (ev: exponent of the dim's largest value). Where every value of
 // the dim is zero or at least 2^(ev - 26), the first is below 2^-24 of sum w |v|, whatever the weights are. Where one is
 // not, rows with a sum below 2^(ev - 26) of the weights' are computed again: of normally distributed values a dim in
-// a thousand tiles, and then one row in ten thousand. (kTop + kRaise = 26: a dim's unit is that bound.)
+// a thousand tiles, and then one row in ten thousand. (kTop + kRaise = 26: a dim's unit is that bound.) The second is
+// left where the keys that weigh more have zeros in the dim: to look at these rows too costs 3 to 11 % without any zero.
 constexpr float kScoreRange = 65536.f;
 
 // Whether `ok` holds for all 128 converter threads; a barrier among them.
@@ -336,8 +340,10 @@ struct TcParams {
   int box_rows;       // rows of one key / value box
 };
 
-constexpr int kItemCost = 3;  // what the begin and end of an item cost, in key tiles
-constexpr int kMinRun = 4;    // weight of a run, at least
+// What the begin and end of an item cost, in key tiles, and the weight of a run, at least: not sharp. Chunks of 64 to 512
+// BF16 rows over 2000 to 65536 positions, alone and beside 255 single tokens, take the same within the noise (3 %) with a
+// cost of 1 or 6, and with runs of 2 or 8.
+constexpr int kItemCost = 3, kMinRun = 4;
 
 // A pair of row tiles of one key head, or a run of its key tiles, as the scheduler warp hands it to the roles.
 struct Item {
@@ -1471,8 +1477,11 @@ bool attn_tc_takes(int type, const AttnParams& p) {
 }
 
 size_t attn_tc_workspace(const AttnParams& p, int sms) {
-  // Prompts bring no workspace; many items keep the GPU busy without cutting any. The line's weight is a 32-bit
-  // number.
+  // Prompts bring no workspace. More than six items a CTA are not cut: where their lengths are alike that saves the
+  // pieces' way through memory (130 chunks of 100 tokens over 2000 positions, 8 key heads of 128: 553 us, cut 595; 255
+  // single tokens over 1000 positions beside 512 over 4000: 325, cut 352). One long item among short ones is then walked
+  // by one CTA a key head (64 tokens over 65536 positions beside 255 single ones over 200: 1090 us, cut 219); the
+  // host does not know the lengths. The line's weight is a 32-bit number.
   if (!p.kv_len) return 0;
   const int64_t max_new = std::min(p.max_new, p.n_rows), pair_tokens = 2 * (kTileRows / p.group);
   const int64_t tiles = std::min(p.n_seqs * ((max_new + pair_tokens - 1) / pair_tokens), p.n_rows / pair_tokens + p.n_seqs);

@@ -359,8 +359,9 @@ int efg_page_store(const efg_page_store_args* args, void* stream);
 /* Causal attention over packed prompts: row r of sequence s attends to rows d_cu[s] .. r.
  * out [n_rows][heads][head_dim] = softmax(scale q k^T) v, query head h reading key head
  * h / (heads / kv_heads). Inputs and output of one type; scores, softmax and sums in FP32 (F32
- * inputs keep FP32 accuracy; magnitudes below 2^127), the weights of 16-bit types rounded to the
- * type. head_dim up to 256. out must not overlap an input (EFG_EINVAL). Keys and values of rows
+ * inputs keep FP32 accuracy, weights below 2^-26 of a row's largest within 2^-48 of that; 8 times the
+ * number of positions times the largest magnitude stays below 2^127), the weights of 16-bit types
+ * rounded to the type. head_dim up to 256. out must not overlap an input (EFG_EINVAL). Keys and values of rows
  * that a row does not attend to never reach it, whatever they are; a row that attends to a NaN or
  * to an infinite key or value has no defined (finite or other) value. */
 typedef struct {

@@ -150,3 +150,20 @@ def test_rows_that_take_longer_alone_than_a_wait_may(cuda):
     for r in (5, 1000, 300001, n - 300, n - 131, n - 130, n - 77, n - 1):
         want = attend(_d(q[r : r + 1]), _d(k[: r + 1]), _d(v[: r + 1]), scale)
         _held(_d(out[r : r + 1]), *want)
+
+
+@pytest.mark.parametrize("share", [0.02, 0.5, 0.98])
+@pytest.mark.parametrize("m,n,dim,spread", [(200, 200, 64, 3.0), (129, 129, 60, 8.0), (150, 2700, 64, 8.0), (64, 64, 12, 8.0),
+                                            (90, 90, 128, 8.0), (3, 2800, 64, 8.0)])
+def test_values_with_zeros(cuda, share, m, n, dim, spread):
+    """Dims where the keys that weigh most have a value of zero: what keys of next to no weight add is all there is.
+    Weights are held within 2^-48 of the row's largest (include/efg.h), which over n keys is n 2^-48 max |v|."""
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(37)
+    q, k, v = (torch.randn(x, h, dim, generator=g, device="cuda") for x, h in ((m, 4), (n, 2), (n, 2)))
+    q = q * spread / dim**0.5 * 2
+    v[torch.rand(v.shape, generator=g, device="cuda") > share] = 0
+    out = _call(torch, q, k, v)
+    want = attend(_d(q), _d(k), _d(v), float(np.float32(dim**-0.5)))
+    assert (np.abs(out - want[0]) <= tolerance("f32", *want) + 2.0**-48 * want[3]).all()
